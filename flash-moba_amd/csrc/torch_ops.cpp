@@ -10,68 +10,21 @@
 // tensors, dispatch modes) or its arguments are not of the common form (non-contiguous last dimension, a head dimension
 // that has to be padded, empty sequences, anything the checks would reject): the caller then takes the path in Python,
 // which handles or reports it.
-#include <torch/extension.h>
+#include "torch_host.h"
 
-#include <ATen/core/grad_mode.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 
-#include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <optional>
 #include <tuple>
 #include <utility>
 
-#include "../../include/flash_moba_hip.h"
-
 namespace {
 
-using at::Tensor;
+using namespace fmoba_host;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-void check(int rc) {
-  if (rc != 0) throw std::runtime_error(fmoba_last_error());
-}
-
-// A C++ exception of the base class becomes RuntimeError in Python.  The device check is made once per device.
-void check_device(int index) {
-  static std::atomic<uint64_t> ok{0};
-  const uint64_t bit = uint64_t(1) << (index & 63);
-  if (index < 64 && (ok.load(std::memory_order_relaxed) & bit)) return;
-  check(fmoba_check_device());
-  if (index < 64) ok.fetch_or(bit);
-}
-
-PyObject *g_parameter_class = nullptr;  // torch.nn.Parameter
-
-// an ordinary tensor (or parameter): no subclass, no wrapper of a transform, no lazy conjugate, no tangent of forward-mode
-// differentiation (a dual tensor has the key set of an ordinary one; the path in Python refuses it, having no derivative of that kind)
-bool plain(const py::handle &h) {
-  if (!THPVariable_CheckExact(h.ptr()) && reinterpret_cast<PyObject *>(Py_TYPE(h.ptr())) != g_parameter_class) return false;
-  const Tensor &t = THPVariable_Unpack(h.ptr());
-  return t.defined() && t.is_cuda() && !t.is_sparse() && !t._fw_grad(/*level=*/0).defined() &&
-         !t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                                   c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative}));
-}
-
-bool eager() { return !c10::impl::TorchDispatchModeTLS::any_modes_set() && !torch::jit::tracer::isTracing(); }
-
-bool is_cu(const Tensor &t, int64_t n, const at::Device &dev) {
-  return t.scalar_type() == at::kInt && t.dim() == 1 && t.numel() == n && t.is_contiguous() && t.device() == dev;
-}
-
-// (rows, heads, dim), last dimension dense, 16-byte vectors
-bool is_rows(const Tensor &t, at::ScalarType dt, const at::Device &dev) {
-  return t.dim() == 3 && t.scalar_type() == dt && t.device() == dev && t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-}
 
 struct Shape {
   int64_t total_q, total_k, heads, heads_k, dim, batch, max_q, max_k, chunk, max_cols;
@@ -98,9 +51,6 @@ bool common_form(Shape &s, const Tensor &q, const Tensor &k, const Tensor &cu_q,
   s.dtype = dt == at::kBFloat16 ? FMOBA_DTYPE_BF16 : FMOBA_DTYPE_F16;
   return true;
 }
-
-Tensor bytes_like(const Tensor &q, size_t n) { return at::empty({static_cast<int64_t>(std::max<size_t>(n, 1))}, q.options().dtype(at::kByte)); }
-size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Pattern {
   Tensor col_offsets, col_nnz, indices, scratch;
@@ -454,10 +404,11 @@ int take_last_backward() { return std::exchange(t_partials, -1); }
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  g_parameter_class = py::object(py::module_::import("torch.nn").attr("Parameter")).release().ptr();
+  fmoba_host::g_parameter_class = py::object(py::module_::import("torch.nn").attr("Parameter")).release().ptr();
   m.def("moba_varlen", &moba_varlen);
   m.def("topk_varlen", &topk_varlen);
   m.def("attn_varlen", &attn_varlen);
   m.def("last_forward", &last_forward);
   m.def("take_last_backward", &take_last_backward);
+  bind_cache_ops(m);
 }

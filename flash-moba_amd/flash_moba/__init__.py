@@ -6,3 +6,4 @@ from flash_moba.flash_moba_interface import (  # noqa: F401
     flash_moba_attn_varlen_func,
     flash_moba_varlen_func,
 )
+from flash_moba.rotary import flash_moba_rotary_func  # noqa: F401

@@ -35,6 +35,14 @@ HOST_PATH = os.path.join(os.path.dirname(_HERE), "lib", "flash_moba_host.so")
 c_i32, c_i64, c_f32, c_vp, c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("k", c_vp), ("q_out", c_vp), ("k_out", c_vp), ("positions", c_vp), ("log2_base", ctypes.c_double), ("total", c_i64),
+                ("q_row_stride", c_i64), ("q_head_stride", c_i64), ("k_row_stride", c_i64), ("k_head_stride", c_i64),
+                ("qo_row_stride", c_i64), ("qo_head_stride", c_i64), ("ko_row_stride", c_i64), ("ko_head_stride", c_i64), ("pos_axis_stride", c_i64),
+                ("heads", c_i32), ("heads_k", c_i32), ("head_dim", c_i32), ("rotary_dim", c_i32),
+                ("axes", c_i32), ("sections", c_i32 * 4), ("positions_64", c_i32), ("interleaved", c_i32), ("inverse", c_i32), ("dtype", c_i32)]
+
+
 class MeanPoolArgs(ctypes.Structure):
     _fields_ = [("k", c_vp), ("km", c_vp), ("cu_seqlens_k", c_vp), ("cu_seqlens_km", c_vp),
                 ("batch", c_i32), ("max_chunks", c_i32), ("heads_k", c_i32), ("head_dim", c_i32),
@@ -122,6 +130,7 @@ EXPORTS = {
     "fmoba_attn_bwd_uses_partials": (c_i32, [ctypes.POINTER(AttnBwdArgs)]),
     "fmoba_attn_bwd": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_vp]),
     "fmoba_attn_bwd_phases": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_i32, c_vp]),
+    "fmoba_rotary": (c_i32, [ctypes.POINTER(RotaryArgs), c_vp]),
 }
 
 _lib = None

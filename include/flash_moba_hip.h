@@ -303,6 +303,29 @@ int fmoba_attn_bwd_grouped(const fmoba_attn_bwd_args *a, int32_t dkv_heads, int3
 /* The same over the lists and visits of fmoba_pool_and_gate_ranked, as fmoba_attn_fwd_ranked. */
 int fmoba_attn_bwd_ranked(const fmoba_attn_bwd_args *a, const uint32_t *visits, int32_t dkv_heads, int32_t phases, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Rotary positions with several axes, on packed q and k (no counterpart in the reference, whose callers turn q and k themselves).
+ * Pair j (j < rotary_dim / 2) of every head of token t is turned by positions[axis][t] * 2^(-log2_base * 2 j / rotary_dim), axis = the one whose
+ * run of `sections` pairs holds j; the pair is features (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved.  Features behind rotary_dim
+ * are copied.  inverse = 1 turns by the negative angles (the backward pass).  q_out and k_out may be q and k (same strides).  heads = 0 or
+ * heads_k = 0: q or k is left out.
+ * ---------------------------------------------------------------------------------- */
+#define FMOBA_ROTARY_AXES 4
+typedef struct {
+  const void *q, *k;        /* (total, heads, head_dim), (total, heads_k, head_dim) */
+  void *q_out, *k_out;
+  const void *positions;    /* (axes, total) int32, or int64 if positions_64 */
+  double log2_base;
+  int64_t total;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+  int64_t qo_row_stride, qo_head_stride, ko_row_stride, ko_head_stride;
+  int64_t pos_axis_stride;  /* the positions of an axis are dense */
+  int32_t heads, heads_k, head_dim, rotary_dim;
+  int32_t axes, sections[FMOBA_ROTARY_AXES];
+  int32_t positions_64, interleaved, inverse, dtype;
+} fmoba_rotary_args;
+int fmoba_rotary(const fmoba_rotary_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
