@@ -1,0 +1,147 @@
+// New keys and values rounded into the pages of an 8-bit cache: a workgroup takes the tokens that one page receives, for one key head, of K or of V.
+//   s = 2^ceil(log2(amax / M)), M = 448 or 127;  held = rne(x / s);  the sum of the page's keys and their mean beside it.
+// A power of two leaves nothing to round in x / s and held * s, and a page whose scale grows (a later token is larger) loses by its second rounding
+// no more than it would have by one at the larger scale, half a step each.
+//
+// Bound by memory: two bytes read and one written per feature.  The scale needs the largest value of the page's new rows before any can be
+// written: they stay in registers in between where a thread has up to kKept pieces (pages of 128 tokens and heads of 128), and are read again from the
+// caches beyond.  A decode step brings one row per page: there it is a launch and two dependent loads.
+#include "kv_cache.h"
+
+#include <algorithm>
+
+namespace fmoba {
+
+constexpr int kAppendThreads = 256;
+constexpr int kKept = 8;
+
+template <typename T, typename H>
+__global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(fmoba_cache_append_args a) {
+  __shared__ float sSum[kAppendThreads * 8];
+  __shared__ float sMax[kAppendThreads / 64];
+  const fmoba_kv_cache &c = a.cache;
+  const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x, P = c.page_size, D = c.head_dim;
+  const bool is_k = (blockIdx.x & 1) == 0;
+  const int row0 = min(max(a.cu_seqlens[b], 0), a.total_new), row1 = min(max(a.cu_seqlens[b + 1], row0), a.total_new);
+  const int end = a.seqlens_k[b], start = end - (row1 - row0);
+  const int slot = max(start, 0) / P + (int)(blockIdx.x >> 1);
+  if (slot >= a.max_pages || (int64_t)slot * P >= end) return;
+  const int lo = max(start, slot * P), hi = min((int64_t)end, (int64_t)slot * P + P);  // the new tokens of the page
+  if (lo >= hi) return;
+  const int page = a.block_table[(int64_t)b * a.table_stride + slot];
+  if (page < 0 || page >= c.num_pages) return;
+  const int old = lo - slot * P;  // tokens that it has already
+  const int64_t at = (int64_t)page * c.heads_k + hk;
+
+  const int lanes = D / 8, rows = kAppendThreads / lanes;  // threads of a row (8 features each), rows of a pass
+  const int r = tid / lanes, e = (tid - r * lanes) * 8;
+  const bool works = r < rows;
+  const int64_t src_stride = is_k ? a.k_row_stride : a.v_row_stride;
+  const uint16_t *src = reinterpret_cast<const uint16_t *>(is_k ? a.k : a.v) + (int64_t)(row0 + (lo - start)) * src_stride + (int64_t)hk * (is_k ? a.k_head_stride : a.v_head_stride) + e;
+  const int64_t dst_stride = is_k ? c.k_token_stride : c.v_token_stride;
+  uint8_t *held = reinterpret_cast<uint8_t *>(is_k ? c.k : c.v) + (int64_t)page * (is_k ? c.k_page_stride : c.v_page_stride) + (int64_t)hk * (is_k ? c.k_head_stride : c.v_head_stride) + e;
+  float *scale_at = (is_k ? c.k_scale : c.v_scale) + at;
+  const float was = old > 0 ? *scale_at : 0.f;
+
+  // ---- the largest finite magnitude, and the sums of the features ----
+  const int n = hi - lo;
+  Pack8 x[kKept];
+  float amax = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int row = i0 + i * rows + r;
+      x[i] = works && row < n ? ld_global16(src + (int64_t)row * src_stride) : zero_pack8();
+    }
+  };
+  const int turn = rows * kKept;  // rows of a turn of the whole workgroup
+  for (int i0 = 0; i0 < n; i0 += turn) {
+    load(i0);
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      float f[8];
+      unpack8<T>(x[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float m = fabsf(f[j]);
+        amax = m < INFINITY ? fmaxf(amax, m) : amax;
+        sum[j] += f[j];
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  if ((tid & 63) == 0) sMax[tid >> 6] = amax;
+  if (is_k && works) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sSum[r * D + e + j] = sum[j];
+  }
+  __syncthreads();
+  amax = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
+  const float scale = old > 0 ? fmaxf(scale_of<H>(amax), was) : scale_of<H>(amax);
+  if (is_k && tid < D) {
+    float s = 0.f;
+    for (int i = 0; i < rows; ++i) s += sSum[i * D + tid];
+    float *k_sum = c.k_sum + at * D + tid;
+    if (old > 0) s += *k_sum;
+    *k_sum = s;
+    reinterpret_cast<uint16_t *>(c.k_mean)[at * D + tid] = float_to_elem_bits<T>(s / (float)(old + n));
+  }
+  if (tid == 0) {
+    *scale_at = scale;
+    if (is_k && old == 0 && c.weight != nullptr) c.weight[at] = 0;
+  }
+
+  // ---- what the page has, at its new scale ----
+  if (scale > was && old > 0 && works) {
+    const float ratio = was / scale;
+    for (int row = r; row < old; row += rows) {
+      uint2 *p = reinterpret_cast<uint2 *>(held + (int64_t)row * dst_stride);
+      uint2 w = *p;
+      float f[4], g[4];
+      H::unpack4(w.x, f);
+      H::unpack4(w.y, g);
+      w.x = H::pack4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+      w.y = H::pack4(g[0] * ratio, g[1] * ratio, g[2] * ratio, g[3] * ratio);
+      *p = w;
+    }
+  }
+  // ---- the new rows ----
+  const float inv = 1.f / scale;
+  for (int i0 = 0; i0 < n; i0 += turn) {
+    if (n > turn) load(i0);
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int row = i0 + i * rows + r;
+      if (!works || row >= n) continue;
+      float f[8];
+      unpack8<T>(x[i], f);
+      uint2 w;
+      w.x = H::pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+      w.y = H::pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+      *reinterpret_cast<uint2 *>(held + (int64_t)(old + row) * dst_stride) = w;
+    }
+  }
+}
+
+}  // namespace fmoba
+
+extern "C" int fmoba_cache_append(const fmoba_cache_append_args *a, void *stream) {
+  using namespace fmoba;
+  FMOBA_REQUIRE(a != nullptr, "cache_append: null args");
+  FMOBA_CHECK_CACHE(a->cache);
+  FMOBA_REQUIRE(a->batch >= 1 && a->batch <= 65535 && a->total_new >= 0 && a->max_seqlen_new >= 0 && a->max_pages >= 0, "cache_append: sizes must not be negative, batch at most 65535");
+  if (a->total_new == 0 || a->max_seqlen_new == 0 || a->max_pages == 0 || a->cache.num_pages == 0) return 0;
+  FMOBA_REQUIRE(a->k && a->v && a->cu_seqlens && a->seqlens_k && a->block_table && a->cache.k_sum, "cache_append: null pointer");
+  FMOBA_REQUIRE(a->k_row_stride % 8 == 0 && a->k_head_stride % 8 == 0 && a->v_row_stride % 8 == 0 && a->v_head_stride % 8 == 0, "cache_append: strides must be multiples of 8 elements");
+  FMOBA_REQUIRE((((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0, "cache_append: k and v must be 16-byte aligned");
+  // the pages that max_seqlen_new tokens can touch, K and V apart
+  const int64_t touched = std::min<int64_t>(ceil_div64(std::min<int64_t>(a->max_seqlen_new, a->total_new), a->cache.page_size) + 1, a->max_pages);
+  const dim3 grid((uint32_t)(2 * touched), a->cache.heads_k, a->batch), block(kAppendThreads);
+  const bool bf16 = a->cache.dtype == FMOBA_DTYPE_BF16, e4m3 = a->cache.format == FMOBA_CACHE_E4M3;
+  auto kern = bf16 ? (e4m3 ? cache_append_kernel<bf16_t, HeldE4M3> : cache_append_kernel<bf16_t, HeldInt8>)
+                   : (e4m3 ? cache_append_kernel<f16_t, HeldE4M3> : cache_append_kernel<f16_t, HeldInt8>);
+  hipLaunchKernelGGL(kern, grid, block, 0, (hipStream_t)stream, *a);
+  FMOBA_LAUNCH_CHECK("cache_append_kernel");
+  return 0;
+}

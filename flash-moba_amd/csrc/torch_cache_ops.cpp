@@ -162,9 +162,160 @@ std::pair<Tensor, Tensor> rotary_raw(const Tensor &q, const Tensor &k, const Ten
   return turn(q, k, positions, f);
 }
 
+// -------------------------------------------------------------------------------------------------------------------- cache
+// The tensors of a cache in the order of MobaKVCache; weight may be undefined.
+struct Cache {
+  Tensor k, v, k_scale, v_scale, k_sum, k_mean, weight;
+};
+constexpr int kCacheTensors = 7;
+
+bool dense(const Tensor &t, at::ScalarType type, const at::Device &dev) { return t.defined() && t.scalar_type() == type && t.device() == dev && t.is_contiguous(); }
+
+fmoba_kv_cache cache_view(const Cache &c) {
+  const Tensor &k = c.k, &v = c.v;
+  require(k.is_cuda(), "the cache must be on a GPU");
+  const at::Device dev = k.device();
+  require(k.dim() == 4 && v.dim() == 4 && v.sizes() == k.sizes() && v.device() == dev, "k and v of a cache must be (pages, heads, page_size, head_size) tensors of one shape on one GPU");
+  require(k.scalar_type() == v.scalar_type() && (k.scalar_type() == at::kFloat8_e4m3fn || k.scalar_type() == at::kChar), "k and v of a cache must be float8_e4m3fn or int8");
+  require(k.size(3) == 1 || (k.stride(3) == 1 && v.stride(3) == 1), "k and v of a cache must be contiguous on the last dim");
+  const int64_t pages = k.size(0), heads = k.size(1);
+  require(pages <= INT32_MAX && heads >= 1 && heads <= 65535 && k.size(2) <= 1024 && k.size(3) <= 256, "cache: too many pages or heads, or page_size above 1024 or head_size above 256");
+  auto per_head = [&](const Tensor &t, at::ScalarType type, int64_t more) {
+    return dense(t, type, dev) && t.dim() == (more ? 3 : 2) && t.size(0) == pages && t.size(1) == heads && (more == 0 || t.size(2) == more);
+  };
+  require(per_head(c.k_scale, at::kFloat, 0) && per_head(c.v_scale, at::kFloat, 0), "k_scale and v_scale of a cache must be dense fp32 (pages, heads)");
+  require(per_head(c.k_sum, at::kFloat, k.size(3)), "k_sum of a cache must be dense fp32 (pages, heads, head_size)");
+  const at::ScalarType dt = c.k_mean.defined() ? c.k_mean.scalar_type() : at::kFloat;
+  require(dt == at::kHalf || dt == at::kBFloat16, "FlashMoBA only supports fp16 and bf16 data types");
+  require(per_head(c.k_mean, dt, k.size(3)), "k_mean of a cache must be dense (pages, heads, head_size)");
+  require(!c.weight.defined() || per_head(c.weight, at::kLong, 0), "weight of a cache must be dense int64 (pages, heads)");
+  for (const Tensor *t : {&c.k, &c.v, &c.k_scale, &c.v_scale, &c.k_sum, &c.k_mean}) require(!t->requires_grad(), "the cache has no gradients");
+  fmoba_kv_cache a{};
+  a.k = k.data_ptr(), a.v = v.data_ptr(), a.k_scale = c.k_scale.data_ptr<float>(), a.v_scale = c.v_scale.data_ptr<float>(), a.k_sum = c.k_sum.data_ptr<float>();
+  a.k_mean = c.k_mean.data_ptr(), a.weight = c.weight.defined() ? c.weight.data_ptr<int64_t>() : nullptr;
+  a.k_page_stride = k.stride(0), a.k_head_stride = k.stride(1), a.k_token_stride = k.stride(2);
+  a.v_page_stride = v.stride(0), a.v_head_stride = v.stride(1), a.v_token_stride = v.stride(2);
+  a.num_pages = pages, a.page_size = k.size(2), a.heads_k = heads, a.head_dim = k.size(3);
+  a.format = k.scalar_type() == at::kChar ? FMOBA_CACHE_INT8 : FMOBA_CACHE_E4M3, a.dtype = dt == at::kBFloat16 ? FMOBA_DTYPE_BF16 : FMOBA_DTYPE_F16;
+  return a;
+}
+
+// lengths and tables of a call's sequences; returns how many there are
+int64_t check_sequences(const Tensor &cu, const Tensor &seqlens_k, const Tensor &table, const at::Device &dev) {
+  require(seqlens_k.dim() == 1 && dense(seqlens_k, at::kInt, dev) && seqlens_k.size(0) >= 1 && seqlens_k.size(0) <= 65535, "seqlens_k must be dense int32 (batch) on the cache's GPU, batch up to 65535");
+  const int64_t batch = seqlens_k.size(0);
+  require(!cu.defined() || is_cu(cu, batch + 1, dev), "cu_seqlens must be dense int32 (batch + 1) on the cache's GPU");
+  require(table.dim() == 2 && table.scalar_type() == at::kInt && table.device() == dev && table.size(0) == batch && (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) <= INT32_MAX,
+          "block_table must be int32 (batch, pages of a sequence) on the cache's GPU, its rows dense");
+  return batch;
+}
+
+void check_inference(std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    require(!(at::GradMode::is_enabled() && t->requires_grad()), "the cache functions have no backward pass: call them under torch.no_grad(), or with detached tensors");
+}
+
+void append_raw(const Cache &c, const Tensor &k_in, const Tensor &v_in, const Tensor &cu, int64_t max_seqlen, const Tensor &seqlens_k, const Tensor &table) {
+  fmoba_cache_append_args a{};
+  a.cache = cache_view(c);
+  const at::Device dev = c.k.device();
+  const at::ScalarType dt = c.k_mean.scalar_type();
+  check_inference({&k_in, &v_in});
+  require(k_in.dim() == 3 && v_in.sizes() == k_in.sizes() && k_in.scalar_type() == dt && v_in.scalar_type() == dt && k_in.device() == dev && v_in.device() == dev,
+          "k and v must be (tokens, heads, head_size) of the cache's k_mean dtype on its GPU");
+  require(k_in.size(1) == c.k.size(1) && k_in.size(2) == c.k.size(3), "heads and head size of k and v must be the cache's");
+  require(k_in.size(0) <= INT32_MAX && max_seqlen >= 0 && max_seqlen <= INT32_MAX, "max_seqlen or the number of tokens is out of range");
+  a.batch = check_sequences(cu, seqlens_k, table, dev);
+  require(cu.defined(), "cu_seqlens must be given");
+  const Tensor k = as_rows(k_in), v = as_rows(v_in);
+  a.k = k.data_ptr(), a.v = v.data_ptr(), a.cu_seqlens = cu.data_ptr<int32_t>(), a.seqlens_k = seqlens_k.data_ptr<int32_t>(), a.block_table = table.data_ptr<int32_t>();
+  a.k_row_stride = k.stride(0), a.k_head_stride = k.stride(1), a.v_row_stride = v.stride(0), a.v_head_stride = v.stride(1), a.table_stride = table.stride(0);
+  a.total_new = k.size(0), a.max_seqlen_new = max_seqlen, a.max_pages = table.size(1);
+  const c10::DeviceGuard guard(dev);
+  check_device(dev.index());
+  check(fmoba_cache_append(&a, current_stream(c.k)));
+}
+
+std::vector<Tensor> evict_raw(const Tensor &weight, const Tensor &seqlens_k, const Tensor &table, int64_t page_size, int64_t keep, int64_t sink, int64_t recent) {
+  require(weight.is_cuda() && weight.dim() == 2 && weight.scalar_type() == at::kLong && weight.is_contiguous() && weight.size(0) <= INT32_MAX && weight.size(1) >= 1 && weight.size(1) <= 65535,
+          "weight must be dense int64 (pages, heads) on a GPU");
+  for (int64_t x : {page_size, keep, sink, recent}) require(x >= INT32_MIN && x <= INT32_MAX, "page_size and numbers of pages must be below 2^31");
+  fmoba_cache_evict_args a{};
+  a.batch = check_sequences(Tensor(), seqlens_k, table, weight.device());
+  const c10::DeviceGuard guard(weight.device());
+  check_device(weight.device().index());
+  const Tensor new_table = at::empty(table.sizes(), table.options()), freed = at::empty(table.sizes(), table.options());
+  const Tensor new_seqlens = at::empty(seqlens_k.sizes(), seqlens_k.options()), num_freed = at::empty(seqlens_k.sizes(), seqlens_k.options());
+  a.weight = weight.data_ptr<int64_t>(), a.seqlens_k = seqlens_k.data_ptr<int32_t>(), a.block_table = table.data_ptr<int32_t>();
+  a.new_table = new_table.data_ptr<int32_t>(), a.new_seqlens = new_seqlens.data_ptr<int32_t>(), a.freed = freed.data_ptr<int32_t>(), a.num_freed = num_freed.data_ptr<int32_t>();
+  a.table_stride = table.stride(0), a.max_pages = table.size(1), a.num_pages = weight.size(0), a.heads_k = weight.size(1);
+  a.page_size = page_size, a.keep = keep, a.sink = sink, a.recent = recent;
+  a.workspace_bytes = fmoba_cache_evict_workspace_bytes(a.batch, a.max_pages);
+  Tensor ws;
+  if (a.workspace_bytes) ws = bytes_like(weight, a.workspace_bytes), a.workspace = ws.data_ptr();
+  check(fmoba_cache_evict(&a, current_stream(weight)));
+  return {new_table, new_seqlens, freed, num_freed};
+}
+
+// a tuple of a cache's tensors (the last may be None) as C++ ones; false if one is not an ordinary tensor
+bool plain_cache(const py::handle &h, Cache &c) {
+  if (!PyTuple_Check(h.ptr()) || PyTuple_GET_SIZE(h.ptr()) != kCacheTensors) throw std::runtime_error("cache must be a MobaKVCache");
+  Tensor *to[kCacheTensors] = {&c.k, &c.v, &c.k_scale, &c.v_scale, &c.k_sum, &c.k_mean, &c.weight};
+  for (int i = 0; i < kCacheTensors; ++i) {
+    PyObject *o = PyTuple_GET_ITEM(h.ptr(), i);
+    if (i == kCacheTensors - 1 && o == Py_None) continue;
+    if (!plain(o)) return false;
+    *to[i] = THPVariable_Unpack(o);
+  }
+  return true;
+}
+
+bool all_plain(std::initializer_list<py::handle> hs) {
+  for (const py::handle &h : hs)
+    if (!plain(h)) return false;
+  return true;
+}
+const Tensor &unpack(const py::handle &h) { return THPVariable_Unpack(h.ptr()); }
+
+bool cache_append(const py::handle &hc, const py::handle &hk, const py::handle &hv, const py::handle &hcu, int64_t max_seqlen, const py::handle &hlen, const py::handle &htable) {
+  Cache c;
+  if (!eager() || !plain_cache(hc, c) || !all_plain({hk, hv, hcu, hlen, htable})) return false;
+  py::gil_scoped_release nogil;
+  at::AutoDispatchBelowADInplaceOrView below;
+  append_raw(c, unpack(hk), unpack(hv), unpack(hcu), max_seqlen, unpack(hlen), unpack(htable));
+  return true;
+}
+
+py::object cache_evict(const py::handle &hw, const py::handle &hlen, const py::handle &htable, int64_t page_size, int64_t keep, int64_t sink, int64_t recent) {
+  if (!eager() || !all_plain({hw, hlen, htable})) return none();
+  std::vector<Tensor> r;
+  {
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    r = evict_raw(unpack(hw), unpack(hlen), unpack(htable), page_size, keep, sink, recent);
+  }
+  return py::make_tuple(wrap(r[0]), wrap(r[1]), wrap(r[2]), wrap(r[3]));
+}
+
+// the same for the custom ops
+using Optional = std::optional<Tensor>;
+Cache cache_of(const Tensor &k, const Tensor &v, const Tensor &k_scale, const Tensor &v_scale, const Tensor &k_sum, const Tensor &k_mean, const Optional &weight) {
+  return Cache{k, v, k_scale, v_scale, k_sum, k_mean, weight.value_or(Tensor())};
+}
+void cache_append_op(const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &sum, const Tensor &mean, const Optional &weight, const Tensor &k, const Tensor &v,
+                     const Tensor &cu, int64_t max_seqlen, const Tensor &seqlens_k, const Tensor &table) {
+  py::gil_scoped_release nogil;
+  at::AutoDispatchBelowADInplaceOrView below;
+  append_raw(cache_of(kc, vc, ks, vs, sum, mean, weight), k, v, cu, max_seqlen, seqlens_k, table);
+}
+
 }  // namespace
 
 void fmoba_host::bind_cache_ops(py::module_ &m) {
   m.def("rotary", &rotary);
   m.def("rotary_raw", &rotary_raw);
+  m.def("cache_append", &cache_append);
+  m.def("cache_append_op", &cache_append_op);
+  m.def("cache_evict", &cache_evict);
+  m.def("cache_evict_op", &evict_raw);
 }

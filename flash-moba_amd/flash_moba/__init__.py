@@ -7,3 +7,8 @@ from flash_moba.flash_moba_interface import (  # noqa: F401
     flash_moba_varlen_func,
 )
 from flash_moba.rotary import flash_moba_rotary_func  # noqa: F401
+from flash_moba.kv_cache import (  # noqa: F401
+    MobaKVCache,
+    flash_moba_cache_append_func,
+    flash_moba_cache_evict_func,
+)

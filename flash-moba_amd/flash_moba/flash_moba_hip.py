@@ -35,6 +35,25 @@ HOST_PATH = os.path.join(os.path.dirname(_HERE), "lib", "flash_moba_host.so")
 c_i32, c_i64, c_f32, c_vp, c_sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("k_sum", c_vp), ("k_mean", c_vp), ("weight", c_vp),
+                ("k_page_stride", c_i64), ("k_head_stride", c_i64), ("k_token_stride", c_i64),
+                ("v_page_stride", c_i64), ("v_head_stride", c_i64), ("v_token_stride", c_i64),
+                ("num_pages", c_i32), ("page_size", c_i32), ("heads_k", c_i32), ("head_dim", c_i32), ("format", c_i32), ("dtype", c_i32)]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    _fields_ = [("cache", KVCache), ("k", c_vp), ("v", c_vp), ("cu_seqlens", c_vp), ("seqlens_k", c_vp), ("block_table", c_vp),
+                ("k_row_stride", c_i64), ("k_head_stride", c_i64), ("v_row_stride", c_i64), ("v_head_stride", c_i64), ("table_stride", c_i64),
+                ("batch", c_i32), ("total_new", c_i32), ("max_seqlen_new", c_i32), ("max_pages", c_i32)]
+
+
+class CacheEvictArgs(ctypes.Structure):
+    _fields_ = [("weight", c_vp), ("seqlens_k", c_vp), ("block_table", c_vp), ("new_table", c_vp), ("new_seqlens", c_vp), ("freed", c_vp), ("num_freed", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", c_sz), ("table_stride", c_i64),
+                ("batch", c_i32), ("max_pages", c_i32), ("num_pages", c_i32), ("heads_k", c_i32), ("page_size", c_i32), ("keep", c_i32), ("sink", c_i32), ("recent", c_i32)]
+
+
 class RotaryArgs(ctypes.Structure):
     _fields_ = [("q", c_vp), ("k", c_vp), ("q_out", c_vp), ("k_out", c_vp), ("positions", c_vp), ("log2_base", ctypes.c_double), ("total", c_i64),
                 ("q_row_stride", c_i64), ("q_head_stride", c_i64), ("k_row_stride", c_i64), ("k_head_stride", c_i64),
@@ -131,6 +150,9 @@ EXPORTS = {
     "fmoba_attn_bwd": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_vp]),
     "fmoba_attn_bwd_phases": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_i32, c_vp]),
     "fmoba_rotary": (c_i32, [ctypes.POINTER(RotaryArgs), c_vp]),
+    "fmoba_cache_append": (c_i32, [ctypes.POINTER(CacheAppendArgs), c_vp]),
+    "fmoba_cache_evict_workspace_bytes": (c_sz, [c_i32, c_i32]),
+    "fmoba_cache_evict": (c_i32, [ctypes.POINTER(CacheEvictArgs), c_vp]),
 }
 
 _lib = None

@@ -1,0 +1,106 @@
+"""A paged key / value cache in 8 bits for serving MoBA models (no counterpart in the reference, which has no cache).
+
+A page holds `page_size` consecutive tokens of one sequence and is the chunk that the gate selects.  Keys and values are held as
+float8_e4m3fn or int8 with a scale for each (page, key head), a power of two; beside them lie what the gate scores, the mean of the
+page's keys, and the attention weight that the page has received, by which pages are let go.  The kernels are those of csrc/kv_*.hip.
+"""
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from flash_moba import flash_moba_hip as flash_moba_gpu
+
+
+class MobaKVCache(NamedTuple):
+    """The tensors of a cache (all layers' caches are their own).  k and v may have any strides that are multiples of 16 with a
+    dense last dimension, the others are dense.  Contents before a page's first token do not matter."""
+    k: torch.Tensor                  # (pages, heads_k, page_size, head_size) float8_e4m3fn or int8
+    v: torch.Tensor
+    k_scale: torch.Tensor            # (pages, heads_k) fp32
+    v_scale: torch.Tensor
+    k_sum: torch.Tensor              # (pages, heads_k, head_size) fp32: sum of the page's keys, as they were given
+    k_mean: torch.Tensor             # the same shape, fp16 / bf16 (the dtype of q, k and v): that sum over the page's tokens
+    weight: Optional[torch.Tensor]   # (pages, heads_k) int64: attention weight received, in units of 2^-32; None: not kept
+
+    @classmethod
+    def allocate(cls, num_pages, page_size, num_heads_k, head_size, dtype=torch.bfloat16, cache_dtype=torch.float8_e4m3fn, device="cuda",
+                 keep_weight=True):
+        """An empty cache: page_size a multiple of 64 up to 1024, head_size of 16 up to 256, dtype that of q, k and v."""
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError("FlashMoBA only supports fp16 and bf16 data types")
+        if cache_dtype not in (torch.float8_e4m3fn, torch.int8):
+            raise RuntimeError("a cache holds float8_e4m3fn or int8")
+        if page_size < 64 or page_size > 1024 or page_size % 64 != 0:
+            raise RuntimeError("page_size must be a multiple of 64 up to 1024")
+        if head_size < 16 or head_size > 256 or head_size % 16 != 0:
+            raise RuntimeError("head_size must be a multiple of 16 up to 256")
+        rows, one = (num_pages, num_heads_k, head_size), (num_pages, num_heads_k)
+        held = (num_pages, num_heads_k, page_size, head_size)
+        return cls(torch.zeros(held, dtype=torch.int8, device=device).view(cache_dtype), torch.zeros(held, dtype=torch.int8, device=device).view(cache_dtype),
+                   torch.ones(one, dtype=torch.float32, device=device), torch.ones(one, dtype=torch.float32, device=device),
+                   torch.zeros(rows, dtype=torch.float32, device=device), torch.zeros(rows, dtype=dtype, device=device),
+                   torch.zeros(one, dtype=torch.int64, device=device) if keep_weight else None)
+
+
+# --------------------------------------------------------------------------------------
+# custom ops, for traced graphs (eager calls go to the host module directly)
+# --------------------------------------------------------------------------------------
+@torch.library.custom_op("flash_moba::_cache_append", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale", "k_sum", "k_mean", "weight"), device_types="cuda")
+def _cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, k_sum: torch.Tensor,
+                  k_mean: torch.Tensor, weight: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                  max_seqlen: int, seqlens_k: torch.Tensor, block_table: torch.Tensor) -> None:
+    flash_moba_gpu.host_module().cache_append_op(k_cache, v_cache, k_scale, v_scale, k_sum, k_mean, weight, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table)
+
+
+@torch.library.register_fake("flash_moba::_cache_append")
+def _cache_append_fake(k_cache, v_cache, k_scale, v_scale, k_sum, k_mean, weight, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table):
+    return None
+
+
+@torch.library.custom_op("flash_moba::_cache_evict", mutates_args=(), device_types="cuda")
+def _cache_evict(weight: torch.Tensor, seqlens_k: torch.Tensor, block_table: torch.Tensor, page_size: int, keep: int, sink: int,
+                 recent: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(flash_moba_gpu.host_module().cache_evict_op(weight, seqlens_k, block_table, page_size, keep, sink, recent))
+
+
+@torch.library.register_fake("flash_moba::_cache_evict")
+def _cache_evict_fake(weight, seqlens_k, block_table, page_size, keep, sink, recent):
+    return (block_table.new_empty(block_table.shape), seqlens_k.new_empty(seqlens_k.shape), block_table.new_empty(block_table.shape),
+            seqlens_k.new_empty(seqlens_k.shape))
+
+
+# --------------------------------------------------------------------------------------
+# public functions
+# --------------------------------------------------------------------------------------
+def flash_moba_cache_append_func(cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table):
+    """Writes new keys and values into the pages of a cache, in place, rounded to 8 bits.
+
+    k, v: (tokens, num_heads_k, head_size) of the dtype of cache.k_mean, any strides; cu_seqlens: (batch + 1,) int32, which of them are whose;
+    max_seqlen: the most that a sequence gets; seqlens_k: (batch,) int32, tokens of every sequence WITH the new ones, which are its
+    last; block_table: (batch, n) int32, page of the tokens i * page_size and on of a sequence at [b, i].  Different sequences must
+    not get tokens in the same page.
+
+    The scale of a page and head is the least power of two (2^-64 to 2^64) that brings the largest finite magnitude among its tokens to
+    448 (e4m3) or 127 (int8) at most; infinities are held as that, NaN as NaN (int8: 0).  Where a later token needs a larger scale, the
+    page's earlier tokens are rounded again.  Places behind the end of a sequence, tokens before its beginning and table entries
+    that are no page (outside [0, pages)) are left alone.  A page's first token starts its sum and its weight anew.
+    """
+    if not torch.compiler.is_compiling() and flash_moba_gpu.host_module().cache_append(cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table):
+        return
+    torch.ops.flash_moba._cache_append(*cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table)
+
+
+def flash_moba_cache_evict_func(weight, seqlens_k, block_table, page_size, keep_pages, sink_pages=1, recent_pages=1):
+    """Which pages every sequence keeps when it has more than `keep_pages`: the first `sink_pages`, the last `recent_pages` (at
+    least 1, the page that is being filled), and of the others those that received most attention weight (cache.weight, summed over
+    heads; of equals the first).  Sequences with fewer pages keep all.
+
+    Returns (block_table, seqlens_k, freed, num_freed): the table of the pages kept, in order, and -1 behind them; the tokens
+    that are left; the pages let go in the same form, and how many they are.  The cache itself stays as it is: the freed pages can be given out again
+    at once.  Keys keep the positions that they were turned by, so rotary positions go on counting from the sequence's own length.
+    """
+    if not torch.compiler.is_compiling():
+        res = flash_moba_gpu.host_module().cache_evict(weight, seqlens_k, block_table, page_size, keep_pages, sink_pages, recent_pages)
+        if res is not None:
+            return res
+    return torch.ops.flash_moba._cache_evict(weight, seqlens_k, block_table, page_size, keep_pages, sink_pages, recent_pages)

@@ -326,6 +326,57 @@ typedef struct {
 } fmoba_rotary_args;
 int fmoba_rotary(const fmoba_rotary_args *a, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Paged key / value cache in 8 bits, for serving (no counterpart in the reference, which has no cache).
+ * A page holds `page_size` consecutive tokens of one sequence, and is the chunk that the gate selects.  What it holds, per key head:
+ *   k, v     [page_size][head_dim] values of 8 bits (row of a token dense, all strides multiples of 16 elements), to be
+ *            multiplied by k_scale, v_scale [num_pages][heads_k] fp32;
+ *   k_sum    [num_pages][heads_k][head_dim] fp32, the sum of the keys as they were given, k_mean the sum divided by the number of tokens, in `dtype`;
+ *   weight   [num_pages][heads_k] int64, attention weight that the page has received, in units of 2^-32.  NULL: not kept.
+ * Token t of sequence b lies in page block_table[b * table_stride + t / page_size], place t % page_size.  A table entry outside [0, num_pages) is no
+ * page: nothing is read or written there.  seqlens_k (batch) int32: tokens of every sequence, with those that the call adds or whose rows it has.
+ * ---------------------------------------------------------------------------------- */
+#define FMOBA_CACHE_E4M3 0 /* 4 exponent, 3 mantissa bits, finite values up to 448, NaN, no infinities */
+#define FMOBA_CACHE_INT8 1 /* -127 .. 127 */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale, *k_sum;
+  void *k_mean;
+  int64_t *weight;
+  int64_t k_page_stride, k_head_stride, k_token_stride, v_page_stride, v_head_stride, v_token_stride;
+  int32_t num_pages, page_size, heads_k, head_dim; /* page_size: a multiple of 64 up to 1024; head_dim: of 16 up to 256 */
+  int32_t format, dtype;
+} fmoba_kv_cache;
+
+/* New keys and values (total_new, heads_k, head_dim) of the tokens seqlens_k[b] - n_b .. seqlens_k[b] - 1, n_b = cu_seqlens[b + 1] - cu_seqlens[b] <=
+ * max_seqlen_new, rounded into their pages.  The scale of a (page, head) is the least power of two, from 2^-64 to 2^64, that brings the
+ * largest finite magnitude to 448 or 127; values beyond are cut off there, NaN is kept (int8: 0).  Where a page has tokens already its scale
+ * never shrinks, and where it grows the tokens there are rounded again.  A page that receives its first token starts with an empty sum and weight. */
+typedef struct {
+  fmoba_kv_cache cache;
+  const void *k, *v;
+  const int32_t *cu_seqlens, *seqlens_k, *block_table;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, table_stride;
+  int32_t batch, total_new, max_seqlen_new, max_pages; /* max_pages: entries of a sequence's table */
+} fmoba_cache_append_args;
+int fmoba_cache_append(const fmoba_cache_append_args *a, void *stream);
+
+/* Which pages a sequence keeps when it has more than `keep`: its first `sink`, its last `recent` (one at least: the page that is being filled), and of the
+ * others those with the most weight, summed over heads; of equals the first.  Their order stays.  new_table and freed (batch, max_pages), dense: pages
+ * kept and pages let go, in order, then -1; num_freed and new_seqlens (batch): how many, and the tokens that are left.  Nothing of
+ * the cache itself moves.  workspace: fmoba_cache_evict_workspace_bytes(batch, max_pages), contents undefined on entry and return. */
+typedef struct {
+  const int64_t *weight;    /* (num_pages, heads_k) */
+  const int32_t *seqlens_k, *block_table;
+  int32_t *new_table, *new_seqlens, *freed, *num_freed;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t table_stride;
+  int32_t batch, max_pages, num_pages, heads_k, page_size, keep, sink, recent;
+} fmoba_cache_evict_args;
+size_t fmoba_cache_evict_workspace_bytes(int32_t batch, int32_t max_pages);
+int fmoba_cache_evict(const fmoba_cache_evict_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
