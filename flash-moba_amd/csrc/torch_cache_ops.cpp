@@ -236,6 +236,46 @@ void append_raw(const Cache &c, const Tensor &k_in, const Tensor &v_in, const Te
   check(fmoba_cache_append(&a, current_stream(c.k)));
 }
 
+struct AttnForm {
+  int64_t max_q, max_k, topk;
+  std::optional<double> scale;
+  bool add_weight;
+};
+
+void check_attn(const Tensor &q, const Cache &c, const AttnForm &f) {
+  check_inference({&q});
+  require(q.dim() == 3 && q.scalar_type() == c.k_mean.scalar_type() && q.device() == c.k.device(), "q must be (tokens, heads, head_size) of the cache's k_mean dtype on its GPU");
+  require(q.size(2) == c.k.size(3), "the head size of q must be the cache's");
+  require(q.size(1) >= 1 && q.size(1) % c.k.size(1) == 0, "#heads in key/value must divide #heads in query");
+  require(q.size(0) <= INT32_MAX && q.size(1) <= 65535 && q.size(0) * q.size(1) <= INT32_MAX && f.max_q >= 0 && f.max_q <= INT32_MAX && f.max_k >= 0 && f.max_k <= INT32_MAX,
+          "max_seqlen or the number of rows is out of range");
+  require(f.topk >= 1 && f.topk <= 64, "moba_topk must be in [1, 64]");
+  require(!f.add_weight || c.weight.defined(), "the cache keeps no weight");
+}
+
+std::pair<Tensor, Tensor> attn_raw(const Tensor &q_in, const Cache &c, const Tensor &cu, const Tensor &seqlens_k, const Tensor &table, const AttnForm &f) {
+  fmoba_cache_attn_args a{};
+  a.cache = cache_view(c);
+  const at::Device dev = c.k.device();
+  check_attn(q_in, c, f);
+  a.batch = check_sequences(cu, seqlens_k, table, dev);
+  require(cu.defined(), "cu_seqlens must be given");
+  const c10::DeviceGuard guard(dev);
+  check_device(dev.index());
+  const Tensor q = as_rows(q_in);
+  const Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  a.q = q.data_ptr(), a.out = out.data_ptr(), a.softmax_lse = lse.data_ptr<float>();
+  a.cu_seqlens_q = cu.data_ptr<int32_t>(), a.seqlens_k = seqlens_k.data_ptr<int32_t>(), a.block_table = table.data_ptr<int32_t>();
+  a.q_row_stride = q.stride(0), a.q_head_stride = q.stride(1), a.o_row_stride = out.stride(0), a.o_head_stride = out.stride(1), a.table_stride = table.stride(0);
+  a.total_q = q.size(0), a.heads = q.size(1), a.max_seqlen_q = f.max_q, a.max_seqlen_k = f.max_k, a.max_pages = table.size(1), a.topk = f.topk, a.add_weight = f.add_weight;
+  a.softmax_scale = static_cast<float>(f.scale ? *f.scale : std::pow(static_cast<double>(q.size(2)), -0.5));
+  a.workspace_bytes = fmoba_cache_attn_workspace_bytes(&a);
+  const Tensor ws = bytes_like(q, a.workspace_bytes + 255);
+  a.workspace = reinterpret_cast<void *>(up256(reinterpret_cast<size_t>(ws.data_ptr())));
+  check(fmoba_cache_attn(&a, current_stream(c.k)));
+  return {out, lse};
+}
+
 std::vector<Tensor> evict_raw(const Tensor &weight, const Tensor &seqlens_k, const Tensor &table, int64_t page_size, int64_t keep, int64_t sink, int64_t recent) {
   require(weight.is_cuda() && weight.dim() == 2 && weight.scalar_type() == at::kLong && weight.is_contiguous() && weight.size(0) <= INT32_MAX && weight.size(1) >= 1 && weight.size(1) <= 65535,
           "weight must be dense int64 (pages, heads) on a GPU");
@@ -297,6 +337,46 @@ py::object cache_evict(const py::handle &hw, const py::handle &hlen, const py::h
   return py::make_tuple(wrap(r[0]), wrap(r[1]), wrap(r[2]), wrap(r[3]));
 }
 
+py::object cache_attn(const py::handle &hq, const py::handle &hc, const py::handle &hcu, int64_t max_q, const py::handle &hlen, int64_t max_k, const py::handle &htable, int64_t topk,
+                      std::optional<double> scale, bool add_weight) {
+  Cache c;
+  if (!eager() || !plain_cache(hc, c) || !all_plain({hq, hcu, hlen, htable})) return none();
+  std::pair<Tensor, Tensor> r;
+  {
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    r = attn_raw(unpack(hq), c, unpack(hcu), unpack(hlen), unpack(htable), AttnForm{max_q, max_k, topk, scale, add_weight});
+  }
+  return py::make_tuple(wrap(r.first), wrap(r.second));
+}
+
+// positions (if there are any), the new keys and values into the cache, attention: one call
+py::object cache_step(const py::handle &hq, const py::handle &hk, const py::handle &hv, const py::handle &hc, const py::handle &hcu, int64_t max_q, const py::handle &hlen, int64_t max_k,
+                      const py::handle &htable, int64_t topk, const py::handle &hp, std::vector<int64_t> sections, double base, int64_t rotary_dim, bool interleaved, std::optional<double> scale,
+                      bool add_weight) {
+  Cache c;
+  const bool turned = !hp.is_none();
+  if (!eager() || !plain_cache(hc, c) || !all_plain({hq, hk, hv, hcu, hlen, htable}) || (turned && !plain(hp))) return none();
+  const RotaryForm f = rotary_form(std::move(sections), base, rotary_dim, interleaved, false);
+  std::pair<Tensor, Tensor> r;
+  {
+    py::gil_scoped_release nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor q = unpack(hq), k = unpack(hk);
+    const AttnForm attn{max_q, max_k, topk, scale, add_weight};
+    cache_view(c);  // (what the attention would refuse is refused before the cache changes)
+    check_attn(q, c, attn);
+    check_inference({&k});
+    if (turned) {
+      check_rotary(q, k, unpack(hp), f);
+      std::tie(q, k) = turn(q, k, unpack(hp), f);
+    }
+    append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable));
+    r = attn_raw(q, c, unpack(hcu), unpack(hlen), unpack(htable), attn);
+  }
+  return py::make_tuple(wrap(r.first), wrap(r.second));
+}
+
 // the same for the custom ops
 using Optional = std::optional<Tensor>;
 Cache cache_of(const Tensor &k, const Tensor &v, const Tensor &k_scale, const Tensor &v_scale, const Tensor &k_sum, const Tensor &k_mean, const Optional &weight) {
@@ -309,6 +389,13 @@ void cache_append_op(const Tensor &kc, const Tensor &vc, const Tensor &ks, const
   append_raw(cache_of(kc, vc, ks, vs, sum, mean, weight), k, v, cu, max_seqlen, seqlens_k, table);
 }
 
+std::pair<Tensor, Tensor> cache_attn_op(const Tensor &q, const Tensor &kc, const Tensor &vc, const Tensor &ks, const Tensor &vs, const Tensor &sum, const Tensor &mean, const Optional &weight,
+                                        const Tensor &cu, int64_t max_q, const Tensor &seqlens_k, int64_t max_k, const Tensor &table, int64_t topk, std::optional<double> scale, bool add_weight) {
+  py::gil_scoped_release nogil;
+  at::AutoDispatchBelowADInplaceOrView below;
+  return attn_raw(q, cache_of(kc, vc, ks, vs, sum, mean, weight), cu, seqlens_k, table, AttnForm{max_q, max_k, topk, scale, add_weight});
+}
+
 }  // namespace
 
 void fmoba_host::bind_cache_ops(py::module_ &m) {
@@ -316,6 +403,9 @@ void fmoba_host::bind_cache_ops(py::module_ &m) {
   m.def("rotary_raw", &rotary_raw);
   m.def("cache_append", &cache_append);
   m.def("cache_append_op", &cache_append_op);
+  m.def("cache_attn", &cache_attn);
+  m.def("cache_attn_op", &cache_attn_op);
+  m.def("cache_step", &cache_step);
   m.def("cache_evict", &cache_evict);
   m.def("cache_evict_op", &evict_raw);
 }

@@ -10,5 +10,7 @@ from flash_moba.rotary import flash_moba_rotary_func  # noqa: F401
 from flash_moba.kv_cache import (  # noqa: F401
     MobaKVCache,
     flash_moba_cache_append_func,
+    flash_moba_cache_attn_func,
     flash_moba_cache_evict_func,
+    flash_moba_with_cache_func,
 )

@@ -48,6 +48,14 @@ class CacheAppendArgs(ctypes.Structure):
                 ("batch", c_i32), ("total_new", c_i32), ("max_seqlen_new", c_i32), ("max_pages", c_i32)]
 
 
+class CacheAttnArgs(ctypes.Structure):
+    _fields_ = [("cache", KVCache), ("q", c_vp), ("out", c_vp), ("softmax_lse", c_vp), ("cu_seqlens_q", c_vp), ("seqlens_k", c_vp), ("block_table", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", c_sz),
+                ("q_row_stride", c_i64), ("q_head_stride", c_i64), ("o_row_stride", c_i64), ("o_head_stride", c_i64), ("table_stride", c_i64),
+                ("batch", c_i32), ("total_q", c_i32), ("heads", c_i32), ("max_seqlen_q", c_i32), ("max_seqlen_k", c_i32), ("max_pages", c_i32), ("topk", c_i32),
+                ("add_weight", c_i32), ("softmax_scale", c_f32)]
+
+
 class CacheEvictArgs(ctypes.Structure):
     _fields_ = [("weight", c_vp), ("seqlens_k", c_vp), ("block_table", c_vp), ("new_table", c_vp), ("new_seqlens", c_vp), ("freed", c_vp), ("num_freed", c_vp),
                 ("workspace", c_vp), ("workspace_bytes", c_sz), ("table_stride", c_i64),
@@ -151,6 +159,8 @@ EXPORTS = {
     "fmoba_attn_bwd_phases": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_i32, c_vp]),
     "fmoba_rotary": (c_i32, [ctypes.POINTER(RotaryArgs), c_vp]),
     "fmoba_cache_append": (c_i32, [ctypes.POINTER(CacheAppendArgs), c_vp]),
+    "fmoba_cache_attn_workspace_bytes": (c_sz, [ctypes.POINTER(CacheAttnArgs)]),
+    "fmoba_cache_attn": (c_i32, [ctypes.POINTER(CacheAttnArgs), c_vp]),
     "fmoba_cache_evict_workspace_bytes": (c_sz, [c_i32, c_i32]),
     "fmoba_cache_evict": (c_i32, [ctypes.POINTER(CacheEvictArgs), c_vp]),
 }

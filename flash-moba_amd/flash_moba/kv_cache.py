@@ -9,6 +9,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from flash_moba import flash_moba_hip as flash_moba_gpu
+from flash_moba.rotary import flash_moba_rotary_func, rotary_form
 
 
 class MobaKVCache(NamedTuple):
@@ -57,6 +58,20 @@ def _cache_append_fake(k_cache, v_cache, k_scale, v_scale, k_sum, k_mean, weight
     return None
 
 
+@torch.library.custom_op("flash_moba::_cache_attn", mutates_args=("weight",), device_types="cuda")
+def _cache_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, k_sum: torch.Tensor,
+                k_mean: torch.Tensor, weight: Optional[torch.Tensor], cu_seqlens_q: torch.Tensor, max_seqlen_q: int, seqlens_k: torch.Tensor,
+                max_seqlen_k: int, block_table: torch.Tensor, topk: int, softmax_scale: Optional[float], add_weight: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    return flash_moba_gpu.host_module().cache_attn_op(q, k_cache, v_cache, k_scale, v_scale, k_sum, k_mean, weight, cu_seqlens_q, max_seqlen_q, seqlens_k,
+                                                      max_seqlen_k, block_table, topk, softmax_scale, add_weight)
+
+
+@torch.library.register_fake("flash_moba::_cache_attn")
+def _cache_attn_fake(q, k_cache, v_cache, k_scale, v_scale, k_sum, k_mean, weight, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, topk,
+                     softmax_scale, add_weight):
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+
+
 @torch.library.custom_op("flash_moba::_cache_evict", mutates_args=(), device_types="cuda")
 def _cache_evict(weight: torch.Tensor, seqlens_k: torch.Tensor, block_table: torch.Tensor, page_size: int, keep: int, sink: int,
                  recent: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -88,6 +103,50 @@ def flash_moba_cache_append_func(cache, k, v, cu_seqlens, max_seqlen, seqlens_k,
     if not torch.compiler.is_compiling() and flash_moba_gpu.host_module().cache_append(cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table):
         return
     torch.ops.flash_moba._cache_append(*cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table)
+
+
+def flash_moba_cache_attn_func(q, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, softmax_scale=None,
+                               add_weight=False, return_lse=False):
+    """MoBA attention of the last tokens of every sequence over a cache: decode steps, drafts, parts of prompts, whole prompts.
+
+    q: (tokens, num_heads, head_size) of the dtype of cache.k_mean, any strides, num_heads a multiple of the cache's heads;
+    cu_seqlens_q: (batch + 1,) int32; max_seqlen_q: the most rows of a sequence; seqlens_k, block_table: as for
+    flash_moba_cache_append_func (the rows' own keys are in the cache already); max_seqlen_k: at least the longest of seqlens_k.
+
+    Row i of a sequence has position seqlens_k - rows + i.  It sees, up to its position, the keys of its own page and of the
+    moba_topk - 1 (at most 63) pages before it whose mean key has the largest product with it, decided as in 64 bits, of equals the
+    later page; a product that is NaN or -inf selects nothing, and neither does a table entry that is no page.
+    softmax_scale defaults to head_size ** -0.5.  Rows that see no key produce 0 (and a log-sum-exp of +inf).
+
+    With add_weight=True the part of a row's softmax that a page holds is added to cache.weight (64-bit integers in units of 2^-32, so that
+    the sums do not depend on an order), which flash_moba_cache_evict_func chooses by.
+
+    Returns out, like q; with return_lse=True (out, softmax_lse (num_heads, tokens) fp32).  No backward pass.
+    """
+    res = None
+    if not torch.compiler.is_compiling():
+        res = flash_moba_gpu.host_module().cache_attn(q, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, softmax_scale, add_weight)
+    if res is None:
+        res = torch.ops.flash_moba._cache_attn(q, *cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, softmax_scale, add_weight)
+    return res if return_lse else res[0]
+
+
+def flash_moba_with_cache_func(q, k, v, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, positions=None,
+                               sections=None, base=10000.0, rotary_dim=None, interleaved=False, softmax_scale=None, add_weight=False,
+                               return_lse=False):
+    """A serving step end to end: rotary positions on q and k (with `positions`, as flash_moba_rotary_func), the keys and values of the
+    tokens into the cache (as flash_moba_cache_append_func), attention of the tokens over it (as flash_moba_cache_attn_func)."""
+    if positions is not None:
+        positions, sections, rotary_dim = rotary_form(q, positions, sections, rotary_dim)
+    if not torch.compiler.is_compiling():
+        res = flash_moba_gpu.host_module().cache_step(q, k, v, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, positions,
+                                                      sections or (), base, rotary_dim or 0, interleaved, softmax_scale, add_weight)
+        if res is not None:
+            return res if return_lse else res[0]
+    if positions is not None:
+        q, k = flash_moba_rotary_func(q, k, positions, sections, base, rotary_dim, interleaved)
+    flash_moba_cache_append_func(cache, k, v, cu_seqlens_q, max_seqlen_q, seqlens_k, block_table)
+    return flash_moba_cache_attn_func(q, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, max_seqlen_k, block_table, moba_topk, softmax_scale, add_weight, return_lse)
 
 
 def flash_moba_cache_evict_func(weight, seqlens_k, block_table, page_size, keep_pages, sink_pages=1, recent_pages=1):

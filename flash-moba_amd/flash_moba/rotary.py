@@ -32,6 +32,19 @@ def _rotary_backward(ctx, dq, dk):
 torch.library.register_autograd("flash_moba::_rotary", _rotary_backward, setup_context=_rotary_setup)
 
 
+def rotary_form(q, positions, sections, rotary_dim):
+    """The defaults: one axis, all features, all pairs on the only axis."""
+    if positions.dim() == 1:
+        positions = positions[None]
+    if rotary_dim is None:
+        rotary_dim = q.shape[-1]
+    if sections is None:
+        if positions.shape[0] != 1:
+            raise RuntimeError("positions of several axes need sections")
+        sections = (rotary_dim // 2,)
+    return positions, sections, rotary_dim
+
+
 def flash_moba_rotary_func(q, k, positions, sections=None, base=10000.0, rotary_dim=None, interleaved=False):
     """Rotary positions with several axes on packed q and k, with autograd.
 
@@ -44,14 +57,7 @@ def flash_moba_rotary_func(q, k, positions, sections=None, base=10000.0, rotary_
 
     Returns (q, k), turned, as new contiguous tensors.
     """
-    if positions.dim() == 1:
-        positions = positions[None]
-    if rotary_dim is None:
-        rotary_dim = q.shape[-1]
-    if sections is None:
-        if positions.shape[0] != 1:
-            raise RuntimeError("positions of several axes need sections")
-        sections = (rotary_dim // 2,)
+    positions, sections, rotary_dim = rotary_form(q, positions, sections, rotary_dim)
     if not torch.compiler.is_compiling():  # plain eager calls: one native call (None: not of its form)
         turned = flash_moba_gpu.host_module().rotary(q, k, positions, sections, base, rotary_dim, interleaved)
         if turned is not None:

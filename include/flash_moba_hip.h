@@ -361,6 +361,28 @@ typedef struct {
 } fmoba_cache_append_args;
 int fmoba_cache_append(const fmoba_cache_append_args *a, void *stream);
 
+/* Gated attention of query rows over the cache.  The rows of sequence b, cu_seqlens_q[b + 1] - cu_seqlens_q[b] of them, are its last tokens: row i has
+ * position p = seqlens_k[b] - rows + i and sees the keys up to p of the pages that it selects: its own, p / page_size, and of the pages before
+ * it the topk - 1 whose k_mean has the largest product with the row (decided as in 64 bits; of equals the later page; a product that is NaN or -inf
+ * selects nothing).  out = softmax(softmax_scale q k^T) v over these keys, softmax_lse (heads, total_q) its log-sum-exp; a row that sees no key gets
+ * out = 0, lse = +inf.  add_weight: every page that a row selected receives its part of the row's softmax in cache.weight.
+ * max_seqlen_k: at least the longest of seqlens_k; a table entry that is no page counts as one that was not selected.
+ * workspace: fmoba_cache_attn_workspace_bytes(a) bytes (sizes are read, pointers are not), contents undefined on entry and return. */
+typedef struct {
+  fmoba_kv_cache cache;
+  const void *q;            /* (total_q, heads, head_dim) */
+  void *out;
+  float *softmax_lse;
+  const int32_t *cu_seqlens_q, *seqlens_k, *block_table;
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t q_row_stride, q_head_stride, o_row_stride, o_head_stride, table_stride;
+  int32_t batch, total_q, heads, max_seqlen_q, max_seqlen_k, max_pages, topk, add_weight;
+  float softmax_scale;
+} fmoba_cache_attn_args;
+size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *a);
+int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream);
+
 /* Which pages a sequence keeps when it has more than `keep`: its first `sink`, its last `recent` (one at least: the page that is being filled), and of the
  * others those with the most weight, summed over heads; of equals the first.  Their order stays.  new_table and freed (batch, max_pages), dense: pages
  * kept and pages let go, in order, then -1; num_freed and new_seqlens (batch): how many, and the tokens that are left.  Nothing of

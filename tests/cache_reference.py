@@ -65,14 +65,14 @@ def append(s, k, v, cu, seqlens_k, table):
 
 
 def attention(s, q, cu, seqlens_k, table, topk, scale=None):
-    """out, lse, weight of every page and head in units of one, and the gap between the scores on either side of every row's cut
-    (infinite where nothing is cut off)."""
+    """out, lse, weight of every page and head in units of one, and what errors are relative to: sum of p |v| (rows, heads, features),
+    largest sum of scale |q| |k| (heads, rows), largest |v| (heads, rows) and number of keys (heads, rows)."""
     P, dim, heads = s["k"].shape[2], q.shape[2], q.shape[1]
     G = heads // s["k"].shape[1]
     scale = dim ** -0.5 if scale is None else scale
     out = torch.zeros(q.shape, dtype=torch.float64)
     lse = torch.full((heads, q.shape[0]), math.inf, dtype=torch.float64)
-    gap = torch.full((heads, q.shape[0]), math.inf, dtype=torch.float64)
+    size, dot, most, count = torch.zeros_like(out), torch.zeros((heads, q.shape[0])).double(), torch.zeros((heads, q.shape[0])).double(), torch.zeros((heads, q.shape[0])).double()
     weight = torch.zeros(s["k_scale"].shape, dtype=torch.float64)
     for b in range(len(seqlens_k)):
         for i in range(cu[b], cu[b + 1]):
@@ -82,25 +82,26 @@ def attention(s, q, cu, seqlens_k, table, topk, scale=None):
             for h in range(heads):
                 hk, x = h // G, q[i, h].double()
                 there = [c for c in range(pos // P + 1) if 0 <= table[b][c] < s["k"].shape[0]]
-                score = sorted(((x @ s["k_mean"][table[b][c], hk]).item(), c) for c in there if c < pos // P)[::-1]
-                score = [e for e in score if e[0] > -math.inf]
+                score = [((x @ s["k_mean"][table[b][c], hk]).item(), c) for c in there if c < pos // P]
+                score = sorted(e for e in score if e[0] > -math.inf)[::-1]
                 chosen = [c for _, c in score[:topk - 1]] + [c for c in there if c == pos // P]
-                if len(score) >= topk > 1:
-                    gap[h, i] = score[topk - 2][0] - score[topk - 1][0]
                 parts, vs = [], []
                 for c in chosen:
                     page, n = table[b][c], min(P, pos + 1 - c * P)
-                    parts.append((s["k"][page, hk, :n] * s["k_scale"][page, hk]) @ x * scale)
+                    k = s["k"][page, hk, :n] * s["k_scale"][page, hk]
+                    parts.append(k @ x * scale)
+                    dot[h, i] = max(dot[h, i].item(), (k.abs() @ x.abs()).max().item() * abs(scale))
                     vs.append(s["v"][page, hk, :n] * s["v_scale"][page, hk])
                 if not chosen:
                     continue
                 w = torch.cat(parts)
                 lse[h, i] = torch.logsumexp(w, 0)
                 p = torch.softmax(w, 0)
-                out[i, h] = p @ torch.cat(vs)
+                vs = torch.cat(vs)
+                out[i, h], size[i, h], most[h, i], count[h, i] = p @ vs, p @ vs.abs(), vs.abs().max(), len(w)
                 for c, part in zip(chosen, p.split([len(x) for x in parts])):
                     weight[table[b][c], hk] += part.sum()
-    return out, lse, weight, gap
+    return out, lse, weight, (size, dot, most, count)
 
 
 def evict(weight, seqlens_k, table, P, keep, sink, recent):

@@ -1,0 +1,427 @@
+"""flash_moba_cache_attn_func (and the whole step) against its definition in 64 bits.
+
+Which pages a row reads is decided as in 64 bits, so nothing is left out of the comparison for near-ties.  Error of an output: a score of D
+products in 32 bits is off by at most (D + 8) 2^-24 of scale sum |q| |k| (8: the scales, the change of base and the exponential's argument), the exponential
+by 2^-22, a sum of n weights by n 2^-24; weights are off by twice the first two, relatively, and an output by that times sum p |v|, and by half a
+step of its type.  Where many rows share a page, its weights and its part of an output are rounded to fp16 (2^-11 each; weights below 2^-14 by 2^-25 of the
+largest)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import cache_reference as R
+import flash_moba
+from flash_moba import flash_moba_hip as H
+from test_gpu_kv_append import BAD_CACHES, cache_struct, random_cache, tables
+
+gpu = pytest.mark.gpu
+
+
+def check(got, lse, want, want_lse, sizes, fp16_parts):
+    size, dot, most, count = sizes
+    D = got.shape[2]
+    delta = ((D + 8) * 2.0 ** -24 * dot + 2.0 ** -22)
+    weights = (2 * delta + count * 2.0 ** -24 + (2 * 2.0 ** -11 if fp16_parts else 0.0)).t()[:, :, None]
+    tol = want.abs() * torch.finfo(got.dtype).eps / 2 * 1.01 + size * weights + (2.0 ** -25 * (count * most).t()[:, :, None] if fp16_parts else 0.0) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    err = (got.float().cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"out {(err - tol).max().item():.3e} over, largest error {err.max().item():.3e}"
+    lse = lse.cpu().double()
+    assert torch.equal(torch.isinf(lse), torch.isinf(want_lse))
+    fine = torch.isfinite(want_lse)
+    assert bool(((lse - want_lse).abs()[fine] <= (delta + count * 2.0 ** -24 + 2.0 ** -22 * want_lse.abs().clamp_min(1.0))[fine]).all()), (lse - want_lse).abs()[fine].max()
+
+
+def filled_cache(pages, heads_k, P, dim, dtype, held, seed, layout="heads"):
+    """Pages with means of their own, so that rows choose by them."""
+    c = random_cache(pages, heads_k, P, dim, dtype, held, seed, layout)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    c.k_scale.copy_(torch.rand(c.k_scale.shape, generator=g, device="cuda") * 0.02 + 0.002)  # (not only powers of two)
+    c.v_scale.copy_(torch.rand(c.k_scale.shape, generator=g, device="cuda") * 0.1 + 0.001)
+    c.k_mean.normal_(generator=g)
+    return c
+
+
+def setup(heads, heads_k, dim, P, lens_q, lens_k, dtype, held, seed=1, layout="heads", spare=2):
+    pages = sum((n + P - 1) // P for n in lens_k) + spare
+    cache = filled_cache(pages, heads_k, P, dim, dtype, held, seed, layout)
+    table = tables(lens_k, P, pages, seed)
+    g = torch.Generator(device="cuda").manual_seed(seed + 2)
+    q = torch.randn((sum(lens_q), heads, dim), generator=g, device="cuda").to(dtype)
+    cu = [0]
+    for n in lens_q:
+        cu.append(cu[-1] + n)
+    return cache, table, q, cu
+
+
+def call(cache, table, q, cu, lens_k, topk, **kw):
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens_q = [b - a for a, b in zip(cu, cu[1:])]
+    return flash_moba.flash_moba_cache_attn_func(q, cache, torch.tensor(cu, **i32), kw.pop("max_q", max(lens_q)), torch.tensor(lens_k, **i32), kw.pop("max_k", max(max(lens_k), 1)),
+                                                 torch.tensor(table, **i32), topk, return_lse=True, **kw)
+
+
+CASES = [  # heads, heads_k, dim, page, lens_q, lens_k, topk
+    (1, 1, 16, 64, [1], [1], 1),
+    (4, 1, 128, 128, [1, 1, 1], [1, 128, 1000], 3),
+    (8, 8, 64, 64, [1, 0, 2], [700, 5, 641], 4),
+    (6, 2, 80, 64, [3, 8], [129, 1500], 5),
+    (4, 2, 256, 64, [5], [900], 64),
+    (2, 1, 96, 1024, [2], [3000], 2),
+    (2, 2, 48, 192, [1, 7], [64 * 40, 192 * 3], 7),
+    (4, 4, 128, 128, [8], [8], 8),                   # a prompt of a few tokens
+    (4, 2, 64, 64, [300], [300], 2),                 # whole prompts
+    (4, 1, 128, 128, [70, 1, 0, 33], [500, 300, 9, 33], 3),
+    (2, 2, 80, 64, [65, 64], [1000, 64], 9),
+    (3, 3, 256, 128, [40], [700], 4),
+    (8, 1, 32, 256, [50], [900], 1),                 # its own page alone
+    (4, 2, 112, 64, [20, 9], [64 * 30, 64 * 21 + 1], 64),
+]
+
+
+@gpu
+@pytest.mark.parametrize("held", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,heads_k,dim,P,lens_q,lens_k,topk", CASES)
+def test_outputs_are_the_definitions(held, dtype, heads, heads_k, dim, P, lens_q, lens_k, topk):
+    cache, table, q, cu = setup(heads, heads_k, dim, P, lens_q, lens_k, dtype, held, layout="tokens" if heads_k == 2 else "heads")
+    s, before = R.state(cache), cache.weight.clone()
+    out, lse = call(cache, table, q, cu, lens_k, topk, add_weight=True)
+    want, want_lse, weight, sizes = R.attention(s, q.cpu(), cu, lens_k, table, topk)
+    many = max(lens_q) > 8
+    check(out, lse, want, want_lse, sizes, many)
+    # weights: relatively as the outputs' weights, and half a unit for every visit
+    got = (cache.weight - before).cpu().double() * 2.0 ** -32
+    D = dim
+    rel = 2 * ((D + 8) * 2.0 ** -24 * sizes[1].max().item() + 2.0 ** -22) + sizes[3].max().item() * 2.0 ** -24 + 2.0 ** -22
+    rows = sum(lens_q) * heads
+    assert bool(((got - weight).abs() <= weight * rel + rows * (P // 64) * 2.0 ** -33).all()), (got - weight).abs().max()
+    # the same without weights, and once more: no bit differs
+    out2, lse2 = call(cache, table, q, cu, lens_k, topk)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    w = cache.weight.clone()
+    call(cache, table, q, cu, lens_k, topk, add_weight=True)
+    assert torch.equal(cache.weight - w, w - before)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 40])
+def test_long_contexts_with_many_pages(rows):
+    """More pages than registers (256) and, for one row, than LDS (4096) hold; few are read."""
+    for n in (300, 5000 if rows == 1 else 1100):
+        lens_k = [64 * n - 7]
+        cache, table, q, cu = setup(2, 1, 16, 64, [rows], lens_k, torch.bfloat16, torch.int8, seed=n)
+        out, lse = call(cache, table, q, cu, lens_k, 6)
+        want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, 6)
+        check(out, lse, want, want_lse, sizes, rows > 8)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 20])
+def test_ties_and_near_ties_are_decided_as_in_64_bits(rows):
+    """Means that differ in the last bits of a sum: in 32 bits the order of its terms would decide.  Equal ones: the later page."""
+    P, dim, n = 64, 64, 40
+    cache, table, q, cu = setup(2, 1, dim, P, [rows], [P * n], torch.bfloat16, torch.float8_e4m3fn)
+    base = torch.randn(dim, device="cuda").bfloat16()
+    cache.k_mean[:] = base
+    for c in range(0, n, 2):  # every other page: one feature by one step
+        page, d = table[0][c], c % dim
+        cache.k_mean[page, 0, d] = base[d].float() * (1 + 2.0 ** -7)
+    # terms of very different sizes: 2^-10 to 2^10, products of 16 bits, 64 of them: 42 bits, so that 64-bit sums are exact
+    q[:] = q[:1, :1] * 2.0 ** torch.linspace(-10, 10, dim, device="cuda").round()
+    q[:, 1] = 0  # all scores equal
+    kw = dict(softmax_scale=2.0 ** -30)  # every key of the pages chosen weighs the same
+    w = cache.weight.clone()
+    out, lse = call(cache, table, q, cu, [P * n], 5, add_weight=True, **kw)
+    want, want_lse, weight, sizes = R.attention(R.state(cache), q.cpu(), cu, [P * n], table, 5, scale=2.0 ** -30)
+    check(out, lse, want, want_lse, sizes, rows > 8)
+    assert torch.equal((cache.weight > w).cpu(), weight > 0)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 33])
+def test_what_lies_behind_a_row_is_not_seen(rows):
+    """NaN in places behind a sequence's end and behind a row, in pages that are no one's, and table entries that are no page."""
+    P, dim = 64, 64
+    lens_k = [P * 5 + 40, 70]
+    cache, table, q, cu = setup(4, 2, dim, P, [rows, rows], lens_k, torch.bfloat16, torch.float8_e4m3fn, spare=3)
+    s = R.state(cache)
+    want, want_lse, _, sizes = R.attention(s, q.cpu(), cu, lens_k, table, 3)
+    out, lse = call(cache, table, q, cu, lens_k, 3)
+    check(out, lse, want, want_lse, sizes, rows > 8)
+    nan = float("nan")
+    for b, n in enumerate(lens_k):
+        for t in (cache.k, cache.v):
+            t.view(torch.int8)[table[b][n // P], :, n % P:] = 0x7F
+    used = {p for row in table for p in row}
+    for page in set(range(cache.k.shape[0])) - used:
+        cache.k.view(torch.int8)[page], cache.v.view(torch.int8)[page] = 0x7F, 0x7F
+        cache.k_scale[page] = cache.v_scale[page] = cache.k_mean[page] = nan
+    out2, lse2 = call(cache, table, q, cu, lens_k, 3)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    # the last key of a sequence: its earlier rows do not see it
+    last = lens_k[0] - 1
+    cache.v.view(torch.int8)[table[0][last // P], :, last % P] = 0x7F
+    cache.k.view(torch.int8)[table[0][last // P], :, last % P] = 0x7F
+    out3, _ = call(cache, table, q, cu, lens_k, 3)
+    assert torch.equal(out3[:rows - 1], out[:rows - 1]) and torch.equal(out3[rows:], out[rows:]) and bool(out3[rows - 1].isnan().all())
+    # entries that are no page: not selected
+    holes = [list(row) for row in table]
+    holes[0][1], holes[0][3], holes[1][0] = -1, cache.k.shape[0], 1 << 30
+    out4, lse4 = call(cache, holes, q[:, :], cu, lens_k, 3)
+    cache.v.view(torch.int8)[table[0][last // P], :, last % P] = 0
+    cache.k.view(torch.int8)[table[0][last // P], :, last % P] = 0
+    out4, lse4 = call(cache, holes, q, cu, lens_k, 3)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, holes, 3)
+    check(out4, lse4, want, want_lse, sizes, rows > 8)
+
+
+@gpu
+def test_rows_that_see_nothing_and_lengths_that_do_not_fit():
+    P, dim = 64, 32
+    cache, table, q, cu = setup(2, 1, dim, P, [1, 12, 1], [1, 200, 64], torch.float16, torch.int8)
+    lens = [0, 5, -3]  # no token, fewer tokens than rows, less than none
+    out, lse = call(cache, table, q, cu, lens, 4, max_k=200)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens, table, 4)
+    check(out, lse, want, want_lse, sizes, True)
+    assert bool((out[:1] == 0).all()) and bool(torch.isinf(lse[:, 0]).all()) and bool((out[1:8] == 0).all())
+    # rows, tables and lengths beyond what the call says: nothing outside is read, what fits is right
+    a = call(cache, table, q, cu, [1, 200, 64], 4)
+    b = call(cache, table, q, cu, [1, 10 ** 6, 64], 4, max_k=200)
+    assert torch.equal(a[0][:1], b[0][:1]) and torch.equal(a[0][13:], b[0][13:])
+    c = call(cache, table, q, cu, [1, 200, 64], 4, max_q=3)
+    assert torch.equal(c[0][:4], a[0][:4]) and bool((c[0][4:13] == 0).all())
+    call(cache, table, q, [0, 100, 7, 900], [9, 200, 64], 4, max_k=200, max_q=12)
+    call(cache, table, q, [-5, 3, 8, 14], [9, 200, 64], 4, max_k=200, max_q=12)
+    torch.cuda.synchronize()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    none = flash_moba.flash_moba_cache_attn_func(q[:0], cache, torch.tensor([0, 0], **i32), 0, torch.tensor([9], **i32), 9, torch.tensor([[0]], **i32), 4)
+    assert none.shape == (0, 2, 32)
+    empty = flash_moba.MobaKVCache.allocate(0, P, 1, dim, torch.float16, torch.int8)
+    out, lse = call(empty, [[0], [0], [0]], q, cu, [1, 12, 1], 4)
+    assert bool((out == 0).all()) and bool(torch.isinf(lse).all())
+    out, lse = call(cache, [[], [], []], q, cu, [1, 12, 1], 4)
+    assert bool((out == 0).all()) and bool(torch.isinf(lse).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [2, 30])
+def test_values_that_are_no_ordinary_numbers(rows):
+    P, dim = 64, 32
+    cache, table, q, cu = setup(2, 2, dim, P, [rows], [64 * 6], torch.bfloat16, torch.float8_e4m3fn)
+    q[0, 0, 0], q[1, 1, 3] = float("nan"), float("inf")
+    cache.k_mean[table[0][2], 0, 5] = float("nan")   # selects nothing
+    cache.k_mean[table[0][1], 0] = -float("inf")
+    out, lse = call(cache, table, q, cu, [64 * 6], 3)
+    assert bool(out[0, 0].isnan().all()) and bool(lse[0, 0].isnan())
+    assert not bool(out[0, 1].isnan().any())
+    clean = [i for i in range(rows) if i > 1]
+    s = R.state(cache)
+    s["k_mean"][table[0][1], 0] = -1e30  # (as a finite score below all others: 6 pages, so it is never among the best 2 of 5)
+    s["k_mean"][table[0][2], 0] = float("nan")
+    qs = q.clone()
+    qs[0], qs[1] = 0, 0
+    qa = qs.abs()  # with it the product with -1e30 is negative, as with -inf
+    out, lse = call(cache, table, qa, cu, [64 * 6], 3)
+    want, want_lse, _, sizes = R.attention(s, qa.cpu(), cu, [64 * 6], table, 3)
+    pick = lambda x: x[clean] if x.dim() == 3 else x[:, clean]  # noqa: E731
+    if clean:
+        check(out[clean], lse[:, clean], pick(want), pick(want_lse), tuple(map(pick, sizes)), rows > 8)
+
+
+@gpu
+def test_strides_scales_and_broadcast():
+    P, dim = 128, 64
+    lens_q, lens_k = [1, 2], [300, 1000]
+    cache, table, q, cu = setup(4, 2, dim, P, lens_q, lens_k, torch.bfloat16, torch.int8)
+    want, lse = call(cache, table, q, cu, lens_k, 3, softmax_scale=0.3)
+    ref, ref_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, 3, scale=0.3)
+    check(want, lse, ref, ref_lse, sizes, False)
+    qkv = torch.zeros((3, 3, 4, dim), dtype=q.dtype, device="cuda")
+    qkv[:, 0] = q
+    assert torch.equal(call(cache, table, qkv[:, 0], cu, lens_k, 3, softmax_scale=0.3)[0], want)
+    assert torch.equal(call(cache, table, q.transpose(1, 2).contiguous().transpose(1, 2), cu, lens_k, 3, softmax_scale=0.3)[0], want)
+    wide = torch.full((2, 50), -1, dtype=torch.int32, device="cuda")
+    wide[:, :len(table[0])] = torch.tensor(table)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = flash_moba.flash_moba_cache_attn_func(q, cache, torch.tensor(cu, **i32), 2, torch.tensor(lens_k, **i32), 10 ** 6, wide[:, :len(table[0]) + 1], 3, softmax_scale=0.3)
+    assert torch.equal(got, want)
+    moved = cache._replace(k=cache.k.transpose(1, 2).contiguous().transpose(1, 2), v=cache.v.permute(1, 0, 2, 3).contiguous().permute(1, 0, 2, 3))
+    assert torch.equal(call(moved, table, q, cu, lens_k, 3, softmax_scale=0.3)[0], want)
+    # a page of a shared beginning, in two sequences' tables
+    table[1][0] = table[0][0]
+    out, lse = call(cache, table, q, cu, lens_k, 3)
+    ref, ref_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, 3)
+    check(out, lse, ref, ref_lse, sizes, False)
+
+
+@gpu
+def test_a_cache_whose_offsets_pass_32_bits():
+    """Pages strided so that the last ones lie more than 2^32 bytes away."""
+    P, dim, pages = 64, 128, 9
+    cache = filled_cache(pages, 1, P, dim, torch.bfloat16, torch.int8, 3)
+    stride = 1 << 29
+    big = torch.empty((pages - 1) * stride + P * dim, dtype=torch.int8, device="cuda")
+    far = cache._replace(k=big.as_strided((pages, 1, P, dim), (stride, P * dim, dim, 1)), v=big.as_strided((pages, 1, P, dim), (stride, P * dim, dim, 1)))
+    far.k.copy_(cache.k)
+    near = cache._replace(v=cache.k.clone())
+    q = torch.randn((1 + 30, 4, dim), device="cuda").bfloat16()
+    table = [[8, 1, 0, 7], [6, 2, 5, 8]]
+    a = call(far, table, q, [0, 1, 31], [250, 256], 3)
+    b = call(near, table, q, [0, 1, 31], [250, 256], 3)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    k = torch.randn((5, 1, dim), device="cuda").bfloat16() * 100
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for c in (far, near):
+        c = flash_moba.MobaKVCache(c.k, torch.empty((pages, 1, P, dim), dtype=torch.int8, device="cuda"), *[t.clone() for t in c[2:]])
+        flash_moba.flash_moba_cache_append_func(c, k, k, torch.tensor([0, 5], **i32), 5, torch.tensor([250], **i32), torch.tensor([[1, 2, 3, 8]], **i32))
+    assert torch.equal(far.k[8], near.k[8])
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 12])
+def test_a_step_replays_from_graphs_that_run_side_by_side(rows):
+    """Positions, append, attention and weights captured twice (two graphs of the same call share nothing but the cache of each) and replayed while tokens come."""
+    P, dim, heads, heads_k = 64, 64, 4, 2
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens = [200, 130]
+    table = torch.tensor(tables([400, 400], P, 20, 4), **i32)
+    caches = [filled_cache(20, heads_k, P, dim, torch.bfloat16, torch.float8_e4m3fn, 5) for _ in range(3)]
+    cu = torch.tensor([0, rows, 2 * rows], **i32)
+    seqlens = torch.tensor(lens, **i32)
+    q, k, v = (torch.randn((2 * rows, h, dim), device="cuda").bfloat16() for h in (heads, heads_k, heads_k))
+    positions = torch.arange(2 * rows, device="cuda")[None]
+
+    def step(cache):
+        return flash_moba.flash_moba_with_cache_func(q, k, v, cache, cu, rows, seqlens, 400, table, 3, positions=positions, add_weight=True)
+
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for cache in caches[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step(cache))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(4):
+        for x in (q, k, v):
+            x.normal_()
+        positions += rows
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        want = step(caches[2])
+        torch.cuda.synchronize()
+        for out, cache in zip(held, caches):
+            assert torch.equal(out, want), turn
+            assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, caches[2])), turn
+        seqlens += rows
+
+
+@gpu
+@pytest.mark.parametrize("held", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("sections", [None, (8, 12, 12)])
+def test_a_program_that_serves(held, sections):
+    """A prompt in two parts, decode steps, eviction, more decode steps, with the freed pages given out again: every step against the definition."""
+    P, dim, heads, heads_k, topk = 64, 64, 4, 2, 3
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = flash_moba.MobaKVCache.allocate(12, P, heads_k, dim, torch.bfloat16, held)
+    s, free, table, length, position = R.state(cache), list(range(12)), [], 0, 0
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for rows in (150, 300, 1, 1, 60, "evict", 1, 1, 2, 70):  # 512 tokens, 8 pages, when 4 are kept
+        if rows == "evict":
+            got = flash_moba.flash_moba_cache_evict_func(cache.weight, torch.tensor([length], **i32), torch.tensor([table], **i32), P, 4, sink_pages=1, recent_pages=2)
+            kept, lens, freed = R.evict(cache.weight.cpu(), [length], [table], P, 4, 1, 2)
+            n = got[3].item()
+            assert got[0][0, :len(kept[0])].tolist() == kept[0] and got[2][0, :n].tolist() == freed[0] and n == 4 and got[1].item() == lens[0]
+            table, length, free = kept[0], lens[0], freed[0] + free
+            continue
+        length, position = length + rows, position + rows
+        while len(table) * P < length:
+            table.append(free.pop(0))
+        q, k, v = (torch.randn((rows, h, dim), generator=g, device="cuda").bfloat16() for h in (heads, heads_k, heads_k))
+        at = torch.arange(position - rows, position, device="cuda")
+        at = at if sections is None else torch.stack([at, at % 7, at // 3])
+        args = (torch.tensor([0, rows], **i32), rows, torch.tensor([length], **i32), length, torch.tensor([table], **i32), topk)
+        out, lse = flash_moba.flash_moba_with_cache_func(q, k, v, cache, *args, positions=at, sections=sections, add_weight=True, return_lse=True)
+        q, k = flash_moba.flash_moba_rotary_func(q, k, at, sections)
+        R.append(s, k.cpu(), v.cpu(), [0, rows], [length], [table])
+        for name in ("k", "v", "k_scale", "v_scale"):
+            assert torch.equal(getattr(cache, name).float().cpu().double(), s[name]), name
+        s["k_mean"] = cache.k_mean.float().cpu().double()  # (rounded to 16 bits: what the gate reads)
+        want, want_lse, weight, sizes = R.attention(s, q.cpu(), [0, rows], [length], [table], topk)
+        check(out, lse, want, want_lse, sizes, rows > 8)
+        s["weight"] = s["weight"] + (weight * 2.0 ** 32).round().long()
+    assert bool(((cache.weight.cpu() - s["weight"]).abs() <= s["weight"].abs().double() * 1e-4 + 2.0 ** 12).all())
+
+
+@gpu
+def test_step_and_attention_from_traced_graphs():
+    P, dim = 64, 32
+    cache, table, q, cu = setup(4, 2, dim, P, [3], [200], torch.bfloat16, torch.int8)
+    other = flash_moba.MobaKVCache(*[t.clone() for t in cache])
+    i32 = dict(dtype=torch.int32, device="cuda")
+    k = torch.randn((3, 2, dim), device="cuda").bfloat16()
+    pos = torch.arange(3, device="cuda")
+    args = (torch.tensor(cu, **i32), 3, torch.tensor([200], **i32), 200, torch.tensor(table, **i32), 3)
+
+    def step(q, k, *tensors):
+        return flash_moba.flash_moba_with_cache_func(q, k, k, flash_moba.MobaKVCache(*tensors), *args, positions=pos, add_weight=True, return_lse=True)
+
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(q, k, *cache)
+    want = step(q, k, *other)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert all(torch.equal(a, b) for a, b in zip(cache, other))
+
+
+@gpu
+@pytest.mark.parametrize("change,message", [
+    (dict(q=lambda q: q.half()), "dtype"), (dict(q=lambda q: q[:, :3]), "divide"), (dict(q=lambda q: q[..., :16]), "head size"), (dict(q=lambda q: q.clone().requires_grad_(True)), "no backward"),
+    (dict(topk=0), "moba_topk"), (dict(topk=65), "moba_topk"), (dict(max_k=-1), "out of range"), (dict(cache=lambda c: c._replace(weight=None)), "keeps no weight"),
+    (dict(cache=lambda c: c._replace(k=c.k.cpu(), v=c.v.cpu())), ""), (dict(table=lambda t: t.float()), "block_table"), (dict(lens=lambda t: t[:0]), "seqlens_k"),
+])
+def test_refusals(change, message):
+    cache = flash_moba.MobaKVCache.allocate(3, 64, 2, 32)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    a = dict(q=torch.zeros((4, 4, 32), dtype=torch.bfloat16, device="cuda"), lens=torch.tensor([4], **i32), table=torch.tensor([[0]], **i32), cache=cache)
+    a = {n: change[n](t) if n in change else t for n, t in a.items()}
+    args = (torch.tensor([0, 4], **i32), 4, a["lens"], change.get("max_k", 4), a["table"], change.get("topk", 3))
+    with pytest.raises(RuntimeError, match=message):
+        flash_moba.flash_moba_cache_attn_func(a["q"], a["cache"], *args, add_weight=True)
+    # and the whole step leaves the cache as it was
+    k = torch.ones((4, 2, 32), dtype=torch.bfloat16, device="cuda")
+    before = [t.clone() for t in cache]
+    with pytest.raises(RuntimeError, match=message):
+        flash_moba.flash_moba_with_cache_func(a["q"], k, k, a["cache"], *args, add_weight=True)
+    assert all(torch.equal(x.view(torch.int8), y.view(torch.int8)) for x, y in zip(cache, before))
+
+
+def test_the_entry_point_refuses_without_a_gpu():
+    lib = H.load_library()
+    assert lib.fmoba_cache_attn(None, None) != 0 and lib.fmoba_cache_attn_workspace_bytes(None) == 0
+
+    def args(cache, **kw):
+        a = H.CacheAttnArgs()
+        a.cache = cache
+        a.q = a.out = a.softmax_lse = a.cu_seqlens_q = a.seqlens_k = a.block_table = a.workspace = 4096
+        a.batch, a.total_q, a.heads, a.max_seqlen_q, a.max_seqlen_k, a.max_pages, a.topk, a.table_stride = 2, 16, 4, 8, 500, 8, 3, 8
+        a.softmax_scale, a.workspace_bytes = 0.1, 1 << 40
+        for n in ("q_row_stride", "q_head_stride", "o_row_stride", "o_head_stride"):
+            setattr(a, n, 64)
+        for n, v in kw.items():
+            setattr(a, n, v)
+        return a
+
+    for kw, message in BAD_CACHES:
+        assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(**kw))), None) != 0, kw
+        assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
+    for kw, message in [(dict(batch=0), b"batch"), (dict(total_q=-1), b"sizes"), (dict(heads=3), b"divide"), (dict(topk=0), b"moba_topk"), (dict(topk=65), b"moba_topk"), (dict(q=0), b"null"),
+                        (dict(softmax_lse=0), b"null"), (dict(block_table=0), b"null"), (dict(q_row_stride=4), b"strides"), (dict(out=4100), b"aligned"), (dict(workspace_bytes=16), b"workspace"),
+                        (dict(workspace=4100), b"workspace"), (dict(total_q=1 << 30, heads=8), b"launch grid")]:
+        assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(), **kw)), None) != 0, kw
+        assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
+    assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(weight=0), add_weight=1)), None) != 0
+    assert b"no weight" in lib.fmoba_last_error()
+    assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(), total_q=0)), None) == 0
