@@ -39,45 +39,53 @@ __device__ __forceinline__ uint64_t score_key(double s) {
 }
 
 // ------------------------------------------------------------------------------------
-// Scores of kScoreRows (row, head of the group) pairs against 64 pages: four lanes share a page's mean, a quarter of the features each.  The pairs' queries
-// lie in LDS as doubles.  Decode steps read every mean once: memory; many rows are bound by the 64-bit products.
+// Scores of NR (row, head of the group) pairs against 64 pages: four lanes share a page's mean, a quarter of the features each.  The pairs' queries
+// lie in LDS as doubles.  A decode step reads every mean once and is bound by latency: the lengths, then the queries and the table, then the means, each once
+// and all of a lane's loads together (with the means asked for one after the other 13 us instead of XX, 16 requests with 512 to 32768 tokens, 8 key
+// heads of 128, 128-key pages).  Many rows are bound by the 64-bit products.
 // ------------------------------------------------------------------------------------
-constexpr int kScoreRows = 8, kScorePages = 64;
-template <typename T>
+constexpr int kScorePages = 64;
+template <typename T, int HD, int NR>
 __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
-  extern __shared__ double sQ[];  // [kScoreRows][D]
+  __shared__ double sQ[NR * HD];
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, tid = threadIdx.x;
   const int b = blockIdx.z / a.cache.heads_k, hk = blockIdx.z - b * a.cache.heads_k;
-  const int q0 = a.cu_seqlens_q[b], R = min(a.cu_seqlens_q[b + 1], a.total_q) - q0, pair0 = blockIdx.y * kScoreRows, c0 = blockIdx.x * kScorePages;
-  const int npairs = min((int64_t)kScoreRows, (int64_t)R * G - pair0);
+  const int c = blockIdx.x * kScorePages + (tid >> 2), part = tid & 3;
+  const int page = c < p.cols - 1 ? a.block_table[(int64_t)b * a.table_stride + c] : -1;
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
+  const int R = min(q1, a.total_q) - q0, pair0 = blockIdx.y * NR;
+  const int npairs = (int)min((int64_t)NR, (int64_t)R * G - pair0);
   if (q0 < 0 || npairs <= 0) return;
-  const int last_pos = a.seqlens_k[b] - (a.cu_seqlens_q[b + 1] - q0) + (pair0 + npairs - 1) / G;  // pairs: row by row, a row's heads one after the other
+  const int last_pos = len - (q1 - q0) + (pair0 + npairs - 1) / G;  // pairs: row by row, a row's heads one after the other
   const int npages = last_pos < 0 ? 0 : min(last_pos / P, p.cols - 1);  // that any of the rows can select beside its own
-  if (c0 >= npages) return;
-  for (int i = tid; i < kScoreRows * D; i += 256) {
-    const int r = i / D, e = i - r * D, pair = pair0 + min(r, npairs - 1);
+  if ((int)blockIdx.x * kScorePages >= npages) return;
+  const bool there = c < npages && page >= 0 && page < a.cache.num_pages;
+  const uint16_t *mean = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + ((int64_t)(there ? page : 0) * a.cache.heads_k + hk) * D;
+  constexpr int NP = HD / 32;
+  Pack8 x[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) x[i] = there && i * 32 + part * 8 < D ? ld_global16(mean + i * 32 + part * 8) : zero_pack8();
+  for (int i = tid; i < NR * HD; i += 256) {
+    const int r = i / HD, e = i % HD, pair = pair0 + min(r, npairs - 1);
     const int row = q0 + pair / G, h = hk * G + pair % G;
-    sQ[i] = (double)elem_to_float<T>(reinterpret_cast<const uint16_t *>(a.q)[(int64_t)row * a.q_row_stride + (int64_t)h * a.q_head_stride + e]);
+    sQ[i] = e < D ? (double)elem_to_float<T>(reinterpret_cast<const uint16_t *>(a.q)[(int64_t)row * a.q_row_stride + (int64_t)h * a.q_head_stride + e]) : 0.0;
   }
   __syncthreads();
-  const int c = c0 + (tid >> 2), part = tid & 3;
-  const int page = c < npages ? a.block_table[(int64_t)b * a.table_stride + c] : -1;
-  const bool there = page >= 0 && page < a.cache.num_pages;
-  const uint16_t *mean = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + ((int64_t)(there ? page : 0) * a.cache.heads_k + hk) * D;
-  double acc[kScoreRows];
+  double acc[NR];
 #pragma unroll
-  for (int r = 0; r < kScoreRows; ++r) acc[r] = 0.0;
-  for (int e = part * 8; e < D; e += 32) {
+  for (int r = 0; r < NR; ++r) acc[r] = 0.0;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
     float f[8];
-    unpack8<T>(there ? ld_global16(mean + e) : zero_pack8(), f);
+    unpack8<T>(x[i], f);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int r = 0; r < kScoreRows; ++r) acc[r] = fma((double)f[j], sQ[r * D + e + j], acc[r]);
+      for (int r = 0; r < NR; ++r) acc[r] = fma((double)f[j], sQ[r * HD + i * 32 + part * 8 + j], acc[r]);
   }
 #pragma unroll
-  for (int r = 0; r < kScoreRows; ++r) {
+  for (int r = 0; r < NR; ++r) {
     double s = acc[r];
     s += __shfl_xor(s, 1, 64);
     s += __shfl_xor(s, 2, 64);
@@ -92,72 +100,69 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
 }
 
 // ------------------------------------------------------------------------------------
-// The best `want` of a row's nc candidates, by one wave, into `chosen` (any order); returns how many.  The upper halves of the keys decide but for ties: the
-// largest cut that leaves `want` of them at or above it is found bit by bit, a count is a ballot; of those that share the cut the lower halves
-// decide, then the later page.  `hi` in registers for up to 256 candidates, else in LDS or, from kPickLds on, where the scores are.
+// The best `want` of n candidates, by one wave: take(candidate, upper half of its key, place) for each, in any order, by the lane that holds it; returns how many.  hi(i) and lo(i)
+// are the halves of candidate i's key, id(i) decides between equal keys (the larger).  The upper halves decide but for ties: the largest cut that leaves
+// `want` of them at or above it is found bit by bit, a count is a ballot; of those that share the cut the lower halves decide.
+// The upper halves are in registers for up to 64 NJ candidates, NJ = 0: asked for each time.
 // ------------------------------------------------------------------------------------
-constexpr int kPickLds = 4096;
-template <int NJ>
-__device__ __forceinline__ int pick_pages(const uint32_t *key_hi, const uint32_t *key_lo, int nc, int want, int lane, uint32_t *keys, int *chosen) {
-  if (want <= 0 || nc <= 0) return 0;
-  const int places = NJ > 0 ? NJ : (nc + 63) / 64;
-  const bool in_lds = NJ == 0 && nc <= kPickLds;
+template <int NJ, typename Hi, typename Lo, typename Id, typename Take>
+__device__ __forceinline__ int pick_best(int n, int want, int lane, Hi hi, Lo lo, Id id, Take take) {
+  if (want <= 0 || n <= 0) return 0;
+  const int places = NJ > 0 ? NJ : (n + 63) / 64;
   uint32_t reg[NJ > 0 ? NJ : 1];
   if constexpr (NJ > 0) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) reg[j] = j * 64 + lane < nc ? key_hi[j * 64 + lane] : 0u;
-  } else if (in_lds) {
-    for (int j = 0; j < places; ++j) keys[j * 64 + lane] = j * 64 + lane < nc ? key_hi[j * 64 + lane] : 0u;
+    for (int j = 0; j < NJ; ++j) reg[j] = j * 64 + lane < n ? hi(j * 64 + lane) : 0u;
   }
   auto each = [&](auto &&f) {  // f(candidate, its upper half), all lanes at once
     if constexpr (NJ > 0) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) f(j * 64 + lane, reg[j]);
     } else {
-      for (int j = 0; j < places; ++j) {
-        const int c = j * 64 + lane;
-        f(c, in_lds ? keys[c] : c < nc ? key_hi[c] : 0u);  // (its own lane wrote it)
-      }
+      for (int j = 0; j < places; ++j) f(j * 64 + lane, j * 64 + lane < n ? hi(j * 64 + lane) : 0u);
     }
   };
   auto count_ge = [&](uint32_t v) {
-    int n = 0;
-    each([&](int, uint32_t k) { n += __popcll(__ballot(k >= v)); });
-    return n;
+    int m = 0;
+    each([&](int, uint32_t k) { m += __popcll(__ballot(k >= v)); });
+    return m;
   };
-  const int all = count_ge(1u);
   uint32_t cut = 1u;
-  int n_cut = all;
-  if (all > want) {
+  int n_cut = count_ge(1u);
+  if (n_cut > want) {
     cut = 0u;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t trial = cut | (1u << bit);
-      const int n = count_ge(trial);
-      if (n >= want) cut = trial, n_cut = n;
-      if (n == want) break;
+      const int m = count_ge(trial);
+      if (m >= want) cut = trial, n_cut = m;
+      if (m == want) break;
     }
   }
   const bool tie = n_cut > want;
   int total = 0;
   each([&](int c, uint32_t k) {
-    const unsigned long long m = __ballot(tie ? k > cut : k >= cut);
-    if ((m >> lane) & 1ull) chosen[total + __popcll(m & ((1ull << lane) - 1ull))] = c;
+    const bool in = tie ? k > cut : k >= cut;
+    const unsigned long long m = __ballot(in);
+    if (in) take(c, k, total + __popcll(m & ((1ull << lane) - 1ull)));
     total += __popcll(m);
   });
-  for (uint64_t below = ~0ull; tie && total < want; ++total) {  // the best of those that share the cut, one by one
-    uint64_t best = 0ull;
+  uint64_t below = ~0ull;
+  for (; tie && total < want; ++total) {  // the best of those that share the cut, one by one
+    uint64_t best = 0ull;  // lower half + 1 | id: of 64 bits the upper 33 and the lower 31 (ids are pages of a table)
+    int mine = -1;
     each([&](int c, uint32_t k) {
       if (k != cut) return;
-      const uint64_t x = (uint64_t)key_lo[c] << 32 | (uint32_t)(c + 1);
-      if (x < below && x > best) best = x;
+      const uint64_t x = ((uint64_t)lo(c) + 1) << 31 | (uint32_t)id(c);
+      if (x < below && x > best) best = x, mine = c;
     });
+    uint64_t top = best;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
-      const uint64_t y = __shfl_xor(best, o, 64);
-      best = y > best ? y : best;
+      const uint64_t y = __shfl_xor(top, o, 64);
+      top = y > top ? y : top;
     }
-    if (lane == 0) chosen[total] = (int)(uint32_t)best - 1;
-    below = best;
+    if (mine >= 0 && best == top) take(mine, cut, total);  // (ids differ: one lane)
+    below = top;
   }
   return total;
 }
@@ -167,6 +172,8 @@ __device__ __forceinline__ int pick_pages(const uint32_t *key_hi, const uint32_t
 // LPR lanes a key.
 // ------------------------------------------------------------------------------------
 constexpr int kRowWaves = 8, kUnitKeys = 64;
+constexpr int kOwnScores = 1024;  // candidates of a row that its workgroup scores itself, at most
+constexpr int kPickAlone = 256;  // candidates that one wave chooses from
 constexpr int kUnitsWithWeight = 1024;  // units of a row, at most: 64 pages of 1024 keys
 
 template <int LPR>
@@ -176,12 +183,62 @@ __device__ __forceinline__ float sum_key_lanes(float x) {  // over the LPR conse
   return x;
 }
 
-template <typename T, typename H, int HD, bool WEIGHT>
-__global__ __launch_bounds__(64 * kRowWaves, 2) void cache_attn_row_kernel(CacheAttn p) {
+// The scores of one row against its nc candidates by a whole workgroup: four lanes a page, 16 pages a wave, two of them in flight.
+template <typename T, int HD>
+__device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t, int h, int hk, int nc, const int32_t *table, uint32_t *key_hi, uint32_t *key_lo) {
+  constexpr int NP = HD / 32, TURN = kRowWaves * 16;
+  const int D = a.cache.head_dim, tid = threadIdx.x, part = tid & 3;
+  const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)t * a.q_row_stride + (int64_t)h * a.q_head_stride + part * 8;
+  Pack8 q[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) q[i] = i * 32 + part * 8 < D ? ld_global16(src + i * 32) : zero_pack8();
+  for (int c0 = 0; c0 < nc; c0 += 2 * TURN) {
+    int page[2];
+    Pack8 x[2][NP];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = c0 + u * TURN + (tid >> 2);
+      page[u] = c < nc ? table[c] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool there = page[u] >= 0 && page[u] < a.cache.num_pages;
+      const uint16_t *mean = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + ((int64_t)(there ? page[u] : 0) * a.cache.heads_k + hk) * D + part * 8;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) x[u][i] = there && i * 32 + part * 8 < D ? ld_global16(mean + i * 32) : zero_pack8();
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        float f[8], g[8];
+        unpack8<T>(x[u][i], f);
+        unpack8<T>(q[i], g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fma((double)f[j], (double)g[j], s);
+      }
+      s += __shfl_xor(s, 1, 64);
+      s += __shfl_xor(s, 2, 64);
+      const int c = c0 + u * TURN + (tid >> 2);
+      if (part == 0 && c < nc) {
+        const uint64_t key = page[u] >= 0 && page[u] < a.cache.num_pages ? score_key(s) : 0ull;
+        key_hi[c] = (uint32_t)(key >> 32);
+        key_lo[c] = (uint32_t)key;
+      }
+    }
+  }
+}
+
+// SCORES: the workgroup scores its row's candidates itself, as cache_scores_kernel does, into LDS.
+template <typename T, typename H, int HD, bool WEIGHT, bool SCORES>
+__global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_row_kernel(CacheAttn p) {
   constexpr int LPR = HD / 16, KPI = 64 / LPR, NIN = kUnitKeys / KPI;
   const fmoba_cache_attn_args &a = p.a;
-  __shared__ int sChosen[64], sCount;
-  __shared__ uint32_t sKeys[kPickLds];
+  __shared__ int sChosen[64], sCount, sPages[64];
+  __shared__ float sScaleK[64], sScaleV[64];
+  __shared__ uint32_t sHi[kRowWaves * 64], sKeyHi[SCORES ? kOwnScores : 1], sKeyLo[SCORES ? kOwnScores : 1];
+  __shared__ int sPage[kRowWaves * 64];
   __shared__ float sAcc[kRowWaves][HD], sM[kRowWaves], sL[kRowWaves];
   __shared__ float sUnitM[WEIGHT ? kUnitsWithWeight : 1], sUnitL[WEIGHT ? kUnitsWithWeight : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -193,20 +250,42 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void cache_attn_row_kernel(Cache
   const int hk = h / (a.heads / a.cache.heads_k);
   const int own = at.pos >= 0 ? at.pos / P : 0, kend = at.pos + 1;
   const int32_t *table = a.block_table + (int64_t)(at.b < a.batch ? at.b : 0) * a.table_stride;
-  if (wave == 0) {
-    int n = 0;
-    if (at.pos >= 0) {
-      const int64_t keys = ((int64_t)t * a.heads + h) * p.cols;
-      const int nc = min(own, p.cols - 1);  // (a sequence longer than max_seqlen_k: what lies behind is not looked at)
-      n = nc <= 256 ? pick_pages<4>(p.key_hi + keys, p.key_lo + keys, nc, a.topk - 1, lane, sKeys, sChosen)
-                    : pick_pages<0>(p.key_hi + keys, p.key_lo + keys, nc, a.topk - 1, lane, sKeys, sChosen);
-      const int page = own < p.cols ? table[own] : -1;
-      if (page >= 0 && page < a.cache.num_pages) {
-        if (lane == 0) sChosen[n] = own;
-        ++n;
-      }
+  // ---- the pages of the row ----
+  const int64_t keys = ((int64_t)t * a.heads + h) * p.cols;
+  const uint32_t *key_hi = SCORES ? sKeyHi : p.key_hi + keys, *key_lo = SCORES ? sKeyLo : p.key_lo + keys;
+  const int nc = at.pos >= 0 ? min(own, p.cols - 1) : 0;  // (a sequence longer than max_seqlen_k: what lies behind is not looked at)
+  const int want = a.topk - 1;
+  if constexpr (SCORES) {
+    if (want > 0 && nc > 0) {
+      score_row<T, HD>(a, t, h, hk, nc, table, sKeyHi, sKeyLo);
+      __syncthreads();
     }
-    if (lane == 0) sCount = n;
+  }
+  auto chosen = [&](int c, uint32_t, int i) { sChosen[i] = c; };
+  int picked = 0;
+  if (nc <= kPickAlone) {
+    if (wave == 0)
+      picked = pick_best<kPickAlone / 64>(nc, want, lane, [&](int c) { return key_hi[c]; }, [&](int c) { return key_lo[c]; }, [](int c) { return c; }, chosen);
+  } else {  // the best of every eighth of the candidates, then the best of these
+    const int seg = ((nc + kRowWaves - 1) / kRowWaves + 63) / 64 * 64, c0 = wave * seg, n = min(seg, nc - c0);
+    auto hi = [&](int c) { return key_hi[c0 + c]; };
+    auto lo = [&](int c) { return key_lo[c0 + c]; };
+    auto id = [&](int c) { return c0 + c; };
+    auto take = [&](int c, uint32_t k, int i) { sHi[wave * 64 + i] = k, sPage[wave * 64 + i] = c0 + c; };
+    const int found = seg <= 256 ? pick_best<4>(n, want, lane, hi, lo, id, take) : seg <= 1024 ? pick_best<16>(n, want, lane, hi, lo, id, take) : pick_best<0>(n, want, lane, hi, lo, id, take);
+    for (int i = found + lane; i < 64; i += 64) sHi[wave * 64 + i] = 0u;
+    __syncthreads();
+    if (wave == 0)
+      picked = pick_best<kRowWaves>(kRowWaves * 64, want, lane, [&](int i) { return sHi[i]; }, [&](int i) { return key_lo[sPage[i]]; }, [&](int i) { return sPage[i]; },
+                                    [&](int i, uint32_t, int at) { sChosen[at] = sPage[i]; });
+  }
+  if (wave == 0) {
+    const int page = at.pos >= 0 && own < p.cols ? table[own] : -1;
+    const bool has_own = page >= 0 && page < a.cache.num_pages;
+    if (lane == 0) {
+      if (has_own) sChosen[picked] = own;
+      sCount = picked + (has_own ? 1 : 0);
+    }
   }
   const int e = (lane % LPR) * 16, ec = min(e, D - 16);
   float q[16];
@@ -219,21 +298,29 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void cache_attn_row_kernel(Cache
     for (int j = 0; j < 8; ++j) q[j] = e < D ? lo[j] : 0.f, q[8 + j] = e < D ? hi[j] : 0.f;
   }
   __syncthreads();
+  if (tid < sCount) {  // where the pages lie, and their scales
+    const int64_t page = table[sChosen[tid]];
+    const bool there = page >= 0 && page < a.cache.num_pages;  // (it was when it was scored)
+    sPages[tid] = there ? (int)page : -1;
+    sScaleK[tid] = there ? a.cache.k_scale[page * a.cache.heads_k + hk] : 0.f;
+    sScaleV[tid] = there ? a.cache.v_scale[page * a.cache.heads_k + hk] : 0.f;
+  }
+  __syncthreads();
   const int upc = P / kUnitKeys, nunit = sCount * upc;
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
   float m = -INFINITY, l = 0.f, acc[16];  // l and acc: over this lane's keys (every KPI-th)
 #pragma unroll
   for (int j = 0; j < 16; ++j) acc[j] = 0.f;
   for (int u = wave; u < nunit; u += kRowWaves) {
-    const int c = sChosen[u / upc], in_page = (u % upc) * kUnitKeys, key0 = c * P + in_page;
-    const int64_t page = table[c];
-    if (key0 >= kend || page < 0 || page >= a.cache.num_pages) {  // (only pages of the cache are chosen, unless another stream changes the table meanwhile)
+    const int n_page = u / upc, c = sChosen[n_page], in_page = (u - n_page * upc) * kUnitKeys;
+    const int64_t page = sPages[n_page];
+    if (c * P + in_page >= kend || page < 0) {
       if (WEIGHT && lane == 0) sUnitM[u] = -INFINITY, sUnitL[u] = 0.f;
       continue;
     }
     const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride + ec;
     const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride + ec;
-    const float ks = a.cache.k_scale[page * a.cache.heads_k + hk] * scale_log2, vs = a.cache.v_scale[page * a.cache.heads_k + hk];
+    const float ks = sScaleK[n_page] * scale_log2, vs = sScaleV[n_page];
     const int r0 = in_page + lane / LPR, last = kend - 1 - c * P;  // keys behind the row's own are copies of it: what lies there may be anything
     Pack8 kx[NIN], vx[NIN];
 #pragma unroll
@@ -311,49 +398,69 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void cache_attn_row_kernel(Cache
   if constexpr (WEIGHT) {
     for (int u = tid; u < nunit; u += 64 * kRowWaves) {
       const float part = __builtin_amdgcn_exp2f(sUnitM[u] - Mref) * sUnitL[u] / L;  // (a unit past the row: 0)
-      if (part > 0.f) atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)table[sChosen[u / upc]] * a.cache.heads_k + hk, (unsigned long long)rintf(part * 4294967296.f));
+      if (part > 0.f) atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)sPages[u / upc] * a.cache.heads_k + hk, (unsigned long long)rintf(part * 4294967296.f));
     }
   }
 }
 
-template <typename T, typename H, bool WEIGHT>
+static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
+// whether the rows' workgroups score their pages themselves
+static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= kOwnScores; }
+
+template <typename T, typename H, bool WEIGHT, bool SCORES>
 static void launch_rows(const CacheAttn &p, hipStream_t s) {
   const dim3 grid((uint32_t)p.a.total_q * p.a.heads), block(64 * kRowWaves);
   if (p.a.cache.head_dim <= 64)
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 64, WEIGHT>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 64, WEIGHT, SCORES>), grid, block, 0, s, p);
   else if (p.a.cache.head_dim <= 128)
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 128, WEIGHT>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 128, WEIGHT, SCORES>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 256, WEIGHT>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 256, WEIGHT, SCORES>), grid, block, 0, s, p);
+}
+template <typename T, typename H>
+static void launch_rows_as(const CacheAttn &p, bool scores, hipStream_t s) {
+  if (p.a.add_weight)
+    scores ? launch_rows<T, H, true, true>(p, s) : launch_rows<T, H, true, false>(p, s);
+  else
+    scores ? launch_rows<T, H, false, true>(p, s) : launch_rows<T, H, false, false>(p, s);
+}
+
+template <typename T, int HD>
+static int launch_scores(const CacheAttn &p, hipStream_t s) {
+  const fmoba_cache_attn_args &a = p.a;
+  const int64_t pairs = (int64_t)a.max_seqlen_q * (a.heads / a.cache.heads_k);
+  const int nr = pairs <= 1 ? 1 : pairs <= 2 ? 2 : pairs <= 4 ? 4 : 8;
+  const int64_t turns = ceil_div64(pairs, nr), z = (int64_t)a.batch * a.cache.heads_k;
+  FMOBA_REQUIRE(turns <= 65535 && z <= 65535, "cache_attn: too many rows, or sequences times heads, for the launch grid");
+  const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)turns, (uint32_t)z);
+  auto kern = nr == 1 ? cache_scores_kernel<T, HD, 1> : nr == 2 ? cache_scores_kernel<T, HD, 2> : nr == 4 ? cache_scores_kernel<T, HD, 4> : cache_scores_kernel<T, HD, 8>;
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
+  return 0;
 }
 
 template <typename T>
 static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
-  if (p.cols > 1 && a.topk > 1) {
-    const int64_t pairs = (int64_t)a.max_seqlen_q * (a.heads / a.cache.heads_k);
-    const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)ceil_div64(pairs, kScoreRows), (uint32_t)a.batch * a.cache.heads_k);
-    FMOBA_REQUIRE(grid.y <= 65535 && (int64_t)a.batch * a.cache.heads_k <= 65535, "cache_attn: too many rows, or sequences times heads, for the launch grid");
-    hipLaunchKernelGGL((cache_scores_kernel<T>), grid, dim3(256), (size_t)kScoreRows * D * 8, s, p);
+  const bool own = own_scores(a);
+  if (!own && p.cols > 1 && a.topk > 1) {
+    if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
     FMOBA_LAUNCH_CHECK("cache_scores_kernel");
   }
   if (a.cache.format == FMOBA_CACHE_E4M3)
-    a.add_weight ? launch_rows<T, HeldE4M3, true>(p, s) : launch_rows<T, HeldE4M3, false>(p, s);
+    launch_rows_as<T, HeldE4M3>(p, own, s);
   else
-    a.add_weight ? launch_rows<T, HeldInt8, true>(p, s) : launch_rows<T, HeldInt8, false>(p, s);
+    launch_rows_as<T, HeldInt8>(p, own, s);
   FMOBA_LAUNCH_CHECK("cache_attn_row_kernel");
   return 0;
 }
-
-static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
 
 }  // namespace fmoba
 
 extern "C" size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *a) {
   using namespace fmoba;
   if (a == nullptr || a->total_q <= 0 || a->heads <= 0 || a->max_seqlen_k <= 0 || a->max_pages <= 0 || a->cache.page_size <= 0) return 0;
-  return (size_t)a->total_q * a->heads * cache_cols(*a) * 8;
+  return own_scores(*a) ? 0 : (size_t)a->total_q * a->heads * cache_cols(*a) * 8;
 }
 
 extern "C" int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream) {
