@@ -19,7 +19,7 @@ HOST_MODULE = "flash_moba_host"  # the eager host path (csrc/torch_ops.cpp), a P
 HOST_LIB = os.path.join(LIBDIR, HOST_MODULE + ".so")
 HOST_SOURCES = ["torch_ops.cpp", "torch_cache_ops.cpp"]
 SOURCES = ["fmoba_host.hip", "mean_pool.hip", "topk_csc.hip", "varlen_sort.hip", "attn_fwd.hip", "attn_fwd_rows.hip", "attn_fwd_rows_wide.hip", "attn_fwd_few.hip", "attn_bwd.hip", "attn_bwd_wide.hip",
-           "rotary.hip", "kv_append.hip", "kv_evict.hip", "kv_attn.hip"]
+           "rotary.hip", "kv_append.hip", "kv_evict.hip", "kv_attn.hip", "kv_attn_columns.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # keep packed-fp32 VALU ops out of the generated code

@@ -3,40 +3,11 @@
 //                                           would let the order of a sum decide which page a row reads
 //   out = sum_j p_j v_j s_v[page of j] / sum_j p_j,   p_j = exp(scale s_k[page of j] (q . k_j) - m)
 // The scale of a page is the same for all of its keys and multiplies a whole score or weight, never a feature.
-#include "kv_cache.h"
+#include "kv_attn.h"
 
 #include <algorithm>
 
 namespace fmoba {
-
-struct CacheAttn {
-  fmoba_cache_attn_args a;
-  uint32_t *key_hi, *key_lo;  // [(row, head)][page of the table]: order keys of the scores, 0: no candidate
-  int32_t cols;               // pages of a sequence, at most
-};
-
-// position of a row, the sequence and its table
-struct RowPlace {
-  int b, row, pos;  // pos < 0: the row sees nothing
-};
-__device__ __forceinline__ RowPlace find_row(const fmoba_cache_attn_args &a, int t) {
-  const int lane = threadIdx.x & 63;
-  int b = 0;  // sequences that end at or before the row (empty ones included) come first
-  for (int b0 = 0; b0 < a.batch; b0 += 64) b += __popcll(__ballot(b0 + lane < a.batch && a.cu_seqlens_q[b0 + lane + 1] <= t));
-  RowPlace r{b, 0, -1};
-  if (b >= a.batch) return r;
-  const int q0 = a.cu_seqlens_q[b];
-  r.row = t - q0;
-  r.pos = q0 < 0 || r.row < 0 || r.row >= a.max_seqlen_q ? -1 : a.seqlens_k[b] - (a.cu_seqlens_q[b + 1] - t);
-  return r;
-}
-
-// order of a score among the candidates of a row: larger is better, 0 is none
-__device__ __forceinline__ uint64_t score_key(double s) {
-  if (!(s > -INFINITY)) return 0ull;
-  const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);  // (-0 is 0)
-  return (u >> 63) ? ~u : u | (1ull << 63);
-}
 
 // ------------------------------------------------------------------------------------
 // Scores of NR (row, head of the group) pairs against 64 pages: four lanes share a page's mean, a quarter of the features each.  The pairs' queries
@@ -97,74 +68,6 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
       p.key_lo[at] = (uint32_t)key;
     }
   }
-}
-
-// ------------------------------------------------------------------------------------
-// The best `want` of n candidates, by one wave: take(candidate, upper half of its key, place) for each, in any order, by the lane that holds it; returns how many.  hi(i) and lo(i)
-// are the halves of candidate i's key, id(i) decides between equal keys (the larger).  The upper halves decide but for ties: the largest cut that leaves
-// `want` of them at or above it is found bit by bit, a count is a ballot; of those that share the cut the lower halves decide.
-// The upper halves are in registers for up to 64 NJ candidates, NJ = 0: asked for each time.
-// ------------------------------------------------------------------------------------
-template <int NJ, typename Hi, typename Lo, typename Id, typename Take>
-__device__ __forceinline__ int pick_best(int n, int want, int lane, Hi hi, Lo lo, Id id, Take take) {
-  if (want <= 0 || n <= 0) return 0;
-  const int places = NJ > 0 ? NJ : (n + 63) / 64;
-  uint32_t reg[NJ > 0 ? NJ : 1];
-  if constexpr (NJ > 0) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) reg[j] = j * 64 + lane < n ? hi(j * 64 + lane) : 0u;
-  }
-  auto each = [&](auto &&f) {  // f(candidate, its upper half), all lanes at once
-    if constexpr (NJ > 0) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) f(j * 64 + lane, reg[j]);
-    } else {
-      for (int j = 0; j < places; ++j) f(j * 64 + lane, j * 64 + lane < n ? hi(j * 64 + lane) : 0u);
-    }
-  };
-  auto count_ge = [&](uint32_t v) {
-    int m = 0;
-    each([&](int, uint32_t k) { m += __popcll(__ballot(k >= v)); });
-    return m;
-  };
-  uint32_t cut = 1u;
-  int n_cut = count_ge(1u);
-  if (n_cut > want) {
-    cut = 0u;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = cut | (1u << bit);
-      const int m = count_ge(trial);
-      if (m >= want) cut = trial, n_cut = m;
-      if (m == want) break;
-    }
-  }
-  const bool tie = n_cut > want;
-  int total = 0;
-  each([&](int c, uint32_t k) {
-    const bool in = tie ? k > cut : k >= cut;
-    const unsigned long long m = __ballot(in);
-    if (in) take(c, k, total + __popcll(m & ((1ull << lane) - 1ull)));
-    total += __popcll(m);
-  });
-  uint64_t below = ~0ull;
-  for (; tie && total < want; ++total) {  // the best of those that share the cut, one by one
-    uint64_t best = 0ull;  // lower half + 1 | id: of 64 bits the upper 33 and the lower 31 (ids are pages of a table)
-    int mine = -1;
-    each([&](int c, uint32_t k) {
-      if (k != cut) return;
-      const uint64_t x = ((uint64_t)lo(c) + 1) << 31 | (uint32_t)id(c);
-      if (x < below && x > best) best = x, mine = c;
-    });
-    uint64_t top = best;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const uint64_t y = __shfl_xor(top, o, 64);
-      top = y > top ? y : top;
-    }
-    if (mine >= 0 && best == top) take(mine, cut, total);  // (ids differ: one lane)
-    below = top;
-  }
-  return total;
 }
 
 // ------------------------------------------------------------------------------------
@@ -404,6 +307,8 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
 }
 
 static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
+// whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own
+static bool many_rows(const fmoba_cache_attn_args &a, int cols) { return cols > 0 && a.max_seqlen_q > 8; }
 // whether the rows' workgroups score their pages themselves
 static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= kOwnScores; }
 
@@ -442,6 +347,7 @@ template <typename T>
 static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
+  if (many_rows(a, p.cols)) return run_cache_columns(p, s);
   const bool own = own_scores(a);
   if (!own && p.cols > 1 && a.topk > 1) {
     if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
@@ -460,6 +366,9 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
 extern "C" size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *a) {
   using namespace fmoba;
   if (a == nullptr || a->total_q <= 0 || a->heads <= 0 || a->max_seqlen_k <= 0 || a->max_pages <= 0 || a->cache.page_size <= 0) return 0;
+  const int cols = a->cache.num_pages > 0 ? cache_cols(*a) : 0;
+  if (cols == 0) return 0;
+  if (many_rows(*a, cols)) return column_workspace_bytes(*a, cols);
   return own_scores(*a) ? 0 : (size_t)a->total_q * a->heads * cache_cols(*a) * 8;
 }
 

@@ -1,0 +1,665 @@
+// Gated attention over the paged 8-bit cache for many rows (parts of prompts, whole prompts): three launches.
+//   gate     32 rows of a head: scores by matrix products in 32 bits, the best pages of every row; a row whose cut lies closer than the error of such a score
+//            decides again in 64 bits.  Leaves the pages of every row, and for every page a word with one bit per row.
+//   columns  a page of a key head and the rows that selected it, read from these words, 32 to a wave: S^T = K Q^T, softmax over the page, O^T = V^T P^T.
+//            A page is brought into LDS once for all of them, widened to 16 bits, exactly; its scales multiply scores and the result of a visit.
+//            Every visit leaves its output over the page and the logarithm of its sum.
+//   combine  adds a row's visits.
+// The weights of a visit are at most 1 and its output, in units of the page's scale, at most 448: both are kept in fp16, whatever the type of q (in bf16 each
+// would cost eight times its error; fp16 leaves 2^-12 of the output beside the 2^-9 of a bf16 one).
+#include "kv_attn.h"
+
+#include <algorithm>
+
+namespace fmoba {
+
+constexpr int kTileRows = 32;  // rows of a head that share a word of bits
+
+struct ColumnPlan {
+  CacheAttn c;
+  int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
+  uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
+  float *scores;     // [block of 32 rows][head][32][cols], where LDS does not hold them
+  float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum, scale of its page's values
+  uint16_t *part;    // [(row, head)][topk4][head_dim]: its output in units of that scale, fp16
+  int32_t topk4;     // topk, rounded up to a multiple of four
+  int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
+  int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
+  int32_t parts, words;  // workgroups of a page, and the words that each of them looks at
+};
+
+// The first block of a sequence: those of a sequence of n rows from q0 on are ceil(n / 32) <= floor((q0 + n) / 32) - floor(q0 / 32) + 1.
+__device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRows + b; }
+
+// ------------------------------------------------------------------------------------
+// gate
+// ------------------------------------------------------------------------------------
+constexpr int kGateCols = 1024;  // pages of a table whose scores of 32 rows LDS holds (128 KB)
+
+// row . mean of a page in 64 bits, by 16 lanes (four pages a wave)
+template <typename T>
+__device__ __forceinline__ double row16_dot(const uint16_t *q, const uint16_t *mean, int D, int lane) {
+  double s = 0.0;
+  for (int e = (lane & 15) * 8; e < D; e += 128) {
+    float f[8], g[8];
+    unpack8<T>(ld_global16(q + e), f);
+    unpack8<T>(ld_global16(mean + e), g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fma((double)f[j], (double)g[j], s);
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  return s;
+}
+template <typename T>
+__device__ __forceinline__ double lane_dot(const uint16_t *q, const uint16_t *mean, int D) {
+  double s = 0.0;
+  for (int e = 0; e < D; ++e) s = fma((double)elem_to_float<T>(q[e]), (double)elem_to_float<T>(mean[e]), s);
+  return s;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+template <typename T, int HD, bool LDS>
+__global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p) {
+  constexpr int KS = HD / 16;
+  extern __shared__ uint32_t smem[];  // bits of every page, then (LDS) the scores
+  __shared__ float sQ2[kTileRows], sMean2[4];
+  const fmoba_cache_attn_args &a = p.c.a;
+  const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
+  const int rb = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / G, cols = p.c.cols;
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
+  const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q), row0 = rb * kTileRows;
+  if (q0 < 0 || row0 >= R) return;
+  const int shift = len - (q1 - q0);  // position of row 0
+  const int rows = min(kTileRows, R - row0), last = shift + row0 + rows - 1;
+  const int npages = min((int)(((int64_t)max(len, 0) + P - 1) / P), cols);  // of the sequence
+  const int nscore = last < 0 ? 0 : min(last / P, cols - 1);                // that any of the rows can select beside its own
+  const int32_t *table = a.block_table + (int64_t)b * a.table_stride;
+  uint32_t *sBits = smem;
+  float *scores = LDS ? reinterpret_cast<float *>(smem + cols) : p.scores + ((block_of(q0, b) + rb) * a.heads + h) * kTileRows * cols;
+  for (int i = tid; i < npages; i += 256) sBits[i] = 0u;
+  const uint16_t *qh = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row0) * a.q_row_stride + (int64_t)h * a.q_head_stride;
+  const uint16_t *means = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + (int64_t)hk * D;
+  const int64_t mean_stride = (int64_t)a.cache.heads_k * D;
+
+  // ---- scores: 32 rows by 32 pages a wave and turn ----
+  if (a.topk > 1 && nscore > 0) {
+    Pack8 q[KS];
+    float q2 = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int e = ks * 16 + hh * 8;
+      q[ks] = e < D ? ld_global16(qh + (int64_t)min(li, rows - 1) * a.q_row_stride + e) : zero_pack8();
+      float f[8];
+      unpack8<T>(q[ks], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q2 = fmaf(f[j], f[j], q2);
+    }
+    q2 = sum_xor32_f(q2);
+    if (wave == 0 && hh == 0) sQ2[li] = q2;
+    float mean2 = 0.f;
+    for (int c0 = wave * 32; c0 < nscore; c0 += 128) {
+      const int c = c0 + li, page = c < nscore ? table[c] : -1;
+      const bool there = page >= 0 && page < a.cache.num_pages;
+      const uint16_t *mean = means + (int64_t)(there ? page : 0) * mean_stride;
+      Pack8 k[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[ks] = there && ks * 16 + hh * 8 < D ? ld_global16(mean + ks * 16 + hh * 8) : zero_pack8();
+      f32x16 acc;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+      float k2 = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        acc = mfma32<T>(q[ks], k[ks], acc);
+        float f[8];
+        unpack8<T>(k[ks], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k2 = fmaf(f[j], f[j], k2);
+      }
+      mean2 = fmaxf(mean2, sum_xor32_f(k2));
+      if (c < nscore) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) scores[(int64_t)acc_row(i, hh) * cols + c] = there ? acc[i] : -INFINITY;
+      }
+    }
+    mean2 = wave_max(mean2);
+    if (lane == 0) sMean2[wave] = mean2;
+  }
+  __syncthreads();
+
+  // ---- the best of every row ----
+  const float mean_norm = a.topk > 1 && nscore > 0 ? sqrtf(fmaxf(fmaxf(sMean2[0], sMean2[1]), fmaxf(sMean2[2], sMean2[3]))) : 0.f;
+  for (int r = wave; r < rows; r += 4) {
+    const int pos = shift + row0 + r;
+    int32_t *sel = p.sel + ((int64_t)(q0 + row0 + r) * a.heads + h) * p.topk4;
+    const int own = pos >= 0 ? pos / P : -1, n = own < 0 ? 0 : min(own, cols - 1), want = min(a.topk - 1, n);
+    float *sc = scores + (int64_t)r * cols;
+    auto take = [&](int c, uint32_t, int at) {
+      sel[at] = c;
+      atomicOr(&sBits[c], 1u << r);
+    };
+    auto key = [&](int c) { return sc[c] > -INFINITY ? float_order_key(sc[c] + 0.f) : 0u; };
+    auto self = [](int c) { return c; };
+    int picked = 0;
+    if (want > 0) {
+      // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-22 of
+      // |q| |mean|: scores further apart than twice that are in the order of 64 bits.
+      const float err = (float)D * 2.384185791015625e-7f * sqrtf(sQ2[r]) * mean_norm;
+      // the smallest score of the `want` best, and the largest of the others
+      uint32_t cut = 1u;
+      int m = 0;
+      uint32_t reg[4];
+      const bool small = n <= 256;
+      if (small) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reg[j] = j * 64 + lane < n ? key(j * 64 + lane) : 0u;
+      }
+      auto each = [&](auto &&f) {
+        if (small) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f(j * 64 + lane, reg[j]);
+        } else {
+          for (int c = lane; c - lane < n; c += 64) f(c, c < n ? key(c) : 0u);
+        }
+      };
+      auto count_ge = [&](uint32_t v) {
+        int x = 0;
+        each([&](int, uint32_t k) { x += __popcll(__ballot(k >= v)); });
+        return x;
+      };
+      m = count_ge(1u);
+      const int candidates = m;
+      if (m > want) {
+        cut = 0u;
+        for (int bit = 31; bit >= 0; --bit) {
+          const uint32_t trial = cut | (1u << bit);
+          const int x = count_ge(trial);
+          if (x >= want) cut = trial, m = x;
+          if (x == want) break;
+        }
+      }
+      float in = INFINITY, out = -INFINITY;
+      each([&](int, uint32_t k) {
+        if (k >= cut)
+          in = fminf(in, order_key_float(k));
+        else if (k > 0u)
+          out = fmaxf(out, order_key_float(k));
+      });
+      in = -wave_max(-in), out = wave_max(out);
+      if (m > want) out = in;  // equal ones on both sides
+      if (err == 0.f && m > want) {  // products of zeros: equal they are, and the later pages come first
+        picked = pick_best<0>(n, want, lane, key, [](int) { return 0u; }, self, take);
+      } else if (err < 1e30f && (candidates <= want || in - out > 2.f * err)) {
+        each([&](int c, uint32_t k) {
+          const unsigned long long mask = __ballot(k >= cut);
+          if (k >= cut) take(c, k, picked + __popcll(mask & ((1ull << lane) - 1ull)));
+          picked += __popcll(mask);
+        });
+      } else {
+        // those above `hi` belong to the best whatever the errors are, those below `lo` do not; the others decide in 64 bits (all of them if the sizes overflow)
+        const float hi = err < 1e30f ? out + 2.f * err : INFINITY, lo = err < 1e30f ? in - 2.f * err : -INFINITY;
+        const bool all = !(err < 1e30f);
+        const uint16_t *qr = qh + (int64_t)r * a.q_row_stride;
+        for (int c0 = 0; c0 < n; c0 += 64) {
+          const int c = c0 + lane;
+          const float s = c < n ? sc[c] : -INFINITY;
+          const bool above = !all && s > hi;
+          const unsigned long long am = __ballot(above);
+          if (above) take(c, 0u, picked + __popcll(am & ((1ull << lane) - 1ull)));
+          picked += __popcll(am);
+          const int page = c < n ? table[c] : -1;
+          const bool near = page >= 0 && page < a.cache.num_pages && (all || (s >= lo && s <= hi));
+          uint32_t mine = 0u;
+          for (unsigned long long todo = __ballot(near); todo;) {  // four at a time
+            int l = -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int first = todo ? (int)__ffsll(todo) - 1 : l;
+              if (lane >> 4 >= u) l = first;
+              todo &= todo - 1ull;
+            }
+            const uint64_t k = score_key(row16_dot<T>(qr, means + (int64_t)__shfl(page, l, 64) * mean_stride, D, lane));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int to = __builtin_amdgcn_readlane(l, u * 16);
+              const uint32_t hi32 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), u * 16);
+              if (lane == to) mine = hi32;
+            }
+          }
+          if (c < n) sc[c] = __uint_as_float(mine);  // its own lane reads it below
+        }
+        const int at0 = picked;
+        picked += pick_best<0>(
+            n, want - picked, lane, [&](int c) { return __float_as_uint(sc[c]); },
+            [&](int c) { return (uint32_t)score_key(lane_dot<T>(qr, means + (int64_t)table[c] * mean_stride, D)); }, self, [&](int c, uint32_t k, int at) { take(c, k, at0 + at); });
+      }
+    }
+    const int own_page = own >= 0 && own < cols ? table[own] : -1;
+    const bool has_own = own_page >= 0 && own_page < a.cache.num_pages;
+    if (has_own && lane == 0) {
+      sel[picked] = own;
+      atomicOr(&sBits[own], 1u << r);
+    }
+    picked += has_own ? 1 : 0;
+    for (int i = picked + lane; i < p.topk4; i += 64) sel[i] = -1;
+  }
+  __syncthreads();
+  uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
+  for (int i = tid; i < npages; i += 256) bits[i] = sBits[i];
+}
+
+// ------------------------------------------------------------------------------------
+// columns
+// ------------------------------------------------------------------------------------
+constexpr int kColumnRows = 128;            // of a turn: 32 a wave
+constexpr int kColumnWords = 64;            // words of bits that are spread out at a time
+constexpr int kColumnList = kColumnRows + kColumnWords * 32;
+// 16-bit rows in LDS: K rows 16 bytes apart beyond their length, so that 16 rows' pieces meet all banks once; V rows 64, so that the four rows of a
+// transposing read do
+template <int HD>
+struct ColumnLds {
+  static constexpr int kStrideK = HD + 8, kStrideV = HD + 32;
+  static constexpr int kRowBytes = (kStrideK + kStrideV) * 2;
+};
+
+template <typename T, typename H, int HD, int KT>  // KT: keys of a softmax step
+__global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
+  constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, SK = ColumnLds<HD>::kStrideK, SV = ColumnLds<HD>::kStrideV;
+  extern __shared__ __align__(16) uint8_t column_smem[];
+  __shared__ int sList[kColumnList];
+  __shared__ int sCount, sNan;
+  uint16_t *sK = reinterpret_cast<uint16_t *>(column_smem), *sV = sK + held * SK;
+  const fmoba_cache_attn_args &a = p.c.a;
+  const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, cols = p.c.cols;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
+  const PairItem item = xcd_pair_item(blockIdx.x, a.batch * a.cache.heads_k, cols * p.parts);
+  const int b = item.pair / a.cache.heads_k, hk = item.pair - b * a.cache.heads_k, c = item.idx / p.parts, part = item.idx - c * p.parts;
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
+  const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q);
+  if (q0 < 0 || R <= 0 || (int64_t)c * P >= len) return;
+  const int page = a.block_table[(int64_t)b * a.table_stride + c];
+  if (page < 0 || page >= a.cache.num_pages) return;
+  const int shift = len - (q1 - q0), tiles = (R + kTileRows - 1) / kTileRows * G;
+  const int w0 = part * p.words, w1 = min(w0 + p.words, tiles);
+  const int keys = min(P, len - c * P);  // of the page that are there
+  const uint32_t *bits = p.bits + ((int64_t)hk * p.blocks + block_of(q0, b)) * G * cols + c;
+  const float k_scale = a.cache.k_scale[(int64_t)page * a.cache.heads_k + hk] * a.softmax_scale * 1.4426950408889634f;
+  const float v_scale = a.cache.v_scale[(int64_t)page * a.cache.heads_k + hk];
+  const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + (int64_t)page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride;
+  const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + (int64_t)page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride;
+  if (tid == 0) sNan = 0;
+
+  // keys [k0, k0 + held) of the page, widened; features past D and keys that are not there are zeros, and so are NaNs among the values (they count below)
+  auto stage = [&](int k0) {
+    const int pieces = HD / 16;
+    for (int i = tid; i < held * pieces; i += 256) {
+      const int r = i / pieces, e = (i - r * pieces) * 16;
+      const bool there = k0 + r < keys && e < D;
+      const Pack8 kx = there ? ld_global16(kg + (int64_t)(k0 + r) * a.cache.k_token_stride + e) : zero_pack8();
+      const Pack8 vx = there ? ld_global16(vg + (int64_t)(k0 + r) * a.cache.v_token_stride + e) : zero_pack8();
+      Pack8 ko[2], vo[2];
+      bool nan = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float f[4], g[4];
+        H::unpack4(kx.w[w], f);
+        H::unpack4(vx.w[w], g);
+        ko[w >> 1].w[(w & 1) * 2] = pack2<T>(f[0], f[1]), ko[w >> 1].w[(w & 1) * 2 + 1] = pack2<T>(f[2], f[3]);
+        if constexpr (H::kFormat == FMOBA_CACHE_E4M3) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            nan = nan || g[j] != g[j];
+            g[j] = g[j] != g[j] ? 0.f : g[j];
+          }
+        }
+        vo[w >> 1].w[(w & 1) * 2] = pack2<f16_t>(g[0], g[1]), vo[w >> 1].w[(w & 1) * 2 + 1] = pack2<f16_t>(g[2], g[3]);
+      }
+      *reinterpret_cast<Pack8 *>(sK + r * SK + e) = ko[0];
+      *reinterpret_cast<Pack8 *>(sK + r * SK + e + 8) = ko[1];
+      *reinterpret_cast<Pack8 *>(sV + r * SV + e) = vo[0];
+      *reinterpret_cast<Pack8 *>(sV + r * SV + e + 8) = vo[1];
+      if (nan) sNan = 1;
+    }
+  };
+
+  // one turn: up to 128 entries of the list from `from` on
+  auto turn = [&](int from, int count) {
+    const int idx = wave * 32 + li;
+    const bool there = idx < count;
+    const int entry = sList[from + min(idx, count - 1)];
+    const int w = entry >> 5, rb = w / G, g = w - rb * G, row = rb * kTileRows + (entry & 31);
+    const int lim = shift + row - c * P;  // last key of the page that the row sees
+    const int64_t rowhead = (int64_t)(q0 + row) * a.heads + hk * G + g;
+    const uint16_t *qr = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
+    Pack8 q[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = ks * 16 + hh * 8 < D ? ld_global16(qr + ks * 16 + hh * 8) : zero_pack8();
+    int slot = 0;
+    {
+      const int4 *sel = reinterpret_cast<const int4 *>(p.sel + rowhead * p.topk4);
+      for (int i = 0; i < p.topk4; i += 4) {
+        const int4 s = sel[i >> 2];
+        slot = s.x == c ? i : s.y == c ? i + 1 : s.z == c ? i + 2 : s.w == c ? i + 3 : slot;
+      }
+    }
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const int last = min(keys - 1, P - 1);
+    for (int k0 = 0; k0 <= last; k0 += held) {
+      if (held < P) {
+        __syncthreads();
+        stage(k0);
+        __syncthreads();
+      }
+      for (int s0 = 0; s0 < held && k0 + s0 <= last; s0 += KT) {
+        const bool seen = __ballot(there && lim >= k0 + s0) != 0ull;
+        if (!seen) continue;
+        f32x16 s[ST];
+#pragma unroll
+        for (int t = 0; t < ST; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+          const uint16_t *kr = sK + (s0 + t * 32 + li) * SK + hh * 8;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[t] = mfma32<T>(*reinterpret_cast<const Pack8 *>(kr + ks * 16), q[ks], s[t]);
+        }
+        const int left = lim - k0 - s0;  // last visible key of this step
+        float mx = -INFINITY;
+        if (__ballot(left < KT - 1) != 0ull) {
+#pragma unroll
+          for (int t = 0; t < ST; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[t][i] = t * 32 + acc_row(i, hh) <= left ? s[t][i] * k_scale : -INFINITY;
+              mx = fmaxf(mx, s[t][i]);
+            }
+        } else {
+#pragma unroll
+          for (int t = 0; t < ST; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[t][i] *= k_scale;
+              mx = fmaxf(mx, s[t][i]);
+            }
+        }
+        mx = max_xor32_f(mx);
+        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+        if (k0 + s0 > 0) {
+          const float resc = __builtin_amdgcn_exp2f(m - ref);
+          l *= resc;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= resc;
+        }
+        m = mn;
+        float sum = 0.f;
+        Pack8 pk[ST][2];
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float x = __builtin_amdgcn_exp2f(s[t][i] - ref), y = __builtin_amdgcn_exp2f(s[t][i + 1] - ref);
+            sum += x + y;
+            pk[t][i >> 3].w[(i & 7) >> 1] = pack2<f16_t>(x, y);
+          }
+        l += sum_xor32_f(sum);
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+              o[d] = mfma32<f16_t>(tr_frag8(sV, SV, s0 + t * 32 + 16 * u + 4 * hh, s0 + t * 32 + 16 * u + 8 + 4 * hh, d * 32, lane), pk[t][u], o[d]);
+      }
+    }
+    // NaNs among the values of the page: a row that sees one has it in that feature
+    if (H::kFormat == FMOBA_CACHE_E4M3 && sNan != 0) {
+      for (int k = 0; k <= last; ++k)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = d * 32 + acc_row(i, hh);
+            if (e < D && k <= lim && (vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) o[d][i] = NAN;
+          }
+    }
+    if (there) {
+      const int64_t at = rowhead * p.topk4 + slot;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
+      uint16_t *dst = p.part + at * D;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = d * 32 + 8 * j + 4 * hh;
+          if (e < D) st_stream8(dst + e, pack2<f16_t>(o[d][4 * j] * inv, o[d][4 * j + 1] * inv), pack2<f16_t>(o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv));
+        }
+    }
+  };
+
+  bool staged = false;
+  int have = 0;  // entries of the list that wait
+  for (int wb = w0; wb < w1; wb += kColumnWords) {
+    if (wave == 0) {
+      const int w = wb + lane;
+      uint32_t x = w < w1 ? bits[(int64_t)w * cols] : 0u;
+      const int n = __popc(x);
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(upto, o, 64);
+        upto += lane >= o ? up : 0;
+      }
+      int at = have + upto - n;
+      while (x) {
+        sList[at++] = w << 5 | (__ffs(x) - 1);
+        x &= x - 1u;
+      }
+      if (lane == 63) sCount = have + upto;
+    }
+    __syncthreads();
+    const int count = sCount;
+    const bool end = wb + kColumnWords >= w1;
+    if (count > 0 && (end || count >= kColumnRows) && held >= P && !staged) {
+      stage(0);
+      staged = true;
+      __syncthreads();
+    }
+    int from = 0;
+    while (count - from >= kColumnRows || (end && from < count)) {
+      turn(from, min(kColumnRows, count - from));
+      from += kColumnRows;
+    }
+    have = max(count - from, 0);
+    __syncthreads();
+    if (from > 0 && have > 0) {
+      const int x = tid < have ? sList[from + tid] : 0;
+      __syncthreads();
+      if (tid < have) sList[tid] = x;
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// combine: LPR lanes a (row, head), eight features each
+// ------------------------------------------------------------------------------------
+template <typename T, int LPR, bool WEIGHT>
+__global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
+  const fmoba_cache_attn_args &a = p.c.a;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, D = a.cache.head_dim;
+  const int64_t rowhead = (int64_t)blockIdx.x * (256 / LPR) + tid / LPR;
+  if (rowhead >= (int64_t)a.total_q * a.heads) return;
+  const int t = (int)(rowhead / a.heads), h = (int)(rowhead - (int64_t)t * a.heads);
+  const int32_t *sel = p.sel + rowhead * p.topk4;
+  const float2 *head = p.head + rowhead * p.topk4;
+  const uint16_t *part = p.part + rowhead * p.topk4 * D;
+  const RowPlace at = find_row_lane(a, t);
+  int n = 0;
+  float m = -INFINITY;
+  if (at.pos >= 0)
+    for (; n < p.topk4; ++n) {
+      if (sel[n] < 0) break;
+      const float x = head[n].x;
+      m = x > m ? x : m;
+    }
+  const float ref = m == -INFINITY ? 0.f : m;
+  const int e = li * 8;
+  float l = 0.f, acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float2 x = head[i];
+    const float w = __builtin_amdgcn_exp2f(x.x - ref), wv = w * x.y;
+    l += w;
+    if (e < D) {
+      float f[8];
+      unpack8<f16_t>(ld_stream16(part + (int64_t)i * D + e), f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = w == 0.f ? acc[j] : fmaf(wv, f[j], acc[j]);
+    }
+  }
+  const bool empty = l == 0.f;
+  const float inv = empty ? 0.f : 1.f / l;
+  if (e < D) {
+    Pack8 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.w[j] = pack2<T>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    *reinterpret_cast<Pack8 *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t)t * a.o_row_stride + (int64_t)h * a.o_head_stride + e) = o;
+  }
+  if (li == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  if constexpr (WEIGHT) {
+    const int hk = h / (a.heads / a.cache.heads_k);
+    const int32_t *table = a.block_table + (int64_t)(at.b < a.batch ? at.b : 0) * a.table_stride;
+    for (int i = li; i < n; i += LPR) {
+      const float part_of = __builtin_amdgcn_exp2f(head[i].x - ref) * inv;
+      const int page = table[sel[i]];
+      if (part_of > 0.f && page >= 0 && page < a.cache.num_pages)
+        atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)page * a.cache.heads_k + hk, (unsigned long long)rintf(part_of * 4294967296.f));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------
+static size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
+struct ColumnSizes {
+  size_t sel, bits, scores, head, part, total;
+};
+static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, ColumnPlan &p) {
+  const size_t rowheads = (size_t)a.total_q * a.heads;
+  p.topk4 = (a.topk + 3) / 4 * 4;
+  p.blocks = a.total_q / kTileRows + a.batch;
+  p.tiles = ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows) * (a.heads / a.cache.heads_k);
+  ColumnSizes z;
+  z.sel = up(rowheads * p.topk4 * 4);
+  z.bits = up((size_t)a.heads * p.blocks * cols * 4);
+  z.scores = cols > kGateCols ? up((size_t)a.heads * p.blocks * kTileRows * cols * 4) : 0;
+  z.head = up(rowheads * p.topk4 * 8);
+  z.part = up(rowheads * p.topk4 * a.cache.head_dim * 2);
+  z.total = z.sel + z.bits + z.scores + z.head + z.part;
+  return z;
+}
+size_t column_workspace_bytes(const fmoba_cache_attn_args &a, int cols) {
+  ColumnPlan p{};
+  return column_sizes(a, cols, p).total;
+}
+
+template <typename K>
+static int with_lds(K kern, size_t bytes, const char *what) {
+  if (bytes > 48 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) {
+    set_error("%s: cannot reserve %zu bytes of LDS", what, bytes);
+    return 2;
+  }
+  return 0;
+}
+
+template <typename T, int HD>
+static int launch_gate(const ColumnPlan &p, hipStream_t s) {
+  const fmoba_cache_attn_args &a = p.c.a;
+  const dim3 grid(ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows), a.heads, a.batch);
+  const bool lds = p.c.cols <= kGateCols;
+  const size_t bytes = (size_t)p.c.cols * 4 * (lds ? 1 + kTileRows : 1);
+  auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
+  if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
+  hipLaunchKernelGGL(kern, grid, dim3(256), bytes, s, p);
+  FMOBA_LAUNCH_CHECK("cache_gate_kernel");
+  return 0;
+}
+template <typename T, typename H, int HD, int KT>
+static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
+  auto kern = cache_columns_kernel<T, H, HD, KT>;
+  const size_t bytes = (size_t)held * ColumnLds<HD>::kRowBytes;
+  if (int rc = with_lds(kern, bytes, "cache_columns")) return rc;
+  const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.parts;
+  FMOBA_REQUIRE(grid <= INT32_MAX, "cache_attn: too many pages for the launch grid");
+  hipLaunchKernelGGL(kern, dim3((uint32_t)grid), dim3(256), bytes, s, p, held);
+  FMOBA_LAUNCH_CHECK("cache_columns_kernel");
+  return 0;
+}
+template <typename T, typename H, int HD>
+static int launch_columns(const ColumnPlan &p, hipStream_t s) {
+  const int P = p.c.a.cache.page_size;
+  // the whole page where two workgroups find room on a compute unit, else 64 keys at a time
+  const int held = P * ColumnLds<HD>::kRowBytes <= 76 * 1024 ? P : 64;
+  if constexpr (HD <= 128) {
+    if (held % 128 == 0) return launch_columns_as<T, H, HD, 128>(p, held, s);
+  }
+  return launch_columns_as<T, H, HD, 64>(p, held, s);
+}
+template <typename T, int LPR>
+static void launch_combine(const ColumnPlan &p, hipStream_t s) {
+  const int64_t rowheads = (int64_t)p.c.a.total_q * p.c.a.heads;
+  const dim3 grid((uint32_t)ceil_div64(rowheads, 256 / LPR));
+  if (p.c.a.add_weight)
+    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, true>), grid, dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, false>), grid, dim3(256), 0, s, p);
+}
+template <typename T, int HD>
+static int run_columns_hd(const ColumnPlan &p, hipStream_t s) {
+  if (int rc = launch_gate<T, HD>(p, s)) return rc;
+  if (int rc = p.c.a.cache.format == FMOBA_CACHE_E4M3 ? launch_columns<T, HeldE4M3, HD>(p, s) : launch_columns<T, HeldInt8, HD>(p, s)) return rc;
+  launch_combine<T, HD / 8>(p, s);
+  FMOBA_LAUNCH_CHECK("cache_combine_kernel");
+  return 0;
+}
+template <typename T>
+static int run_columns_as(const ColumnPlan &p, hipStream_t s) {
+  const int D = p.c.a.cache.head_dim;
+  return D <= 64 ? run_columns_hd<T, 64>(p, s) : D <= 128 ? run_columns_hd<T, 128>(p, s) : run_columns_hd<T, 256>(p, s);
+}
+
+int run_cache_columns(const CacheAttn &c, hipStream_t s) {
+  const fmoba_cache_attn_args &a = c.a;
+  FMOBA_REQUIRE(a.heads <= 65535 && a.batch <= 65535, "cache_attn: batch/heads too large for the launch grid");
+  ColumnPlan p{};
+  p.c = c;
+  const ColumnSizes z = column_sizes(a, c.cols, p);
+  uint8_t *at = reinterpret_cast<uint8_t *>(a.workspace);
+  p.sel = reinterpret_cast<int32_t *>(at), at += z.sel;
+  p.bits = reinterpret_cast<uint32_t *>(at), at += z.bits;
+  p.scores = reinterpret_cast<float *>(at), at += z.scores;
+  p.head = reinterpret_cast<float2 *>(at), at += z.head;
+  p.part = reinterpret_cast<uint16_t *>(at);
+  // words that bring a workgroup three turns of rows if rows choose evenly
+  const int64_t words = ceil_div64((int64_t)3 * kColumnRows * c.cols, (int64_t)kTileRows * std::min(a.topk, c.cols));
+  p.words = (int)std::min<int64_t>(std::max<int64_t>((words + kColumnWords - 1) / kColumnWords * kColumnWords, kColumnWords), std::max(p.tiles, 1));
+  p.parts = ceil_div(p.tiles, p.words);
+  return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
+}
+
+}  // namespace fmoba
