@@ -25,7 +25,7 @@ struct ColumnPlan {
   int32_t topk4;     // topk, rounded up to a multiple of four
   int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
   int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
-  int32_t parts, words;  // workgroups of a page, and the words that each of them looks at
+  int32_t parts;     // workgroups of a page
 };
 
 // The first block of a sequence: those of a sequence of n rows from q0 on are ceil(n / 32) <= floor((q0 + n) / 32) - floor(q0 / 32) + 1.
@@ -257,24 +257,16 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p) {
 // ------------------------------------------------------------------------------------
 // columns
 // ------------------------------------------------------------------------------------
-constexpr int kColumnRows = 128;            // of a turn: 32 a wave
-constexpr int kColumnWords = 64;            // words of bits that are spread out at a time
+constexpr int kColumnRows = 128;  // of a turn: 32 a wave
+constexpr int kColumnWords = 32;  // words of bits that are spread out at a time
 constexpr int kColumnList = kColumnRows + kColumnWords * 32;
-// 16-bit rows in LDS: K rows 16 bytes apart beyond their length, so that 16 rows' pieces meet all banks once; V rows 64, so that the four rows of a
-// transposing read do
-template <int HD>
-struct ColumnLds {
-  static constexpr int kStrideK = HD + 8, kStrideV = HD + 32;
-  static constexpr int kRowBytes = (kStrideK + kStrideV) * 2;
-};
 
 template <typename T, typename H, int HD, int KT>  // KT: keys of a softmax step
-__global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
-  constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, SK = ColumnLds<HD>::kStrideK, SV = ColumnLds<HD>::kStrideV;
-  extern __shared__ __align__(16) uint8_t column_smem[];
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
+  constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, ROW = HD * 2;  // (LDS rows of exactly HD elements, their pieces swizzled: tile_swz)
+  extern __shared__ __align__(1024) uint8_t column_smem[];
   __shared__ int sList[kColumnList];
   __shared__ int sCount, sNan;
-  uint16_t *sK = reinterpret_cast<uint16_t *>(column_smem), *sV = sK + held * SK;
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, cols = p.c.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
@@ -285,48 +277,76 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
   if (q0 < 0 || R <= 0 || (int64_t)c * P >= len) return;
   const int page = a.block_table[(int64_t)b * a.table_stride + c];
   if (page < 0 || page >= a.cache.num_pages) return;
-  const int shift = len - (q1 - q0), tiles = (R + kTileRows - 1) / kTileRows * G;
-  const int w0 = part * p.words, w1 = min(w0 + p.words, tiles);
+  const int shift = len - (q1 - q0), G_tiles = (R + kTileRows - 1) / kTileRows * G;
+  // the words of rows that can see the page, shared out evenly
+  const int first = max(c * P - shift, 0) / kTileRows * G;
+  const int each = ((G_tiles - first + p.parts - 1) / p.parts + kColumnWords - 1) / kColumnWords * kColumnWords;
+  const int w0 = first + part * each, w1 = min(w0 + each, G_tiles);
+  if (w0 >= w1) return;
   const int keys = min(P, len - c * P);  // of the page that are there
   const uint32_t *bits = p.bits + ((int64_t)hk * p.blocks + block_of(q0, b)) * G * cols + c;
-  const float k_scale = a.cache.k_scale[(int64_t)page * a.cache.heads_k + hk] * a.softmax_scale * 1.4426950408889634f;
-  const float v_scale = a.cache.v_scale[(int64_t)page * a.cache.heads_k + hk];
   const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + (int64_t)page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride;
   const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + (int64_t)page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride;
+  uint32_t word = wave == 0 && lane < kColumnWords && w0 + lane < w1 ? bits[(int64_t)(w0 + lane) * cols] : 0u;  // (those of the next turn of words, always)
+  const float k_scale = a.cache.k_scale[(int64_t)page * a.cache.heads_k + hk] * a.softmax_scale * 1.4426950408889634f;
+  const float v_scale = a.cache.v_scale[(int64_t)page * a.cache.heads_k + hk];
   if (tid == 0) sNan = 0;
 
+  const uint32_t k_base = (uint32_t)(uintptr_t)to_lds(column_smem), v_base = k_base + (uint32_t)(held * ROW);
   // keys [k0, k0 + held) of the page, widened; features past D and keys that are not there are zeros, and so are NaNs among the values (they count below)
   auto stage = [&](int k0) {
-    const int pieces = HD / 16;
-    for (int i = tid; i < held * pieces; i += 256) {
-      const int r = i / pieces, e = (i - r * pieces) * 16;
-      const bool there = k0 + r < keys && e < D;
-      const Pack8 kx = there ? ld_global16(kg + (int64_t)(k0 + r) * a.cache.k_token_stride + e) : zero_pack8();
-      const Pack8 vx = there ? ld_global16(vg + (int64_t)(k0 + r) * a.cache.v_token_stride + e) : zero_pack8();
-      Pack8 ko[2], vo[2];
+    constexpr int PIECES = HD / 16, AT_ONCE = 4;
+    for (int i0 = tid; i0 < held * PIECES; i0 += 256 * AT_ONCE) {
+      Pack8 kx[AT_ONCE], vx[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * 256, r = i / PIECES, e = (i % PIECES) * 16;
+        const bool there = i < held * PIECES && k0 + r < keys && e < D;
+        kx[u] = there ? ld_global16(kg + (int64_t)(k0 + r) * a.cache.k_token_stride + e) : zero_pack8();
+        vx[u] = there ? ld_global16(vg + (int64_t)(k0 + r) * a.cache.v_token_stride + e) : zero_pack8();
+      }
       bool nan = false;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float f[4], g[4];
-        H::unpack4(kx.w[w], f);
-        H::unpack4(vx.w[w], g);
-        ko[w >> 1].w[(w & 1) * 2] = pack2<T>(f[0], f[1]), ko[w >> 1].w[(w & 1) * 2 + 1] = pack2<T>(f[2], f[3]);
-        if constexpr (H::kFormat == FMOBA_CACHE_E4M3) {
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const int i = i0 + u * 256, r = i / PIECES, piece = (i % PIECES) * 2;
+        if (i >= held * PIECES) continue;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            nan = nan || g[j] != g[j];
-            g[j] = g[j] != g[j] ? 0.f : g[j];
+        for (int half = 0; half < 2; ++half) {
+          u32x4_t ko, vo;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            float f[4], g[4];
+            H::unpack4(kx[u].w[half * 2 + w], f);
+            H::unpack4(vx[u].w[half * 2 + w], g);
+            ko[2 * w] = pack2<T>(f[0], f[1]), ko[2 * w + 1] = pack2<T>(f[2], f[3]);
+            if constexpr (H::kFormat == FMOBA_CACHE_E4M3) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                nan = nan || g[j] != g[j];
+                g[j] = g[j] != g[j] ? 0.f : g[j];
+              }
+            }
+            vo[2 * w] = pack2<f16_t>(g[0], g[1]), vo[2 * w + 1] = pack2<f16_t>(g[2], g[3]);
           }
+          const uint32_t at = (uint32_t)(r * ROW + ((piece + half) ^ tile_swz<HD>(r)) * 16);
+          lds_write_vec(k_base + at, ko);
+          lds_write_vec(v_base + at, vo);
         }
-        vo[w >> 1].w[(w & 1) * 2] = pack2<f16_t>(g[0], g[1]), vo[w >> 1].w[(w & 1) * 2 + 1] = pack2<f16_t>(g[2], g[3]);
       }
-      *reinterpret_cast<Pack8 *>(sK + r * SK + e) = ko[0];
-      *reinterpret_cast<Pack8 *>(sK + r * SK + e + 8) = ko[1];
-      *reinterpret_cast<Pack8 *>(sV + r * SV + e) = vo[0];
-      *reinterpret_cast<Pack8 *>(sV + r * SV + e + 8) = vo[1];
       if (nan) sNan = 1;
     }
   };
+  // where this lane's operands lie: of K row li, its pieces; of V four features of a row of four, and the row eight further down
+  uint32_t k_at[KS], v_lo[DT], v_hi[DT];
+  {
+    const uint32_t k0 = (uint32_t)(li * ROW + (tile_frag_piece<HD>(hh, 0) ^ tile_swz<HD>(li)) * 16);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_at[ks] = k_base + tile_frag_addr<HD>(k0, ks);
+    const int i = lane & 15, r = 4 * hh + (i >> 2);
+    const uint32_t v0 = (uint32_t)(r * ROW + (((li >> 4) * 2 + ((i & 3) >> 1)) ^ tile_swz<HD>(r)) * 16 + (i & 1) * 8);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) v_lo[d] = v_base + tile_tr_addr<HD>(v0, d), v_hi[d] = v_base + tile_tr_addr8<HD>(v0, d);
+  }
 
   // one turn: up to 128 entries of the list from `from` on
   auto turn = [&](int from, int count) {
@@ -339,13 +359,16 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
     const uint16_t *qr = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
     Pack8 q[KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) q[ks] = ks * 16 + hh * 8 < D ? ld_global16(qr + ks * 16 + hh * 8) : zero_pack8();
+    for (int ks = 0; ks < KS; ++ks) {
+      const int e = tile_frag_piece<HD>(hh, ks) * 8;
+      q[ks] = e < D ? ld_global16(qr + e) : zero_pack8();
+    }
     int slot = 0;
     {
       const int4 *sel = reinterpret_cast<const int4 *>(p.sel + rowhead * p.topk4);
-      for (int i = 0; i < p.topk4; i += 4) {
-        const int4 s = sel[i >> 2];
-        slot = s.x == c ? i : s.y == c ? i + 1 : s.z == c ? i + 2 : s.w == c ? i + 3 : slot;
+      for (int i = 0; i < p.topk4; i += 8) {
+        const int4 s = sel[i >> 2], s2 = i + 4 < p.topk4 ? sel[(i >> 2) + 1] : s;
+        slot = s.x == c ? i : s.y == c ? i + 1 : s.z == c ? i + 2 : s.w == c ? i + 3 : s2.x == c ? i + 4 : s2.y == c ? i + 5 : s2.z == c ? i + 6 : s2.w == c ? i + 7 : slot;
       }
     }
     f32x16 o[DT];
@@ -354,24 +377,22 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const int last = min(keys - 1, P - 1);
-    for (int k0 = 0; k0 <= last; k0 += held) {
+    for (int k0 = 0; k0 < keys; k0 += held) {
       if (held < P) {
         __syncthreads();
         stage(k0);
         __syncthreads();
       }
-      for (int s0 = 0; s0 < held && k0 + s0 <= last; s0 += KT) {
-        const bool seen = __ballot(there && lim >= k0 + s0) != 0ull;
-        if (!seen) continue;
+      for (int s0 = 0; s0 < held && k0 + s0 < keys; s0 += KT) {
+        if (__ballot(there && lim >= k0 + s0) == 0ull) continue;
+        const uint32_t off = (uint32_t)(s0 * ROW);
         f32x16 s[ST];
 #pragma unroll
         for (int t = 0; t < ST; ++t) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-          const uint16_t *kr = sK + (s0 + t * 32 + li) * SK + hh * 8;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s[t] = mfma32<T>(*reinterpret_cast<const Pack8 *>(kr + ks * 16), q[ks], s[t]);
+          for (int ks = 0; ks < KS; ++ks) s[t] = mfma32<T>(lds_read16(k_at[ks] + off + (uint32_t)(t * 32 * ROW)), q[ks], s[t]);
         }
         const int left = lim - k0 - s0;  // last visible key of this step
         float mx = -INFINITY;
@@ -404,57 +425,58 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
         }
         m = mn;
         float sum = 0.f;
-        Pack8 pk[ST][2];
 #pragma unroll
         for (int t = 0; t < ST; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float x = __builtin_amdgcn_exp2f(s[t][i] - ref), y = __builtin_amdgcn_exp2f(s[t][i + 1] - ref);
-            sum += x + y;
-            pk[t][i >> 3].w[(i & 7) >> 1] = pack2<f16_t>(x, y);
+          for (int u = 0; u < 2; ++u) {
+            Pack8 pk;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const float x = __builtin_amdgcn_exp2f(s[t][8 * u + i] - ref), y = __builtin_amdgcn_exp2f(s[t][8 * u + i + 1] - ref);
+              sum += x + y;
+              pk.w[i >> 1] = pack2<f16_t>(x, y);
+            }
+            const uint32_t rows = off + (uint32_t)((t * 32 + 16 * u) * ROW);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = mfma32<f16_t>(lds_tr8(v_lo[d] + rows, v_hi[d] + rows), pk, o[d]);
           }
         l += sum_xor32_f(sum);
-#pragma unroll
-        for (int t = 0; t < ST; ++t)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-              o[d] = mfma32<f16_t>(tr_frag8(sV, SV, s0 + t * 32 + 16 * u + 4 * hh, s0 + t * 32 + 16 * u + 8 + 4 * hh, d * 32, lane), pk[t][u], o[d]);
       }
     }
-    // NaNs among the values of the page: a row that sees one has it in that feature
-    if (H::kFormat == FMOBA_CACHE_E4M3 && sNan != 0) {
-      for (int k = 0; k <= last; ++k)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int e = d * 32 + acc_row(i, hh);
-            if (e < D && k <= lim && (vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) o[d][i] = NAN;
-          }
-    }
+    const int64_t at = rowhead * p.topk4 + slot;
+    uint16_t *dst = p.part + at * D;
     if (there) {
-      const int64_t at = rowhead * p.topk4 + slot;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
-      uint16_t *dst = p.part + at * D;
+      // features 8 j + 4 hh .. of both halves to eight of one lane: 16 bytes each
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = d * 32 + 8 * j + 4 * hh;
-          if (e < D) st_stream8(dst + e, pack2<f16_t>(o[d][4 * j] * inv, o[d][4 * j + 1] * inv), pack2<f16_t>(o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv));
+        for (int j = 0; j < 4; j += 2) {
+          uint32_t x0 = pack2<f16_t>(o[d][4 * j] * inv, o[d][4 * j + 1] * inv), x1 = pack2<f16_t>(o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv);
+          uint32_t y0 = pack2<f16_t>(o[d][4 * j + 4] * inv, o[d][4 * j + 5] * inv), y1 = pack2<f16_t>(o[d][4 * j + 6] * inv, o[d][4 * j + 7] * inv);
+#if defined(__HIP_DEVICE_COMPILE__)
+          const auto r0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), r1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+          x0 = r0[0], y0 = r0[1], x1 = r1[0], y1 = r1[1];
+#endif
+          const int e = d * 32 + 8 * j + 8 * hh;
+          if (e < D) *reinterpret_cast<Pack8 *>(dst + e) = Pack8{{x0, x1, y0, y1}};
         }
+      // NaNs among the values of the page: a row that sees one has it in that feature
+      if (H::kFormat == FMOBA_CACHE_E4M3 && sNan != 0) {
+        const int last = min(lim, keys - 1);
+        for (int e = hh * 8; e < D; e += (e & 7) == 7 ? 9 : 1)  // (the features that this lane has written)
+          for (int k = 0; k <= last; ++k)
+            if ((vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) dst[e] = 0x7e00;
+      }
     }
   };
 
-  bool staged = false;
+  if (held >= P) stage(0);
   int have = 0;  // entries of the list that wait
   for (int wb = w0; wb < w1; wb += kColumnWords) {
     if (wave == 0) {
-      const int w = wb + lane;
-      uint32_t x = w < w1 ? bits[(int64_t)w * cols] : 0u;
+      uint32_t x = word;
       const int n = __popc(x);
       int upto = n;
 #pragma unroll
@@ -464,19 +486,16 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
       }
       int at = have + upto - n;
       while (x) {
-        sList[at++] = w << 5 | (__ffs(x) - 1);
+        sList[at++] = (wb + lane) << 5 | (__ffs(x) - 1);
         x &= x - 1u;
       }
       if (lane == 63) sCount = have + upto;
+      const int next = wb + kColumnWords + lane;
+      word = lane < kColumnWords && next < w1 ? bits[(int64_t)next * cols] : 0u;
     }
     __syncthreads();
     const int count = sCount;
     const bool end = wb + kColumnWords >= w1;
-    if (count > 0 && (end || count >= kColumnRows) && held >= P && !staged) {
-      stage(0);
-      staged = true;
-      __syncthreads();
-    }
     int from = 0;
     while (count - from >= kColumnRows || (end && from < count)) {
       turn(from, min(kColumnRows, count - from));
@@ -498,8 +517,9 @@ __global__ __launch_bounds__(256, 2) void cache_columns_kernel(ColumnPlan p, int
 // ------------------------------------------------------------------------------------
 template <typename T, int LPR, bool WEIGHT>
 __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
+  constexpr int NS = 64 / LPR, AT_ONCE = 8;  // slots of a lane; rows asked for together
   const fmoba_cache_attn_args &a = p.c.a;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, D = a.cache.head_dim;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim;
   const int64_t rowhead = (int64_t)blockIdx.x * (256 / LPR) + tid / LPR;
   if (rowhead >= (int64_t)a.total_q * a.heads) return;
   const int t = (int)(rowhead / a.heads), h = (int)(rowhead - (int64_t)t * a.heads);
@@ -507,28 +527,58 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
   const float2 *head = p.head + rowhead * p.topk4;
   const uint16_t *part = p.part + rowhead * p.topk4 * D;
   const RowPlace at = find_row_lane(a, t);
-  int n = 0;
-  float m = -INFINITY;
-  if (at.pos >= 0)
-    for (; n < p.topk4; ++n) {
-      if (sel[n] < 0) break;
-      const float x = head[n].x;
-      m = x > m ? x : m;
-    }
+  // the row's visits, one or more a lane: their pages fill the slots from the first on
+  int page_of[NS];
+  float w[NS], vs[NS], m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const int s = j * LPR + li;
+    page_of[j] = s < p.topk4 && at.pos >= 0 ? sel[s] : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const float2 x = page_of[j] >= 0 ? head[j * LPR + li] : make_float2(-INFINITY, 0.f);
+    w[j] = x.x, vs[j] = x.y;
+    m = x.x > m ? x.x : m;
+  }
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    w[j] = __builtin_amdgcn_exp2f(w[j] - ref);
+    l += w[j];
+    vs[j] *= w[j];
+    n += page_of[j] >= 0 ? 1 : 0;
+  }
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64), n += __shfl_xor(n, o, 64);
   const int e = li * 8;
-  float l = 0.f, acc[8];
+  float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const float2 x = head[i];
-    const float w = __builtin_amdgcn_exp2f(x.x - ref), wv = w * x.y;
-    l += w;
-    if (e < D) {
-      float f[8];
-      unpack8<f16_t>(ld_stream16(part + (int64_t)i * D + e), f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = w == 0.f ? acc[j] : fmaf(wv, f[j], acc[j]);
+  for (int j = 0; j < NS; ++j) {
+    if (j * LPR >= p.topk4) break;
+    for (int i0 = 0; i0 < LPR && j * LPR + i0 < p.topk4; i0 += AT_ONCE) {
+      Pack8 x[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int s = j * LPR + i0 + i;
+        x[i] = s < n && e < D ? ld_stream16(part + (int64_t)s * D + e) : zero_pack8();
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float wv = __shfl(vs[j], group + i0 + i, 64);
+        float f[8];
+        unpack8<f16_t>(x[i], f);
+        if (j * LPR + i0 + i < n && wv != 0.f) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = fmaf(wv, f[k], acc[k]);
+        }
+      }
     }
   }
   const bool empty = l == 0.f;
@@ -543,9 +593,10 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
   if constexpr (WEIGHT) {
     const int hk = h / (a.heads / a.cache.heads_k);
     const int32_t *table = a.block_table + (int64_t)(at.b < a.batch ? at.b : 0) * a.table_stride;
-    for (int i = li; i < n; i += LPR) {
-      const float part_of = __builtin_amdgcn_exp2f(head[i].x - ref) * inv;
-      const int page = table[sel[i]];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      const float part_of = w[j] * inv;
+      const int page = page_of[j] >= 0 ? table[page_of[j]] : -1;
       if (part_of > 0.f && page >= 0 && page < a.cache.num_pages)
         atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)page * a.cache.heads_k + hk, (unsigned long long)rintf(part_of * 4294967296.f));
     }
@@ -602,7 +653,7 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
 template <typename T, typename H, int HD, int KT>
 static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
   auto kern = cache_columns_kernel<T, H, HD, KT>;
-  const size_t bytes = (size_t)held * ColumnLds<HD>::kRowBytes;
+  const size_t bytes = (size_t)held * HD * 4;
   if (int rc = with_lds(kern, bytes, "cache_columns")) return rc;
   const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.parts;
   FMOBA_REQUIRE(grid <= INT32_MAX, "cache_attn: too many pages for the launch grid");
@@ -614,8 +665,8 @@ template <typename T, typename H, int HD>
 static int launch_columns(const ColumnPlan &p, hipStream_t s) {
   const int P = p.c.a.cache.page_size;
   // the whole page where two workgroups find room on a compute unit, else 64 keys at a time
-  const int held = P * ColumnLds<HD>::kRowBytes <= 76 * 1024 ? P : 64;
-  if constexpr (HD <= 128) {
+  const int held = P * HD * 4 <= 64 * 1024 ? P : 64;
+  if constexpr (HD <= 64) {
     if (held % 128 == 0) return launch_columns_as<T, H, HD, 128>(p, held, s);
   }
   return launch_columns_as<T, H, HD, 64>(p, held, s);
@@ -655,10 +706,9 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   p.scores = reinterpret_cast<float *>(at), at += z.scores;
   p.head = reinterpret_cast<float2 *>(at), at += z.head;
   p.part = reinterpret_cast<uint16_t *>(at);
-  // words that bring a workgroup three turns of rows if rows choose evenly
-  const int64_t words = ceil_div64((int64_t)3 * kColumnRows * c.cols, (int64_t)kTileRows * std::min(a.topk, c.cols));
-  p.words = (int)std::min<int64_t>(std::max<int64_t>((words + kColumnWords - 1) / kColumnWords * kColumnWords, kColumnWords), std::max(p.tiles, 1));
-  p.parts = ceil_div(p.tiles, p.words);
+  // workgroups of a page: three turns of rows each, if rows choose evenly
+  const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
+  p.parts = (int)std::min<int64_t>(std::max<int64_t>(visits / (3 * kColumnRows), 1), ceil_div(p.tiles, kColumnWords));
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 
