@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
 
 static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
 // whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own
-static bool many_rows(const fmoba_cache_attn_args &a, int cols) { return cols > 0 && a.max_seqlen_q > 8; }
+static bool many_rows(const fmoba_cache_attn_args &a, int cols) { return cols > 0 && a.max_seqlen_q > kRowFormRows; }
 // whether the rows' workgroups score their pages themselves
 static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= kOwnScores; }
 

@@ -13,13 +13,14 @@
 
 namespace fmoba {
 
+constexpr int kColumnCols = 32768;  // pages of a table, at most (a word of bits for each in LDS, and its number in a score)
 constexpr int kTileRows = 32;  // rows of a head that share a word of bits
 
 struct ColumnPlan {
   CacheAttn c;
   int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
   uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
-  float *scores;     // [block of 32 rows][head][32][cols], where LDS does not hold them
+  float *scores;     // [block of 32 rows][head][32 rows][half of the wave][slot], where LDS does not hold them
   float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum, scale of its page's values
   uint16_t *part;    // [(row, head)][topk4][head_dim]: its output in units of that scale, fp16
   int32_t topk4;     // topk, rounded up to a multiple of four
@@ -32,9 +33,13 @@ struct ColumnPlan {
 __device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRows + b; }
 
 // ------------------------------------------------------------------------------------
-// gate
+// gate: one wave takes 32 rows of a head.  Scores^T = means q^T, so that a lane has half of a row's scores (the other half of the wave the others), 16 of a
+// product's 32 pages.  A score gives its lowest bits up for the page's number; eight groups of a lane's scores are known by their largest, and the best
+// are taken off one by one: the largest of eight, whose group is then looked through again.  About 60 instructions for one page of 32 rows, where counting
+// scores above a cut (a ballot per 64 scores and bit) takes 30 for one bit of one row: XX instead of 142 us, 8191 tokens, 16 heads, 64 pages.
 // ------------------------------------------------------------------------------------
-constexpr int kGateCols = 1024;  // pages of a table whose scores of 32 rows LDS holds (128 KB)
+constexpr int kGateCols = 1024;   // pages whose scores of 32 rows LDS holds (135 KB); beyond, in the workspace
+constexpr int kGateGroups = 8;
 
 // row . mean of a page in 64 bits, by 16 lanes (four pages a wave)
 template <typename T>
@@ -62,196 +67,219 @@ __device__ __forceinline__ float wave_max(float x) {
   for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
   return x;
 }
+// sum of the squares of eight elements, added to s
+template <typename T>
+__device__ __forceinline__ float add_squares(const Pack8 &x, float s) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef T pair_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    pair_t v;
+    __builtin_memcpy(&v, &x.w[w], 4);
+    if constexpr (std::is_same<T, bf16_t>::value)
+      s = __builtin_amdgcn_fdot2_f32_bf16(v, v, s, false);
+    else
+      s = __builtin_amdgcn_fdot2(v, v, s, false);
+  }
+#endif
+  return s;
+}
+// where a lane keeps the score of page c of its row: tile of 32 pages, 16 of them in each half of the wave
+__device__ __forceinline__ int gate_half(int c) { return (c >> 2) & 1; }
+__device__ __forceinline__ int gate_slot(int c) { return (c >> 5) * 16 + ((c >> 3) & 3) * 4 + (c & 3); }
+__host__ __device__ __forceinline__ int gate_stride(int cols) { return (cols + 31) / 32 * 16 + 4; }  // floats of a lane (four more: 16 lanes' reads of 16 bytes meet all banks once)
 
 template <typename T, int HD, bool LDS>
-__global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p) {
+__global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_bits) {
   constexpr int KS = HD / 16;
-  extern __shared__ uint32_t smem[];  // bits of every page, then (LDS) the scores
-  __shared__ float sQ2[kTileRows], sMean2[4];
+  extern __shared__ __align__(16) float gate_smem[];  // (LDS) the scores, [row][half][slot]; then the bits of every page
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
+  const int lane = threadIdx.x, hh = lane >> 5, li = lane & 31;
   const int rb = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / G, cols = p.c.cols;
   const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
   const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q), row0 = rb * kTileRows;
   if (q0 < 0 || row0 >= R) return;
   const int shift = len - (q1 - q0);  // position of row 0
   const int rows = min(kTileRows, R - row0), last = shift + row0 + rows - 1;
-  const int npages = min((int)(((int64_t)max(len, 0) + P - 1) / P), cols);  // of the sequence
-  const int nscore = last < 0 ? 0 : min(last / P, cols - 1);                // that any of the rows can select beside its own
+  const int npages = min((int)(((int64_t)max(len, 0) + P - 1) / P), cols);                 // of the sequence
+  const int nscore = last < 0 || a.topk <= 1 ? 0 : min(last / P, cols - 1);                // that any of the rows can select beside its own
   const int32_t *table = a.block_table + (int64_t)b * a.table_stride;
-  uint32_t *sBits = smem;
-  float *scores = LDS ? reinterpret_cast<float *>(smem + cols) : p.scores + ((block_of(q0, b) + rb) * a.heads + h) * kTileRows * cols;
-  for (int i = tid; i < npages; i += 256) sBits[i] = 0u;
+  const int stride = gate_stride(cols);
+  float *scores = LDS ? gate_smem : p.scores + ((block_of(q0, b) + rb) * a.heads + h) * kTileRows * 2 * stride;
+  uint32_t *sBits = reinterpret_cast<uint32_t *>(gate_smem + (LDS ? kTileRows * 2 * stride : 0));
+  float *mine = scores + (li * 2 + hh) * stride;
   const uint16_t *qh = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row0) * a.q_row_stride + (int64_t)h * a.q_head_stride;
   const uint16_t *means = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + (int64_t)hk * D;
   const int64_t mean_stride = (int64_t)a.cache.heads_k * D;
+  for (int i = lane; i < npages; i += 64) sBits[i] = 0u;
+  // this lane's row (both halves have it), its own page and the candidates before it
+  const int pos = li < rows ? shift + row0 + li : -1;
+  const int own = pos >= 0 ? pos / P : -1, n_row = own < 0 ? 0 : min(own, nscore), want = min(a.topk - 1, n_row);
+  const int own_page = own >= 0 && own < cols ? table[own] : -1;
+  int32_t *sel = p.sel + ((int64_t)(q0 + row0 + min(li, rows - 1)) * a.heads + h) * p.topk4;
 
-  // ---- scores: 32 rows by 32 pages a wave and turn ----
-  if (a.topk > 1 && nscore > 0) {
-    Pack8 q[KS];
-    float q2 = 0.f;
+  // ---- scores ----
+  const int tiles = (nscore + 31) / 32, per_group = (tiles + kGateGroups - 1) / kGateGroups;
+  float top[kGateGroups], err = 0.f;
+#pragma unroll
+  for (int g = 0; g < kGateGroups; ++g) top[g] = -INFINITY;
+  if (nscore > 0) {
+    const uint32_t number = (1u << page_bits) - 1u;
+    Pack8 q[KS], k[KS];
+    float q2 = 0.f, mean2 = 0.f;
+    bool there = false;
+    auto load = [&](int tile) {
+      const int c = tile * 32 + li, page = tile < tiles && c < nscore ? table[c] : -1;
+      there = page >= 0 && page < a.cache.num_pages;
+      const uint16_t *mean = means + (int64_t)(there ? page : 0) * mean_stride + hh * 8;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[ks] = there && ks * 16 + hh * 8 < D ? ld_global16(mean + ks * 16) : zero_pack8();
+    };
+    load(0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int e = ks * 16 + hh * 8;
       q[ks] = e < D ? ld_global16(qh + (int64_t)min(li, rows - 1) * a.q_row_stride + e) : zero_pack8();
-      float f[8];
-      unpack8<T>(q[ks], f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q2 = fmaf(f[j], f[j], q2);
     }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q2 = add_squares<T>(q[ks], q2);
     q2 = sum_xor32_f(q2);
-    if (wave == 0 && hh == 0) sQ2[li] = q2;
-    float mean2 = 0.f;
-    for (int c0 = wave * 32; c0 < nscore; c0 += 128) {
-      const int c = c0 + li, page = c < nscore ? table[c] : -1;
-      const bool there = page >= 0 && page < a.cache.num_pages;
-      const uint16_t *mean = means + (int64_t)(there ? page : 0) * mean_stride;
-      Pack8 k[KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k[ks] = there && ks * 16 + hh * 8 < D ? ld_global16(mean + ks * 16 + hh * 8) : zero_pack8();
-      f32x16 acc;
+    for (int g = 0; g < kGateGroups; ++g)
+      for (int tile = g * per_group; tile < min((g + 1) * per_group, tiles); ++tile) {
+        f32x16 acc;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-      float k2 = 0.f;
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        float k2 = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        acc = mfma32<T>(q[ks], k[ks], acc);
-        float f[8];
-        unpack8<T>(k[ks], f);
+        for (int ks = 0; ks < KS; ++ks) acc = mfma32<T>(k[ks], q[ks], acc);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k2 = fmaf(f[j], f[j], k2);
+        for (int ks = 0; ks < KS; ++ks) k2 = add_squares<T>(k[ks], k2);
+        mean2 = fmaxf(mean2, sum_xor32_f(k2));
+        const uint32_t valid = (uint32_t)__ballot(there);  // (both halves ask for the same pages)
+        load(tile + 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int in_tile = 8 * j + 4 * hh + i, c = tile * 32 + in_tile;
+            const float s = __uint_as_float((__float_as_uint(acc[4 * j + i]) & ~number) | (uint32_t)c);
+            v[i] = c < n_row && ((valid >> in_tile) & 1u) ? s : NAN;  // (a NaN is never the largest)
+            top[g] = fmaxf(top[g], v[i]);
+          }
+          *reinterpret_cast<f32x4 *>(mine + tile * 16 + 4 * j) = v;
+        }
       }
-      mean2 = fmaxf(mean2, sum_xor32_f(k2));
-      if (c < nscore) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) scores[(int64_t)acc_row(i, hh) * cols + c] = there ? acc[i] : -INFINITY;
-      }
-    }
-    mean2 = wave_max(mean2);
-    if (lane == 0) sMean2[wave] = mean2;
+    // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-22 of
+    // |q| |mean|: scores further apart than twice that are in the order of 64 bits.
+    err = (float)D * 2.384185791015625e-7f * sqrtf(q2) * sqrtf(wave_max(mean2));
   }
+  // (an order in memory for what the lanes of the wave exchange: LDS or, of the scores, global memory)
   __syncthreads();
 
-  // ---- the best of every row ----
-  const float mean_norm = a.topk > 1 && nscore > 0 ? sqrtf(fmaxf(fmaxf(sMean2[0], sMean2[1]), fmaxf(sMean2[2], sMean2[3]))) : 0.f;
-  for (int r = wave; r < rows; r += 4) {
-    const int pos = shift + row0 + r;
-    int32_t *sel = p.sel + ((int64_t)(q0 + row0 + r) * a.heads + h) * p.topk4;
-    const int own = pos >= 0 ? pos / P : -1, n = own < 0 ? 0 : min(own, cols - 1), want = min(a.topk - 1, n);
-    float *sc = scores + (int64_t)r * cols;
-    auto take = [&](int c, uint32_t, int at) {
-      sel[at] = c;
-      atomicOr(&sBits[c], 1u << r);
-    };
-    auto key = [&](int c) { return sc[c] > -INFINITY ? float_order_key(sc[c] + 0.f) : 0u; };
-    auto self = [](int c) { return c; };
-    int picked = 0;
-    if (want > 0) {
-      // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-22 of
-      // |q| |mean|: scores further apart than twice that are in the order of 64 bits.
-      const float err = (float)D * 2.384185791015625e-7f * sqrtf(sQ2[r]) * mean_norm;
-      // the smallest score of the `want` best, and the largest of the others
-      uint32_t cut = 1u;
-      int m = 0;
-      uint32_t reg[4];
-      const bool small = n <= 256;
-      if (small) {
+  // ---- the best, one by one ----
+  auto set_bit = [&](int c, int r) { atomicOr(&sBits[c], 1u << r); };
+  int picked = 0;
+  float in = INFINITY, out = -INFINITY;  // the last one taken, and the best that was not
+  const uint32_t number = (1u << page_bits) - 1u;
+  int steps = want;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) reg[j] = j * 64 + lane < n ? key(j * 64 + lane) : 0u;
+  for (int o = 16; o >= 1; o >>= 1) steps = max(steps, __shfl_xor(steps, o, 64));
+  for (int i = 0; i <= steps && nscore > 0; ++i) {
+    float best = top[0];
+#pragma unroll
+    for (int g = 1; g < kGateGroups; ++g) best = fmaxf(best, top[g]);
+    best = max_xor32_f(best);
+    const bool any = best > -INFINITY;
+    if (any && i < want) {
+      const int c = (int)(__float_as_uint(best) & number), tile = c >> 5;
+      in = best;
+      ++picked;
+      if (hh == 0) {
+        sel[i] = c;
+        set_bit(c, li);
       }
-      auto each = [&](auto &&f) {
-        if (small) {
+      if (gate_half(c) == hh) {
+        mine[gate_slot(c)] = -INFINITY;  // taken
+        const int g = tile / per_group;
+        float m = -INFINITY;
+        for (int s = g * per_group; s < min((g + 1) * per_group, tiles); ++s)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f(j * 64 + lane, reg[j]);
-        } else {
-          for (int c = lane; c - lane < n; c += 64) f(c, c < n ? key(c) : 0u);
-        }
-      };
-      auto count_ge = [&](uint32_t v) {
-        int x = 0;
-        each([&](int, uint32_t k) { x += __popcll(__ballot(k >= v)); });
-        return x;
-      };
-      m = count_ge(1u);
-      const int candidates = m;
-      if (m > want) {
-        cut = 0u;
-        for (int bit = 31; bit >= 0; --bit) {
-          const uint32_t trial = cut | (1u << bit);
-          const int x = count_ge(trial);
-          if (x >= want) cut = trial, m = x;
-          if (x == want) break;
-        }
-      }
-      float in = INFINITY, out = -INFINITY;
-      each([&](int, uint32_t k) {
-        if (k >= cut)
-          in = fminf(in, order_key_float(k));
-        else if (k > 0u)
-          out = fmaxf(out, order_key_float(k));
-      });
-      in = -wave_max(-in), out = wave_max(out);
-      if (m > want) out = in;  // equal ones on both sides
-      if (err == 0.f && m > want) {  // products of zeros: equal they are, and the later pages come first
-        picked = pick_best<0>(n, want, lane, key, [](int) { return 0u; }, self, take);
-      } else if (err < 1e30f && (candidates <= want || in - out > 2.f * err)) {
-        each([&](int c, uint32_t k) {
-          const unsigned long long mask = __ballot(k >= cut);
-          if (k >= cut) take(c, k, picked + __popcll(mask & ((1ull << lane) - 1ull)));
-          picked += __popcll(mask);
-        });
-      } else {
-        // those above `hi` belong to the best whatever the errors are, those below `lo` do not; the others decide in 64 bits (all of them if the sizes overflow)
-        const float hi = err < 1e30f ? out + 2.f * err : INFINITY, lo = err < 1e30f ? in - 2.f * err : -INFINITY;
-        const bool all = !(err < 1e30f);
-        const uint16_t *qr = qh + (int64_t)r * a.q_row_stride;
-        for (int c0 = 0; c0 < n; c0 += 64) {
-          const int c = c0 + lane;
-          const float s = c < n ? sc[c] : -INFINITY;
-          const bool above = !all && s > hi;
-          const unsigned long long am = __ballot(above);
-          if (above) take(c, 0u, picked + __popcll(am & ((1ull << lane) - 1ull)));
-          picked += __popcll(am);
-          const int page = c < n ? table[c] : -1;
-          const bool near = page >= 0 && page < a.cache.num_pages && (all || (s >= lo && s <= hi));
-          uint32_t mine = 0u;
-          for (unsigned long long todo = __ballot(near); todo;) {  // four at a time
-            int l = -1;
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + s * 16 + 4 * j);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int first = todo ? (int)__ffsll(todo) - 1 : l;
-              if (lane >> 4 >= u) l = first;
-              todo &= todo - 1ull;
-            }
-            const uint64_t k = score_key(row16_dot<T>(qr, means + (int64_t)__shfl(page, l, 64) * mean_stride, D, lane));
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int to = __builtin_amdgcn_readlane(l, u * 16);
-              const uint32_t hi32 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), u * 16);
-              if (lane == to) mine = hi32;
-            }
+            for (int k = 0; k < 4; ++k) m = fmaxf(m, v[k]);
           }
-          if (c < n) sc[c] = __uint_as_float(mine);  // its own lane reads it below
-        }
-        const int at0 = picked;
-        picked += pick_best<0>(
-            n, want - picked, lane, [&](int c) { return __float_as_uint(sc[c]); },
-            [&](int c) { return (uint32_t)score_key(lane_dot<T>(qr, means + (int64_t)table[c] * mean_stride, D)); }, self, [&](int c, uint32_t k, int at) { take(c, k, at0 + at); });
+#pragma unroll
+        for (int k = 0; k < kGateGroups; ++k) top[k] = k == g ? m : top[k];
       }
+    } else if (any && i == want) {
+      out = best;
     }
-    const int own_page = own >= 0 && own < cols ? table[own] : -1;
-    const bool has_own = own_page >= 0 && own_page < a.cache.num_pages;
-    if (has_own && lane == 0) {
-      sel[picked] = own;
-      atomicOr(&sBits[own], 1u << r);
+  }
+
+  // ---- rows whose cut is too close, in 64 bits: of those taken and those within the error of the last one taken ----
+  // (the page's number in a score: less than 2^(page_bits - 23) of it.  Products of zeros are equal, and of them the later pages came first.)
+  const float near = 2.f * err + ldexpf(2.f * fmaxf(fabsf(in), fabsf(out)), page_bits - 23);
+  const bool zeros = err == 0.f && ((__float_as_uint(in) | __float_as_uint(out)) & ~number) == 0u;
+  const bool sized = err < 1e30f && (err > 0.f || zeros);  // (else sizes overflow or vanish, or are no numbers: all pages decide in 64 bits)
+  const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && !zeros && !(in - out > near)));
+  __syncthreads();
+  for (uint32_t todo = (uint32_t)__ballot(unsure && hh == 0); todo; todo &= todo - 1u) {
+    const int r = __ffs((int)todo) - 1;
+    const int n = __builtin_amdgcn_readlane(n_row, r), most = __builtin_amdgcn_readlane(want, r);
+    const bool all = __builtin_amdgcn_readlane((int)!sized, r) != 0;
+    const float lo = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(in - near), r));
+    float *rs = scores + r * 2 * stride;
+    int32_t *rsel = p.sel + ((int64_t)(q0 + row0 + r) * a.heads + h) * p.topk4;
+    const uint16_t *qr = qh + (int64_t)r * a.q_row_stride;
+    for (int c0 = 0; c0 < n; c0 += 64) {
+      const int c = c0 + lane, page = c < n ? table[c] : -1;
+      float *at = rs + gate_half(c) * stride + gate_slot(c);
+      const float s = c < n ? *at : NAN;
+      const bool taken = s == -INFINITY;
+      if (taken) atomicAnd(&sBits[c], ~(1u << r));
+      const bool decides = page >= 0 && page < a.cache.num_pages && (all || taken || s >= lo);
+      uint32_t key = 0u;
+      for (unsigned long long left = __ballot(decides); left;) {  // four at a time
+        int l = -1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int next = left ? (int)__ffsll(left) - 1 : l;
+          if (lane >> 4 >= u) l = next;
+          left &= left - 1ull;
+        }
+        const uint64_t x = score_key(row16_dot<T>(qr, means + (int64_t)__shfl(page, l, 64) * mean_stride, D, lane));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int to = __builtin_amdgcn_readlane(l, u * 16);
+          const uint32_t hi32 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u * 16);
+          if (lane == to) key = hi32;
+        }
+      }
+      if (c < n) *at = __uint_as_float(key);  // its own lane reads it below
     }
-    picked += has_own ? 1 : 0;
-    for (int i = picked + lane; i < p.topk4; i += 64) sel[i] = -1;
+    const int got = pick_best<0>(
+        n, most, lane, [&](int c) { return __float_as_uint(rs[gate_half(c) * stride + gate_slot(c)]); },
+        [&](int c) { return (uint32_t)score_key(lane_dot<T>(qr, means + (int64_t)table[c] * mean_stride, D)); }, [](int c) { return c; },
+        [&](int c, uint32_t, int i) {
+          rsel[i] = c;
+          set_bit(c, r);
+        });
+    if (li == r) picked = got;
+  }
+  if (hh == 0 && li < rows) {
+    if (own_page >= 0 && own_page < a.cache.num_pages) {
+      sel[picked++] = own;
+      set_bit(own, li);
+    }
+    for (int i = picked; i < p.topk4; ++i) sel[i] = -1;
   }
   __syncthreads();
   uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
-  for (int i = tid; i < npages; i += 256) bits[i] = sBits[i];
+  for (int i = lane; i < npages; i += 64) bits[i] = sBits[i];
 }
 
 // ------------------------------------------------------------------------------------
@@ -515,14 +543,27 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 // ------------------------------------------------------------------------------------
 // combine: LPR lanes a (row, head), eight features each
 // ------------------------------------------------------------------------------------
+// WEIGHT: what pages receive is added up in LDS for the 64 rows of the workgroup first (integers, so in no order): rows next to each other choose alike, and
+// atomics on few addresses of memory are slow (a million of them 180 us).
+constexpr int kCombineRows = 64, kCombineCols = 2048;
 template <typename T, int LPR, bool WEIGHT>
 __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
   constexpr int NS = 64 / LPR, AT_ONCE = 8;  // slots of a lane; rows asked for together
+  __shared__ unsigned long long sWeight[WEIGHT ? kCombineCols : 1];
   const fmoba_cache_attn_args &a = p.c.a;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim;
-  const int64_t rowhead = (int64_t)blockIdx.x * (256 / LPR) + tid / LPR;
-  if (rowhead >= (int64_t)a.total_q * a.heads) return;
-  const int t = (int)(rowhead / a.heads), h = (int)(rowhead - (int64_t)t * a.heads);
+  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim, h = blockIdx.y, t0 = blockIdx.x * kCombineRows;
+  const int hk = h / (a.heads / a.cache.heads_k), cols = min(p.c.cols, kCombineCols);
+  const int b0 = WEIGHT ? find_row_lane(a, t0).b : 0;
+  auto receive = [&](int b, int c, unsigned long long x) {
+    const int page = a.block_table[(int64_t)b * a.table_stride + c];
+    if (page >= 0 && page < a.cache.num_pages) atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)page * a.cache.heads_k + hk, x);
+  };
+  if constexpr (WEIGHT) {
+    for (int i = tid; i < cols; i += 256) sWeight[i] = 0ull;
+    __syncthreads();
+  }
+  for (int t = t0 + tid / LPR; t < min(t0 + kCombineRows, a.total_q); t += 256 / LPR) {
+  const int64_t rowhead = (int64_t)t * a.heads + h;
   const int32_t *sel = p.sel + rowhead * p.topk4;
   const float2 *head = p.head + rowhead * p.topk4;
   const uint16_t *part = p.part + rowhead * p.topk4 * D;
@@ -591,15 +632,22 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
   }
   if (li == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
   if constexpr (WEIGHT) {
-    const int hk = h / (a.heads / a.cache.heads_k);
-    const int32_t *table = a.block_table + (int64_t)(at.b < a.batch ? at.b : 0) * a.table_stride;
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
       const float part_of = w[j] * inv;
-      const int page = page_of[j] >= 0 ? table[page_of[j]] : -1;
-      if (part_of > 0.f && page >= 0 && page < a.cache.num_pages)
-        atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)page * a.cache.heads_k + hk, (unsigned long long)rintf(part_of * 4294967296.f));
+      if (!(part_of > 0.f) || page_of[j] < 0) continue;
+      const unsigned long long x = (unsigned long long)rintf(part_of * 4294967296.f);
+      if (at.b == b0 && page_of[j] < cols)
+        atomicAdd(&sWeight[page_of[j]], x);
+      else
+        receive(at.b, page_of[j], x);
     }
+  }
+  }
+  if constexpr (WEIGHT) {
+    __syncthreads();
+    for (int i = tid; i < cols; i += 256)
+      if (sWeight[i] != 0ull) receive(b0, i, sWeight[i]);
   }
 }
 
@@ -618,7 +666,7 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   ColumnSizes z;
   z.sel = up(rowheads * p.topk4 * 4);
   z.bits = up((size_t)a.heads * p.blocks * cols * 4);
-  z.scores = cols > kGateCols ? up((size_t)a.heads * p.blocks * kTileRows * cols * 4) : 0;
+  z.scores = cols > kGateCols ? up((size_t)a.heads * p.blocks * kTileRows * 2 * gate_stride(cols) * 4) : 0;
   z.head = up(rowheads * p.topk4 * 8);
   z.part = up(rowheads * p.topk4 * a.cache.head_dim * 2);
   z.total = z.sel + z.bits + z.scores + z.head + z.part;
@@ -643,10 +691,12 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.c.a;
   const dim3 grid(ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows), a.heads, a.batch);
   const bool lds = p.c.cols <= kGateCols;
-  const size_t bytes = (size_t)p.c.cols * 4 * (lds ? 1 + kTileRows : 1);
+  const size_t bytes = ((size_t)p.c.cols + (lds ? (size_t)kTileRows * 2 * gate_stride(p.c.cols) : 0)) * 4;
+  int page_bits = 1;
+  while ((1 << page_bits) < p.c.cols) ++page_bits;
   auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
   if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
-  hipLaunchKernelGGL(kern, grid, dim3(256), bytes, s, p);
+  hipLaunchKernelGGL(kern, grid, dim3(64), bytes, s, p, page_bits);
   FMOBA_LAUNCH_CHECK("cache_gate_kernel");
   return 0;
 }
@@ -673,8 +723,7 @@ static int launch_columns(const ColumnPlan &p, hipStream_t s) {
 }
 template <typename T, int LPR>
 static void launch_combine(const ColumnPlan &p, hipStream_t s) {
-  const int64_t rowheads = (int64_t)p.c.a.total_q * p.c.a.heads;
-  const dim3 grid((uint32_t)ceil_div64(rowheads, 256 / LPR));
+  const dim3 grid(ceil_div(p.c.a.total_q, kCombineRows), p.c.a.heads);
   if (p.c.a.add_weight)
     hipLaunchKernelGGL((cache_combine_kernel<T, LPR, true>), grid, dim3(256), 0, s, p);
   else
@@ -696,7 +745,7 @@ static int run_columns_as(const ColumnPlan &p, hipStream_t s) {
 
 int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   const fmoba_cache_attn_args &a = c.a;
-  FMOBA_REQUIRE(a.heads <= 65535 && a.batch <= 65535, "cache_attn: batch/heads too large for the launch grid");
+  FMOBA_REQUIRE(c.cols <= kColumnCols, "cache_attn: %d pages per sequence; at most %d are supported for more than %d rows of a sequence", c.cols, kColumnCols, kRowFormRows);
   ColumnPlan p{};
   p.c = c;
   const ColumnSizes z = column_sizes(a, c.cols, p);
