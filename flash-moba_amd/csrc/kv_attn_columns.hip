@@ -33,7 +33,7 @@ struct ColumnPlan {
 __device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRows + b; }
 
 // ------------------------------------------------------------------------------------
-// gate: one wave takes 32 rows of a head.  Scores^T = means q^T, so that a lane has half of a row's scores (the other half of the wave the others), 16 of a
+// gate: a workgroup takes 32 rows of a head, its waves a quarter of the pages each.  Scores^T = means q^T, so that a lane has half of a row's scores (the other half of the wave the others), 16 of a
 // product's 32 pages.  A score gives its lowest bits up for the page's number; eight groups of a lane's scores are known by their largest, and the best
 // are taken off one by one: the largest of eight, whose group is then looked through again.  About 60 instructions for one page of 32 rows, where counting
 // scores above a cut (a ballot per 64 scores and bit) takes 30 for one bit of one row: XX instead of 142 us, 8191 tokens, 16 heads, 64 pages.
@@ -84,18 +84,25 @@ __device__ __forceinline__ float add_squares(const Pack8 &x, float s) {
 #endif
   return s;
 }
+// what the lanes of a wave have written is there for its other lanes
+__device__ __forceinline__ void wave_memory_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
 // where a lane keeps the score of page c of its row: tile of 32 pages, 16 of them in each half of the wave
 __device__ __forceinline__ int gate_half(int c) { return (c >> 2) & 1; }
 __device__ __forceinline__ int gate_slot(int c) { return (c >> 5) * 16 + ((c >> 3) & 3) * 4 + (c & 3); }
 __host__ __device__ __forceinline__ int gate_stride(int cols) { return (cols + 31) / 32 * 16 + 4; }  // floats of a lane (four more: 16 lanes' reads of 16 bytes meet all banks once)
 
 template <typename T, int HD, bool LDS>
-__global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_bits) {
+__global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_bits) {
   constexpr int KS = HD / 16;
+  __shared__ float sTop[kGateGroups][64], sMean2[4];
   extern __shared__ __align__(16) float gate_smem[];  // (LDS) the scores, [row][half][slot]; then the bits of every page
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k;
-  const int lane = threadIdx.x, hh = lane >> 5, li = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
   const int rb = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / G, cols = p.c.cols;
   const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
   const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q), row0 = rb * kTileRows;
@@ -112,7 +119,7 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
   const uint16_t *qh = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row0) * a.q_row_stride + (int64_t)h * a.q_head_stride;
   const uint16_t *means = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + (int64_t)hk * D;
   const int64_t mean_stride = (int64_t)a.cache.heads_k * D;
-  for (int i = lane; i < npages; i += 64) sBits[i] = 0u;
+  for (int i = tid; i < npages; i += 256) sBits[i] = 0u;
   // this lane's row (both halves have it), its own page and the candidates before it
   const int pos = li < rows ? shift + row0 + li : -1;
   const int own = pos >= 0 ? pos / P : -1, n_row = own < 0 ? 0 : min(own, nscore), want = min(a.topk - 1, n_row);
@@ -121,13 +128,10 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
 
   // ---- scores ----
   const int tiles = (nscore + 31) / 32, per_group = (tiles + kGateGroups - 1) / kGateGroups;
-  float top[kGateGroups], err = 0.f;
-#pragma unroll
-  for (int g = 0; g < kGateGroups; ++g) top[g] = -INFINITY;
+  const uint32_t number = (1u << page_bits) - 1u;
+  float top[kGateGroups], q2 = 0.f, mean2 = 0.f;
   if (nscore > 0) {
-    const uint32_t number = (1u << page_bits) - 1u;
     Pack8 q[KS], k[KS];
-    float q2 = 0.f, mean2 = 0.f;
     bool there = false;
     auto load = [&](int tile) {
       const int c = tile * 32 + li, page = tile < tiles && c < nscore ? table[c] : -1;
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) k[ks] = there && ks * 16 + hh * 8 < D ? ld_global16(mean + ks * 16) : zero_pack8();
     };
-    load(0);
+    load(wave * per_group);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int e = ks * 16 + hh * 8;
@@ -146,8 +150,10 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
     for (int ks = 0; ks < KS; ++ks) q2 = add_squares<T>(q[ks], q2);
     q2 = sum_xor32_f(q2);
 #pragma unroll
-    for (int g = 0; g < kGateGroups; ++g)
-      for (int tile = g * per_group; tile < min((g + 1) * per_group, tiles); ++tile) {
+    for (int u = 0; u < kGateGroups / 4; ++u) {  // the groups of a wave
+      const int g = wave + 4 * u, end = min((g + 1) * per_group, tiles);
+      float best = -INFINITY;
+      for (int tile = g * per_group; tile < end; ++tile) {
         f32x16 acc;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = 0.f;
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
         for (int ks = 0; ks < KS; ++ks) k2 = add_squares<T>(k[ks], k2);
         mean2 = fmaxf(mean2, sum_xor32_f(k2));
         const uint32_t valid = (uint32_t)__ballot(there);  // (both halves ask for the same pages)
-        load(tile + 1);
+        load(tile + 1 < end ? tile + 1 : (g + 4) * per_group);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f32x4 v;
@@ -167,23 +173,31 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
             const int in_tile = 8 * j + 4 * hh + i, c = tile * 32 + in_tile;
             const float s = __uint_as_float((__float_as_uint(acc[4 * j + i]) & ~number) | (uint32_t)c);
             v[i] = c < n_row && ((valid >> in_tile) & 1u) ? s : NAN;  // (a NaN is never the largest)
-            top[g] = fmaxf(top[g], v[i]);
+            best = fmaxf(best, v[i]);
           }
           *reinterpret_cast<f32x4 *>(mine + tile * 16 + 4 * j) = v;
         }
       }
+      sTop[g][lane] = best;
+    }
+    mean2 = wave_max(mean2);
+    if (lane == 0) sMean2[wave] = mean2;
+  }
+  __syncthreads();
+  uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
+  if (wave == 0) {
+  float err = 0.f;
+#pragma unroll
+  for (int g = 0; g < kGateGroups; ++g) top[g] = nscore > 0 ? sTop[g][lane] : -INFINITY;
+  if (nscore > 0)
     // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-22 of
     // |q| |mean|: scores further apart than twice that are in the order of 64 bits.
-    err = (float)D * 2.384185791015625e-7f * sqrtf(q2) * sqrtf(wave_max(mean2));
-  }
-  // (an order in memory for what the lanes of the wave exchange: LDS or, of the scores, global memory)
-  __syncthreads();
+    err = (float)D * 2.384185791015625e-7f * sqrtf(q2) * sqrtf(fmaxf(fmaxf(sMean2[0], sMean2[1]), fmaxf(sMean2[2], sMean2[3])));
 
   // ---- the best, one by one ----
   auto set_bit = [&](int c, int r) { atomicOr(&sBits[c], 1u << r); };
   int picked = 0;
   float in = INFINITY, out = -INFINITY;  // the last one taken, and the best that was not
-  const uint32_t number = (1u << page_bits) - 1u;
   int steps = want;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) steps = max(steps, __shfl_xor(steps, o, 64));
@@ -226,7 +240,7 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
   const bool zeros = err == 0.f && ((__float_as_uint(in) | __float_as_uint(out)) & ~number) == 0u;
   const bool sized = err < 1e30f && (err > 0.f || zeros);  // (else sizes overflow or vanish, or are no numbers: all pages decide in 64 bits)
   const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && !zeros && !(in - out > near)));
-  __syncthreads();
+  if (__ballot(unsure) != 0ull) wave_memory_fence();  // (the lanes' scores, LDS or global memory, before other lanes read them)
   for (uint32_t todo = (uint32_t)__ballot(unsure && hh == 0); todo; todo &= todo - 1u) {
     const int r = __ffs((int)todo) - 1;
     const int n = __builtin_amdgcn_readlane(n_row, r), most = __builtin_amdgcn_readlane(want, r);
@@ -277,24 +291,26 @@ __global__ __launch_bounds__(64) void cache_gate_kernel(ColumnPlan p, int page_b
     }
     for (int i = picked; i < p.topk4; ++i) sel[i] = -1;
   }
+  }
   __syncthreads();
-  uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
-  for (int i = lane; i < npages; i += 64) bits[i] = sBits[i];
+  for (int i = tid; i < npages; i += 256) bits[i] = sBits[i];
 }
 
 // ------------------------------------------------------------------------------------
 // columns
 // ------------------------------------------------------------------------------------
 constexpr int kColumnRows = 128;  // of a turn: 32 a wave
-constexpr int kColumnWords = 32;  // words of bits that are spread out at a time
+constexpr int kColumnWords = 128;  // words of bits that are spread out at a time: 32 a wave
 constexpr int kColumnList = kColumnRows + kColumnWords * 32;
+constexpr int kColumnPart = 2048;  // words of a workgroup, at most: an entry of its list has 16 bits
 
-template <typename T, typename H, int HD, int KT>  // KT: keys of a softmax step
+// ONE: the page is one step of KT keys, which LDS holds
+template <typename T, typename H, int HD, int KT, bool ONE>  // KT: keys of a softmax step
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
   constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, ROW = HD * 2;  // (LDS rows of exactly HD elements, their pieces swizzled: tile_swz)
   extern __shared__ __align__(1024) uint8_t column_smem[];
-  __shared__ int sList[kColumnList];
-  __shared__ int sCount, sNan;
+  __shared__ uint16_t sList[kColumnList];
+  __shared__ int sFound[4], sNan;
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, cols = p.c.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
@@ -308,15 +324,19 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   const int shift = len - (q1 - q0), G_tiles = (R + kTileRows - 1) / kTileRows * G;
   // the words of rows that can see the page, shared out evenly
   const int first = max(c * P - shift, 0) / kTileRows * G;
-  const int each = ((G_tiles - first + p.parts - 1) / p.parts + kColumnWords - 1) / kColumnWords * kColumnWords;
+  const int each = ((G_tiles - first + p.parts - 1) / p.parts + 31) / 32 * 32;
   const int w0 = first + part * each, w1 = min(w0 + each, G_tiles);
   if (w0 >= w1) return;
   const int keys = min(P, len - c * P);  // of the page that are there
   const uint32_t *bits = p.bits + ((int64_t)hk * p.blocks + block_of(q0, b)) * G * cols + c;
   const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + (int64_t)page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride;
   const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + (int64_t)page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride;
-  uint32_t word = wave == 0 && lane < kColumnWords && w0 + lane < w1 ? bits[(int64_t)(w0 + lane) * cols] : 0u;  // (those of the next turn of words, always)
-  const float k_scale = a.cache.k_scale[(int64_t)page * a.cache.heads_k + hk] * a.softmax_scale * 1.4426950408889634f;
+  const int my_word = wave * 32 + li;
+  uint32_t word = hh == 0 && w0 + my_word < w1 ? bits[(int64_t)(w0 + my_word) * cols] : 0u;  // (those of the next turn of words, always)
+  // the scale of a score, its sign with q (the largest product is the largest score), and not 0 (times which a masked product would be no number)
+  const float scale_log2 = a.softmax_scale * 1.4426950408889634f, scale_abs = fabsf(scale_log2) * a.cache.k_scale[(int64_t)page * a.cache.heads_k + hk];
+  const float k_scale = scale_abs < 1e-30f ? 1e-30f : scale_abs;
+  const uint32_t q_sign = scale_log2 < 0.f ? 0x80008000u : 0u;
   const float v_scale = a.cache.v_scale[(int64_t)page * a.cache.heads_k + hk];
   if (tid == 0) sNan = 0;
 
@@ -343,18 +363,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
           u32x4_t ko, vo;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            float f[4], g[4];
-            H::unpack4(kx[u].w[half * 2 + w], f);
-            H::unpack4(vx[u].w[half * 2 + w], g);
-            ko[2 * w] = pack2<T>(f[0], f[1]), ko[2 * w + 1] = pack2<T>(f[2], f[3]);
-            if constexpr (H::kFormat == FMOBA_CACHE_E4M3) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                nan = nan || g[j] != g[j];
-                g[j] = g[j] != g[j] ? 0.f : g[j];
-              }
-            }
-            vo[2 * w] = pack2<f16_t>(g[0], g[1]), vo[2 * w + 1] = pack2<f16_t>(g[2], g[3]);
+            uint32_t lo, hi, vw = vx[u].w[half * 2 + w];
+            H::template widen4<T>(kx[u].w[half * 2 + w], lo, hi);
+            ko[2 * w] = lo, ko[2 * w + 1] = hi;
+            if (H::any_nan4(vw)) nan = true, vw = H::without_nan4(vw);
+            H::template widen4<f16_t>(vw, lo, hi);
+            vo[2 * w] = lo, vo[2 * w + 1] = hi;
           }
           const uint32_t at = (uint32_t)(r * ROW + ((piece + half) ^ tile_swz<HD>(r)) * 16);
           lds_write_vec(k_base + at, ko);
@@ -381,7 +395,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     const int idx = wave * 32 + li;
     const bool there = idx < count;
     const int entry = sList[from + min(idx, count - 1)];
-    const int w = entry >> 5, rb = w / G, g = w - rb * G, row = rb * kTileRows + (entry & 31);
+    const int w = w0 + (entry >> 5), rb = w / G, g = w - rb * G, row = rb * kTileRows + (entry & 31);
     const int lim = shift + row - c * P;  // last key of the page that the row sees
     const int64_t rowhead = (int64_t)(q0 + row) * a.heads + hk * G + g;
     const uint16_t *qr = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
@@ -390,6 +404,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     for (int ks = 0; ks < KS; ++ks) {
       const int e = tile_frag_piece<HD>(hh, ks) * 8;
       q[ks] = e < D ? ld_global16(qr + e) : zero_pack8();
+    }
+    if (q_sign != 0u) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[ks].w[i] ^= q_sign;
     }
     int slot = 0;
     {
@@ -405,13 +425,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    for (int k0 = 0; k0 < keys; k0 += held) {
-      if (held < P) {
+    for (int k0 = 0; k0 < (ONE ? 1 : keys); k0 += held) {
+      if (!ONE && held < P) {
         __syncthreads();
         stage(k0);
         __syncthreads();
       }
-      for (int s0 = 0; s0 < held && k0 + s0 < keys; s0 += KT) {
+      for (int s0 = 0; s0 < (ONE ? 1 : held) && k0 + s0 < keys; s0 += KT) {
         if (__ballot(there && lim >= k0 + s0) == 0ull) continue;
         const uint32_t off = (uint32_t)(s0 * ROW);
         f32x16 s[ST];
@@ -428,22 +448,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
           for (int t = 0; t < ST; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              s[t][i] = t * 32 + acc_row(i, hh) <= left ? s[t][i] * k_scale : -INFINITY;
-              mx = fmaxf(mx, s[t][i]);
-            }
-        } else {
-#pragma unroll
-          for (int t = 0; t < ST; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              s[t][i] *= k_scale;
-              mx = fmaxf(mx, s[t][i]);
-            }
+            for (int i = 0; i < 16; ++i) s[t][i] = t * 32 + acc_row(i, hh) <= left ? s[t][i] : -INFINITY;
         }
-        mx = max_xor32_f(mx);
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = max_xor32_f(mx) * k_scale;
         const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        if (k0 + s0 > 0) {
+        if (!ONE && k0 + s0 > 0) {
           const float resc = __builtin_amdgcn_exp2f(m - ref);
           l *= resc;
 #pragma unroll
@@ -460,7 +473,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
             Pack8 pk;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-              const float x = __builtin_amdgcn_exp2f(s[t][8 * u + i] - ref), y = __builtin_amdgcn_exp2f(s[t][8 * u + i + 1] - ref);
+              const float x = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i], k_scale, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i + 1], k_scale, -ref));
               sum += x + y;
               pk.w[i >> 1] = pack2<f16_t>(x, y);
             }
@@ -500,29 +513,32 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
   };
 
-  if (held >= P) stage(0);
+  if (ONE || held >= P) stage(0);
   int have = 0;  // entries of the list that wait
   for (int wb = w0; wb < w1; wb += kColumnWords) {
-    if (wave == 0) {
-      uint32_t x = word;
-      const int n = __popc(x);
-      int upto = n;
+    uint32_t x = word;
+    const int n = __popc(x);
+    int upto = n;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(upto, o, 64);
-        upto += lane >= o ? up : 0;
-      }
-      int at = have + upto - n;
-      while (x) {
-        sList[at++] = (wb + lane) << 5 | (__ffs(x) - 1);
-        x &= x - 1u;
-      }
-      if (lane == 63) sCount = have + upto;
-      const int next = wb + kColumnWords + lane;
-      word = lane < kColumnWords && next < w1 ? bits[(int64_t)next * cols] : 0u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up(upto, o, 32);
+      upto += li >= o ? before : 0;
+    }
+    if (lane == 31) sFound[wave] = upto;
+    const int next = wb + kColumnWords + my_word;
+    word = hh == 0 && next < w1 ? bits[(int64_t)next * cols] : 0u;
+    __syncthreads();
+    int at = have + upto - n, count = have;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      at += w < wave ? sFound[w] : 0;
+      count += sFound[w];
+    }
+    while (x) {
+      sList[at++] = (uint16_t)((wb - w0 + my_word) << 5 | (__ffs(x) - 1));
+      x &= x - 1u;
     }
     __syncthreads();
-    const int count = sCount;
     const bool end = wb + kColumnWords >= w1;
     int from = 0;
     while (count - from >= kColumnRows || (end && from < count)) {
@@ -532,9 +548,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     have = max(count - from, 0);
     __syncthreads();
     if (from > 0 && have > 0) {
-      const int x = tid < have ? sList[from + tid] : 0;
+      const uint16_t moved = tid < have ? sList[from + tid] : (uint16_t)0;
       __syncthreads();
-      if (tid < have) sList[tid] = x;
+      if (tid < have) sList[tid] = moved;
     }
     __syncthreads();
   }
@@ -696,13 +712,13 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   while ((1 << page_bits) < p.c.cols) ++page_bits;
   auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
   if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
-  hipLaunchKernelGGL(kern, grid, dim3(64), bytes, s, p, page_bits);
+  hipLaunchKernelGGL(kern, grid, dim3(256), bytes, s, p, page_bits);
   FMOBA_LAUNCH_CHECK("cache_gate_kernel");
   return 0;
 }
-template <typename T, typename H, int HD, int KT>
+template <typename T, typename H, int HD, int KT, bool ONE>
 static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
-  auto kern = cache_columns_kernel<T, H, HD, KT>;
+  auto kern = cache_columns_kernel<T, H, HD, KT, ONE>;
   const size_t bytes = (size_t)held * HD * 4;
   if (int rc = with_lds(kern, bytes, "cache_columns")) return rc;
   const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.parts;
@@ -716,10 +732,11 @@ static int launch_columns(const ColumnPlan &p, hipStream_t s) {
   const int P = p.c.a.cache.page_size;
   // the whole page where two workgroups find room on a compute unit, else 64 keys at a time
   const int held = P * HD * 4 <= 64 * 1024 ? P : 64;
-  if constexpr (HD <= 64) {
-    if (held % 128 == 0) return launch_columns_as<T, H, HD, 128>(p, held, s);
+  if constexpr (HD <= 128) {
+    if (P == 128) return launch_columns_as<T, H, HD, 128, true>(p, held, s);
   }
-  return launch_columns_as<T, H, HD, 64>(p, held, s);
+  if (P == 64) return launch_columns_as<T, H, HD, 64, true>(p, held, s);
+  return launch_columns_as<T, H, HD, 64, false>(p, held, s);
 }
 template <typename T, int LPR>
 static void launch_combine(const ColumnPlan &p, hipStream_t s) {
@@ -757,7 +774,7 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   p.part = reinterpret_cast<uint16_t *>(at);
   // workgroups of a page: three turns of rows each, if rows choose evenly
   const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
-  p.parts = (int)std::min<int64_t>(std::max<int64_t>(visits / (3 * kColumnRows), 1), ceil_div(p.tiles, kColumnWords));
+  p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (3 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32));
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 

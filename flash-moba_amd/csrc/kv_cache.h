@@ -18,6 +18,30 @@ struct HeldE4M3 {
     (void)w, (void)f;
 #endif
   }
+  // four values as two words of two 16-bit elements, exact
+  template <typename T>
+  static __device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (std::is_same<T, bf16_t>::value) {
+      const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, true);
+      __builtin_memcpy(&lo, &a, 4);
+      __builtin_memcpy(&hi, &b, 4);
+    } else {
+      const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, true);
+      __builtin_memcpy(&lo, &a, 4);
+      __builtin_memcpy(&hi, &b, 4);
+    }
+#else
+    (void)w, (void)lo, (void)hi;
+#endif
+  }
+  // whether any of four values is NaN (all bits but the sign set)
+  static __device__ __forceinline__ bool any_nan4(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u; }
+  // the values with zeros for NaNs
+  static __device__ __forceinline__ uint32_t without_nan4(uint32_t w) {
+    const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in the bytes that are
+    return w & ~(nan * 255u);
+  }
   static __device__ __forceinline__ float limit(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
   static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -37,6 +61,15 @@ struct HeldInt8 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w >> (8 * i));
   }
+  template <typename T>
+  static __device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    float f[4];
+    unpack4(w, f);
+    lo = pack2<T>(f[0], f[1]);
+    hi = pack2<T>(f[2], f[3]);
+  }
+  static __device__ __forceinline__ bool any_nan4(uint32_t) { return false; }
+  static __device__ __forceinline__ uint32_t without_nan4(uint32_t w) { return w; }
   static __device__ __forceinline__ uint32_t pack1(float x) { return (uint32_t)(int)(x != x ? 0.f : rintf(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu; }
   static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack1(a) | pack1(b) << 8 | pack1(c) << 16 | pack1(d) << 24; }
   // 127 = 1.984375 * 2^6

@@ -233,6 +233,19 @@ def test_values_that_are_no_ordinary_numbers(rows):
 
 
 @gpu
+@pytest.mark.parametrize("P", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 4.0])
+def test_scales_of_any_sign_and_pages_without_any(scale, rows, P):
+    cache, table, q, cu = setup(4, 2, 64, P, [rows], [P * 5 + 30], torch.bfloat16, torch.float8_e4m3fn)
+    cache.k_scale[table[0][2]] = 0.0
+    cache.v_scale[table[0][3]] = 0.0
+    out, lse = call(cache, table, q, cu, [P * 5 + 30], 4, softmax_scale=scale)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [P * 5 + 30], table, 4, scale=scale)
+    check(out, lse, want, want_lse, sizes, rows > 8)
+
+
+@gpu
 def test_strides_scales_and_broadcast():
     P, dim = 128, 64
     lens_q, lens_k = [1, 2], [300, 1000]
