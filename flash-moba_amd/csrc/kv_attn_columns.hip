@@ -84,12 +84,6 @@ __device__ __forceinline__ float add_squares(const Pack8 &x, float s) {
 #endif
   return s;
 }
-// what the lanes of a wave have written is there for its other lanes
-__device__ __forceinline__ void wave_memory_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-}
 // where a lane keeps the score of page c of its row: tile of 32 pages, 16 of them in each half of the wave
 __device__ __forceinline__ int gate_half(int c) { return (c >> 2) & 1; }
 __device__ __forceinline__ int gate_slot(int c) { return (c >> 5) * 16 + ((c >> 3) & 3) * 4 + (c & 3); }
@@ -98,7 +92,9 @@ __host__ __device__ __forceinline__ int gate_stride(int cols) { return (cols + 3
 template <typename T, int HD, bool LDS>
 __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_bits) {
   constexpr int KS = HD / 16;
-  __shared__ float sTop[kGateGroups][64], sMean2[4];
+  __shared__ float sTop[kGateGroups][64], sMean2[4], sLow[kTileRows];
+  __shared__ int sPicked[kTileRows], sCandidate[4][64];
+  __shared__ uint32_t sUnsure, sAll;
   extern __shared__ __align__(16) float gate_smem[];  // (LDS) the scores, [row][half][slot]; then the bits of every page
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k;
@@ -119,7 +115,8 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   const uint16_t *qh = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row0) * a.q_row_stride + (int64_t)h * a.q_head_stride;
   const uint16_t *means = reinterpret_cast<const uint16_t *>(a.cache.k_mean) + (int64_t)hk * D;
   const int64_t mean_stride = (int64_t)a.cache.heads_k * D;
-  for (int i = tid; i < npages; i += 256) sBits[i] = 0u;
+  const int nw = blockDim.x >> 6;
+  for (int i = tid; i < npages; i += blockDim.x) sBits[i] = 0u;
   // this lane's row (both halves have it), its own page and the candidates before it
   const int pos = li < rows ? shift + row0 + li : -1;
   const int own = pos >= 0 ? pos / P : -1, n_row = own < 0 ? 0 : min(own, nscore), want = min(a.topk - 1, n_row);
@@ -149,9 +146,8 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q2 = add_squares<T>(q[ks], q2);
     q2 = sum_xor32_f(q2);
-#pragma unroll
-    for (int u = 0; u < kGateGroups / 4; ++u) {  // the groups of a wave
-      const int g = wave + 4 * u, end = min((g + 1) * per_group, tiles);
+    for (int g = wave; g < kGateGroups; g += nw) {  // the groups of a wave
+      const int end = min((g + 1) * per_group, tiles);
       float best = -INFINITY;
       for (int tile = g * per_group; tile < end; ++tile) {
         f32x16 acc;
@@ -164,7 +160,7 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
         for (int ks = 0; ks < KS; ++ks) k2 = add_squares<T>(k[ks], k2);
         mean2 = fmaxf(mean2, sum_xor32_f(k2));
         const uint32_t valid = (uint32_t)__ballot(there);  // (both halves ask for the same pages)
-        load(tile + 1 < end ? tile + 1 : (g + 4) * per_group);
+        load(tile + 1 < end ? tile + 1 : (g + nw) * per_group);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f32x4 v;
@@ -184,116 +180,159 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
     if (lane == 0) sMean2[wave] = mean2;
   }
   __syncthreads();
-  uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
-  if (wave == 0) {
-  float err = 0.f;
-#pragma unroll
-  for (int g = 0; g < kGateGroups; ++g) top[g] = nscore > 0 ? sTop[g][lane] : -INFINITY;
-  if (nscore > 0)
-    // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-22 of
-    // |q| |mean|: scores further apart than twice that are in the order of 64 bits.
-    err = (float)D * 2.384185791015625e-7f * sqrtf(q2) * sqrtf(fmaxf(fmaxf(sMean2[0], sMean2[1]), fmaxf(sMean2[2], sMean2[3])));
-
-  // ---- the best, one by one ----
   auto set_bit = [&](int c, int r) { atomicOr(&sBits[c], 1u << r); };
-  int picked = 0;
-  float in = INFINITY, out = -INFINITY;  // the last one taken, and the best that was not
-  int steps = want;
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) steps = max(steps, __shfl_xor(steps, o, 64));
-  for (int i = 0; i <= steps && nscore > 0; ++i) {
-    float best = top[0];
-#pragma unroll
-    for (int g = 1; g < kGateGroups; ++g) best = fmaxf(best, top[g]);
-    best = max_xor32_f(best);
-    const bool any = best > -INFINITY;
-    if (any && i < want) {
-      const int c = (int)(__float_as_uint(best) & number), tile = c >> 5;
-      in = best;
-      ++picked;
-      if (hh == 0) {
-        sel[i] = c;
-        set_bit(c, li);
-      }
-      if (gate_half(c) == hh) {
-        mine[gate_slot(c)] = -INFINITY;  // taken
-        const int g = tile / per_group;
-        float m = -INFINITY;
-        for (int s = g * per_group; s < min((g + 1) * per_group, tiles); ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + s * 16 + 4 * j);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m = fmaxf(m, v[k]);
-          }
-#pragma unroll
-        for (int k = 0; k < kGateGroups; ++k) top[k] = k == g ? m : top[k];
-      }
-    } else if (any && i == want) {
-      out = best;
-    }
-  }
 
-  // ---- rows whose cut is too close, in 64 bits: of those taken and those within the error of the last one taken ----
-  // (the page's number in a score: less than 2^(page_bits - 23) of it.  Products of zeros are equal, and of them the later pages came first.)
-  const float near = 2.f * err + ldexpf(2.f * fmaxf(fabsf(in), fabsf(out)), page_bits - 23);
-  const bool zeros = err == 0.f && ((__float_as_uint(in) | __float_as_uint(out)) & ~number) == 0u;
-  const bool sized = err < 1e30f && (err > 0.f || zeros);  // (else sizes overflow or vanish, or are no numbers: all pages decide in 64 bits)
-  const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && !zeros && !(in - out > near)));
-  if (__ballot(unsure) != 0ull) wave_memory_fence();  // (the lanes' scores, LDS or global memory, before other lanes read them)
-  for (uint32_t todo = (uint32_t)__ballot(unsure && hh == 0); todo; todo &= todo - 1u) {
-    const int r = __ffs((int)todo) - 1;
-    const int n = __builtin_amdgcn_readlane(n_row, r), most = __builtin_amdgcn_readlane(want, r);
-    const bool all = __builtin_amdgcn_readlane((int)!sized, r) != 0;
-    const float lo = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(in - near), r));
+  // ---- the best, one by one, by the first wave ----
+  if (wave == 0) {
+    float err = 0.f;
+    // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-23 of
+    // |q| |mean| (and these by less than 2^-10): scores further apart than twice that are in the order of 64 bits.
+    if (nscore > 0) {
+      for (int w = 0; w < nw; ++w) mean2 = fmaxf(mean2, sMean2[w]);
+      err = (float)D * (1.192092896e-7f * 1.002f) * sqrtf(q2) * sqrtf(mean2);
+    }
+#pragma unroll
+    for (int g = 0; g < kGateGroups; ++g) top[g] = nscore > 0 ? sTop[g][lane] : -INFINITY;
+    int picked = 0;
+    float in = INFINITY, out = -INFINITY;  // the last one taken, and the best that was not
+    int steps = want;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) steps = max(steps, __shfl_xor(steps, o, 64));
+    for (int i = 0; i <= steps && nscore > 0; ++i) {
+      float best = top[0];
+#pragma unroll
+      for (int g = 1; g < kGateGroups; ++g) best = fmaxf(best, top[g]);
+      best = max_xor32_f(best);
+      const bool any = best > -INFINITY;
+      if (any && i < want) {
+        const int c = (int)(__float_as_uint(best) & number), tile = c >> 5;
+        in = best;
+        ++picked;
+        if (hh == 0) {
+          sel[i] = c;
+          set_bit(c, li);
+        }
+        if (gate_half(c) == hh) {
+          mine[gate_slot(c)] = -INFINITY;  // taken
+          const int g = tile / per_group;
+          float m = -INFINITY;
+          for (int s = g * per_group; s < min((g + 1) * per_group, tiles); ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + s * 16 + 4 * j);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) m = fmaxf(m, v[k]);
+            }
+#pragma unroll
+          for (int k = 0; k < kGateGroups; ++k) top[k] = k == g ? m : top[k];
+        }
+      } else if (any && i == want) {
+        out = best;
+      }
+    }
+    // Rows whose cut is too close for 32 bits.  (The page's number in a score: less than 2^(page_bits - 23) of it.  Products of zeros are equal, and of them the
+    // later pages came first.)
+    const float near = 2.f * err + ldexpf(2.f * fmaxf(fabsf(in), fabsf(out)), page_bits - 23);
+    const bool zeros = err == 0.f && ((__float_as_uint(in) | __float_as_uint(out)) & ~number) == 0u;
+    const bool sized = err < 1e30f && (err > 0.f || zeros);  // (else sizes overflow or vanish, or are no numbers: all pages decide in 64 bits)
+    const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && !zeros && !(in - out > near)));
+    if (hh == 0) sPicked[li] = picked, sLow[li] = in - near;
+    const uint32_t unsure_rows = (uint32_t)__ballot(unsure), all_rows = (uint32_t)__ballot(!sized);
+    if (lane == 0) sUnsure = unsure_rows, sAll = all_rows;
+  }
+  __syncthreads();
+
+  // ---- these in 64 bits, by all waves: of the pages taken and those that the errors could bring before them, the best ----
+  int nth = 0;
+  for (uint32_t todo = sUnsure; todo; todo &= todo - 1u, ++nth) {
+    if (nth % nw != wave) continue;
+    const int r = __ffs((int)todo) - 1, n = __builtin_amdgcn_readlane(n_row, r), most = __builtin_amdgcn_readlane(want, r);
+    const bool all = (sAll >> r) & 1u;
+    const float low = sLow[r];
     float *rs = scores + r * 2 * stride;
     int32_t *rsel = p.sel + ((int64_t)(q0 + row0 + r) * a.heads + h) * p.topk4;
     const uint16_t *qr = qh + (int64_t)r * a.q_row_stride;
+    auto at = [&](int c) { return rs + gate_half(c) * stride + gate_slot(c); };
+    auto score64 = [&](int page) { return score_key(row16_dot<T>(qr, means + (int64_t)page * mean_stride, D, lane)); };
+    int m = 0, got;
     for (int c0 = 0; c0 < n; c0 += 64) {
-      const int c = c0 + lane, page = c < n ? table[c] : -1;
-      float *at = rs + gate_half(c) * stride + gate_slot(c);
-      const float s = c < n ? *at : NAN;
-      const bool taken = s == -INFINITY;
+      const int c = c0 + lane;
+      const float s = c < n ? *at(c) : NAN;
+      const bool taken = s == -INFINITY, decides = taken || s >= low;
+      const unsigned long long mask = __ballot(decides);
+      const int place = m + __popcll(mask & ((1ull << lane) - 1ull));
+      if (decides && place < 64) sCandidate[wave][place] = c;
       if (taken) atomicAnd(&sBits[c], ~(1u << r));
-      const bool decides = page >= 0 && page < a.cache.num_pages && (all || taken || s >= lo);
-      uint32_t key = 0u;
-      for (unsigned long long left = __ballot(decides); left;) {  // four at a time
-        int l = -1;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int next = left ? (int)__ffsll(left) - 1 : l;
-          if (lane >> 4 >= u) l = next;
-          left &= left - 1ull;
-        }
-        const uint64_t x = score_key(row16_dot<T>(qr, means + (int64_t)__shfl(page, l, 64) * mean_stride, D, lane));
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int to = __builtin_amdgcn_readlane(l, u * 16);
-          const uint32_t hi32 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u * 16);
-          if (lane == to) key = hi32;
-        }
-      }
-      if (c < n) *at = __uint_as_float(key);  // its own lane reads it below
+      m += __popcll(mask);
     }
-    const int got = pick_best<0>(
-        n, most, lane, [&](int c) { return __float_as_uint(rs[gate_half(c) * stride + gate_slot(c)]); },
-        [&](int c) { return (uint32_t)score_key(lane_dot<T>(qr, means + (int64_t)table[c] * mean_stride, D)); }, [](int c) { return c; },
-        [&](int c, uint32_t, int i) {
-          rsel[i] = c;
-          set_bit(c, r);
-        });
-    if (li == r) picked = got;
+    wave_lds_fence();
+    if (m <= 64 && !all) {  // one a lane
+      const int c = lane < m ? sCandidate[wave][lane] : 0, page = table[c];
+      uint64_t key = 0ull;
+      for (int i = 0; i < m; i += 4) {  // 16 lanes a product
+        const uint64_t x = score64(__shfl(page, min(i + (lane >> 4), m - 1), 64));
+        const uint64_t y = __shfl(x, (lane & 3) * 16, 64);
+        if ((lane >> 2) == (i >> 2)) key = y;
+      }
+      if (lane >= m) key = 0ull;
+      int rank = 0;
+      for (int i = 0; i < m; ++i) {
+        const uint64_t other = __shfl(key, i, 64);
+        rank += other > key || (other == key && __builtin_amdgcn_readlane(c, i) > c) ? 1 : 0;
+      }
+      const bool chosen = key != 0ull && rank < most;
+      const unsigned long long mask = __ballot(chosen);
+      if (chosen) {
+        rsel[__popcll(mask & ((1ull << lane) - 1ull))] = c;
+        set_bit(c, r);
+      }
+      got = __popcll(mask);
+    } else {
+      for (int c0 = 0; c0 < n; c0 += 64) {
+        const int c = c0 + lane, page = c < n ? table[c] : -1;
+        const float s = c < n ? *at(c) : NAN;
+        const bool decides = page >= 0 && page < a.cache.num_pages && (all || s == -INFINITY || s >= low);
+        uint32_t key = 0u;
+        for (unsigned long long left = __ballot(decides); left;) {  // four at a time
+          int l = -1;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int next = left ? (int)__ffsll(left) - 1 : l;
+            if (lane >> 4 >= u) l = next;
+            left &= left - 1ull;
+          }
+          const uint64_t x = score64(__shfl(page, l, 64));
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int to = __builtin_amdgcn_readlane(l, u * 16);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u * 16);
+            if (lane == to) key = hi;
+          }
+        }
+        if (c < n) *at(c) = __uint_as_float(key);  // its own lane reads it below
+      }
+      got = pick_best<0>(
+          n, most, lane, [&](int c) { return __float_as_uint(*at(c)); }, [&](int c) { return (uint32_t)score_key(lane_dot<T>(qr, means + (int64_t)table[c] * mean_stride, D)); },
+          [](int c) { return c; },
+          [&](int c, uint32_t, int i) {
+            rsel[i] = c;
+            set_bit(c, r);
+          });
+    }
+    if (lane == 0) sPicked[r] = got;
   }
-  if (hh == 0 && li < rows) {
+  __syncthreads();
+  if (wave == 0 && hh == 0 && li < rows) {
+    int picked = sPicked[li];
     if (own_page >= 0 && own_page < a.cache.num_pages) {
       sel[picked++] = own;
       set_bit(own, li);
     }
     for (int i = picked; i < p.topk4; ++i) sel[i] = -1;
   }
-  }
   __syncthreads();
-  for (int i = tid; i < npages; i += 256) bits[i] = sBits[i];
+  uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
+  for (int i = tid; i < npages; i += blockDim.x) bits[i] = sBits[i];
 }
 
 // ------------------------------------------------------------------------------------
@@ -390,6 +429,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     for (int d = 0; d < DT; ++d) v_lo[d] = v_base + tile_tr_addr<HD>(v0, d), v_hi[d] = v_base + tile_tr_addr8<HD>(v0, d);
   }
 
+  // the value of the lane of this half with lane % 32 = lane % 16, or 16 + lane % 16
+  auto of_pair = [&](int64_t x, bool odd) {
+    const UPair lo = swap16((uint32_t)x), hi = swap16((uint32_t)((uint64_t)x >> 32));
+    return (int64_t)((uint64_t)(odd ? hi.b : hi.a) << 32 | (odd ? lo.b : lo.a));
+  };
   // one turn: up to 128 entries of the list from `from` on
   auto turn = [&](int from, int count) {
     const int idx = wave * 32 + li;
@@ -398,12 +442,18 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     const int w = w0 + (entry >> 5), rb = w / G, g = w - rb * G, row = rb * kTileRows + (entry & 31);
     const int lim = shift + row - c * P;  // last key of the page that the row sees
     const int64_t rowhead = (int64_t)(q0 + row) * a.heads + hk * G + g;
-    const uint16_t *qr = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
+    // the rows' queries, four lanes 64 bytes of a row at a time, each lane of entries lane % 16 and 16 + lane % 16 (q_rows_load)
     Pack8 q[KS];
+    {
+      const int64_t qr = (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
+      const uint16_t *even = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, false), *odd = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, true);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int e = tile_frag_piece<HD>(hh, ks) * 8;
-      q[ks] = e < D ? ld_global16(qr + e) : zero_pack8();
+      for (int i = 0; i < HD / 32; ++i) {
+        const int e = min((4 * i + (lane >> 4)) * 8, D - 8);  // (features past D: zeroed by the exchange)
+        q[2 * i] = ld_global16(even + e);
+        q[2 * i + 1] = ld_global16(odd + e);
+      }
+      q_rows_arrange<HD>(q, hh, D);
     }
     if (q_sign != 0u) {
 #pragma unroll
@@ -486,27 +536,43 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
     const int64_t at = rowhead * p.topk4 + slot;
     uint16_t *dst = p.part + at * D;
-    if (there) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      if (hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
-      // features 8 j + 4 hh .. of both halves to eight of one lane: 16 bytes each
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
+    {
+      // Features 8 j + 4 hh .. of both halves to eight of one lane, then to four lanes with 64 bytes of a row, as the queries were loaded: stores of 16 bytes of 64
+      // rows at a time take the caches a cycle for each.
+      uint16_t *even = p.part + of_pair(at * D, false), *odd = p.part + of_pair(at * D, true);
+      const bool even_there = wave * 32 + (lane & 15) < count, odd_there = wave * 32 + 16 + (lane & 15) < count;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
+        uint32_t x[4], y[4];  // pieces 4 d + hh and 4 d + 2 + hh of row li
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          uint32_t x0 = pack2<f16_t>(o[d][4 * j] * inv, o[d][4 * j + 1] * inv), x1 = pack2<f16_t>(o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv);
-          uint32_t y0 = pack2<f16_t>(o[d][4 * j + 4] * inv, o[d][4 * j + 5] * inv), y1 = pack2<f16_t>(o[d][4 * j + 6] * inv, o[d][4 * j + 7] * inv);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) (j < 2 ? x : y)[(j & 1) * 2 + i] = pack2<f16_t>(o[d][4 * j + 2 * i] * inv, o[d][4 * j + 2 * i + 1] * inv);
 #if defined(__HIP_DEVICE_COMPILE__)
-          const auto r0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), r1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
-          x0 = r0[0], y0 = r0[1], x1 = r1[0], y1 = r1[1];
-#endif
-          const int e = d * 32 + 8 * j + 8 * hh;
-          if (e < D) *reinterpret_cast<Pack8 *>(dst + e) = Pack8{{x0, x1, y0, y1}};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto r = __builtin_amdgcn_permlane32_swap(x[i], x[2 + i], false, false), s = __builtin_amdgcn_permlane32_swap(y[i], y[2 + i], false, false);
+          x[i] = r[0], x[2 + i] = r[1], y[i] = s[0], y[2 + i] = s[1];
         }
-      // NaNs among the values of the page: a row that sees one has it in that feature
-      if (H::kFormat == FMOBA_CACHE_E4M3 && sNan != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const auto r = __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false);
+          x[i] = r[0], y[i] = r[1];
+        }
+#endif
+        const int e = d * 32 + ((lane >> 4 & 1) * 2 + hh) * 8;
+        if (e < D && even_there) *reinterpret_cast<Pack8 *>(even + e) = Pack8{{x[0], x[1], x[2], x[3]}};
+        if (e < D && odd_there) *reinterpret_cast<Pack8 *>(odd + e) = Pack8{{y[0], y[1], y[2], y[3]}};
+      }
+    }
+    // NaNs among the values of the page: a row that sees one has it in that feature
+    if (H::kFormat == FMOBA_CACHE_E4M3 && sNan != 0) {
+      wait_all_loads();  // (the stores above, which other lanes made)
+      if (there) {
         const int last = min(lim, keys - 1);
-        for (int e = hh * 8; e < D; e += (e & 7) == 7 ? 9 : 1)  // (the features that this lane has written)
+        for (int e = hh; e < D; e += 2)
           for (int k = 0; k <= last; ++k)
             if ((vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) dst[e] = 0x7e00;
       }
@@ -712,7 +778,8 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   while ((1 << page_bits) < p.c.cols) ++page_bits;
   auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
   if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
-  hipLaunchKernelGGL(kern, grid, dim3(256), bytes, s, p, page_bits);
+  const int waves = p.c.cols <= 64 ? 1 : p.c.cols <= 320 ? 2 : 4;
+  hipLaunchKernelGGL(kern, grid, dim3(64 * waves), bytes, s, p, page_bits);
   FMOBA_LAUNCH_CHECK("cache_gate_kernel");
   return 0;
 }
