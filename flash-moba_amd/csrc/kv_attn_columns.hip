@@ -434,41 +434,49 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     const UPair lo = swap16((uint32_t)x), hi = swap16((uint32_t)((uint64_t)x >> 32));
     return (int64_t)((uint64_t)(odd ? hi.b : hi.a) << 32 | (odd ? lo.b : lo.a));
   };
-  // one turn: up to 128 entries of the list from `from` on
-  auto turn = [&](int from, int count) {
-    const int idx = wave * 32 + li;
-    const bool there = idx < count;
-    const int entry = sList[from + min(idx, count - 1)];
-    const int w = w0 + (entry >> 5), rb = w / G, g = w - rb * G, row = rb * kTileRows + (entry & 31);
-    const int lim = shift + row - c * P;  // last key of the page that the row sees
-    const int64_t rowhead = (int64_t)(q0 + row) * a.heads + hk * G + g;
-    // the rows' queries, four lanes 64 bytes of a row at a time, each lane of entries lane % 16 and 16 + lane % 16 (q_rows_load)
-    Pack8 q[KS];
-    {
-      const int64_t qr = (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
-      const uint16_t *even = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, false), *odd = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, true);
+  // What a turn of 128 entries of the list needs of memory: the rows' queries, four lanes 64 bytes of a row at a time, each lane of entries lane % 16 and
+  // 16 + lane % 16 (q_rows_load), and the first of their pages, among which the visit's place is.  Asked for while the turn before is under way, once its
+  // products with the keys are done (the registers of its queries are free then).
+  Pack8 q[KS];
+  int4 pages[2];
+  int row, g;
+  int64_t rowhead;
+  auto ask = [&](int from, int count) {
+    const int entry = sList[from + min(wave * 32 + li, count - 1)], w = w0 + (entry >> 5), rb = w / G;
+    g = w - rb * G, row = rb * kTileRows + (entry & 31);
+    rowhead = (int64_t)(q0 + row) * a.heads + hk * G + g;
+    const int64_t qr = (int64_t)(q0 + row) * a.q_row_stride + (int64_t)(hk * G + g) * a.q_head_stride;
+    const uint16_t *even = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, false), *odd = reinterpret_cast<const uint16_t *>(a.q) + of_pair(qr, true);
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int e = min((4 * i + (lane >> 4)) * 8, D - 8);  // (features past D: zeroed by the exchange)
-        q[2 * i] = ld_global16(even + e);
-        q[2 * i + 1] = ld_global16(odd + e);
-      }
-      q_rows_arrange<HD>(q, hh, D);
+    for (int i = 0; i < HD / 32; ++i) {
+      const int e = min((4 * i + (lane >> 4)) * 8, D - 8);  // (features past D: zeroed by the exchange)
+      q[2 * i] = ld_global16(even + e);
+      q[2 * i + 1] = ld_global16(odd + e);
     }
+    const int4 *sel = reinterpret_cast<const int4 *>(p.sel + rowhead * p.topk4);
+    pages[0] = sel[0], pages[1] = sel[p.topk4 > 4 ? 1 : 0];
+  };
+  auto place = [&]() {  // of the visit among the row's
+    auto among = [&](const int4 &s, int i, int slot) { return s.x == c ? i : s.y == c ? i + 1 : s.z == c ? i + 2 : s.w == c ? i + 3 : slot; };
+    int slot = among(pages[0], 0, among(pages[1], 4, 0));
+    const int4 *sel = reinterpret_cast<const int4 *>(p.sel + rowhead * p.topk4);
+    for (int i = 8; i < p.topk4; i += 4) slot = among(sel[i >> 2], i, slot);
+    return slot;
+  };
+  // one turn: up to 128 entries of the list from `from` on, which were asked for; `next`: as many behind them follow
+  auto turn = [&](int count, int from_next, int next) {
+    if (ONE && wave * 32 >= count) return;  // (a last turn: nothing follows)
+    const bool there = wave * 32 + li < count;
+    const int lim = shift + row - c * P;  // last key of the page that the row sees
+    q_rows_arrange<HD>(q, hh, D);
     if (q_sign != 0u) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[ks].w[i] ^= q_sign;
     }
-    int slot = 0;
-    {
-      const int4 *sel = reinterpret_cast<const int4 *>(p.sel + rowhead * p.topk4);
-      for (int i = 0; i < p.topk4; i += 8) {
-        const int4 s = sel[i >> 2], s2 = i + 4 < p.topk4 ? sel[(i >> 2) + 1] : s;
-        slot = s.x == c ? i : s.y == c ? i + 1 : s.z == c ? i + 2 : s.w == c ? i + 3 : s2.x == c ? i + 4 : s2.y == c ? i + 5 : s2.z == c ? i + 6 : s2.w == c ? i + 7 : slot;
-      }
-    }
+    int64_t at = 0;
+    if (!ONE) at = rowhead * p.topk4 + place();
     f32x16 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -482,7 +490,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
         __syncthreads();
       }
       for (int s0 = 0; s0 < (ONE ? 1 : held) && k0 + s0 < keys; s0 += KT) {
-        if (__ballot(there && lim >= k0 + s0) == 0ull) continue;
+        if (!ONE && __ballot(there && lim >= k0 + s0) == 0ull) continue;
         const uint32_t off = (uint32_t)(s0 * ROW);
         f32x16 s[ST];
 #pragma unroll
@@ -491,6 +499,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
           for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) s[t] = mfma32<T>(lds_read16(k_at[ks] + off + (uint32_t)(t * 32 * ROW)), q[ks], s[t]);
+        }
+        if (ONE) {
+          at = rowhead * p.topk4 + place();
+          if (next > 0) ask(from_next, next);
         }
         const int left = lim - k0 - s0;  // last visible key of this step
         float mx = -INFINITY;
@@ -534,7 +546,6 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
         l += sum_xor32_f(sum);
       }
     }
-    const int64_t at = rowhead * p.topk4 + slot;
     uint16_t *dst = p.part + at * D;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
@@ -607,8 +618,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     __syncthreads();
     const bool end = wb + kColumnWords >= w1;
     int from = 0;
-    while (count - from >= kColumnRows || (end && from < count)) {
-      turn(from, min(kColumnRows, count - from));
+    auto turn_at = [&](int f) { return count - f >= kColumnRows || end ? min(kColumnRows, count - f) : 0; };  // entries of the turn that begins there
+    if (ONE && turn_at(0) > 0) ask(0, turn_at(0));
+    for (int now = turn_at(0), then; now > 0; now = then) {
+      then = turn_at(from + kColumnRows);
+      if (!ONE) ask(from, now);
+      turn(now, from + kColumnRows, then);
       from += kColumnRows;
     }
     have = max(count - from, 0);
