@@ -355,11 +355,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
   const PairItem item = xcd_pair_item(blockIdx.x, a.batch * a.cache.heads_k, cols * p.parts);
   const int b = item.pair / a.cache.heads_k, hk = item.pair - b * a.cache.heads_k, c = item.idx / p.parts, part = item.idx - c * p.parts;
-  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
+  const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b], page = a.block_table[(int64_t)b * a.table_stride + c];  // (asked for together)
   const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q);
-  if (q0 < 0 || R <= 0 || (int64_t)c * P >= len) return;
-  const int page = a.block_table[(int64_t)b * a.table_stride + c];
-  if (page < 0 || page >= a.cache.num_pages) return;
+  if (q0 < 0 || R <= 0 || (int64_t)c * P >= len || page < 0 || page >= a.cache.num_pages) return;
   const int shift = len - (q1 - q0), G_tiles = (R + kTileRows - 1) / kTileRows * G;
   // the words of rows that can see the page, shared out evenly
   const int first = max(c * P - shift, 0) / kTileRows * G;
@@ -381,40 +379,46 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 
   const uint32_t k_base = (uint32_t)(uintptr_t)to_lds(column_smem), v_base = k_base + (uint32_t)(held * ROW);
   // keys [k0, k0 + held) of the page, widened; features past D and keys that are not there are zeros, and so are NaNs among the values (they count below)
-  auto stage = [&](int k0) {
-    constexpr int PIECES = HD / 16, AT_ONCE = 4;
-    for (int i0 = tid; i0 < held * PIECES; i0 += 256 * AT_ONCE) {
-      Pack8 kx[AT_ONCE], vx[AT_ONCE];
+  constexpr int PIECES = HD / 16, AT_ONCE = 4;  // 16-byte pieces of a row; of K and of V that a thread has on their way at a time (a page of one step: all of its)
+  Pack8 kx[AT_ONCE], vx[AT_ONCE];
+  auto stage_ask = [&](int k0, int i0) {
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = i0 + u * 256, r = i / PIECES, e = (i % PIECES) * 16;
-        const bool there = i < held * PIECES && k0 + r < keys && e < D;
-        kx[u] = there ? ld_global16(kg + (int64_t)(k0 + r) * a.cache.k_token_stride + e) : zero_pack8();
-        vx[u] = there ? ld_global16(vg + (int64_t)(k0 + r) * a.cache.v_token_stride + e) : zero_pack8();
-      }
-      bool nan = false;
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * 256, r = i / PIECES, e = (i % PIECES) * 16;
+      const bool there = i < held * PIECES && k0 + r < keys && e < D;
+      kx[u] = there ? ld_global16(kg + (int64_t)(k0 + r) * a.cache.k_token_stride + e) : zero_pack8();
+      vx[u] = there ? ld_global16(vg + (int64_t)(k0 + r) * a.cache.v_token_stride + e) : zero_pack8();
+    }
+  };
+  auto stage_put = [&](int i0) {
+    bool nan = false;
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        const int i = i0 + u * 256, r = i / PIECES, piece = (i % PIECES) * 2;
-        if (i >= held * PIECES) continue;
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * 256, r = i / PIECES, piece = (i % PIECES) * 2;
+      if (i >= held * PIECES) continue;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          u32x4_t ko, vo;
+      for (int half = 0; half < 2; ++half) {
+        u32x4_t ko, vo;
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t lo, hi, vw = vx[u].w[half * 2 + w];
-            H::template widen4<T>(kx[u].w[half * 2 + w], lo, hi);
-            ko[2 * w] = lo, ko[2 * w + 1] = hi;
-            if (H::any_nan4(vw)) nan = true, vw = H::without_nan4(vw);
-            H::template widen4<f16_t>(vw, lo, hi);
-            vo[2 * w] = lo, vo[2 * w + 1] = hi;
-          }
-          const uint32_t at = (uint32_t)(r * ROW + ((piece + half) ^ tile_swz<HD>(r)) * 16);
-          lds_write_vec(k_base + at, ko);
-          lds_write_vec(v_base + at, vo);
+        for (int w = 0; w < 2; ++w) {
+          uint32_t lo, hi, vw = vx[u].w[half * 2 + w];
+          H::template widen4<T>(kx[u].w[half * 2 + w], lo, hi);
+          ko[2 * w] = lo, ko[2 * w + 1] = hi;
+          if (H::any_nan4(vw)) nan = true, vw = H::without_nan4(vw);
+          H::template widen4<f16_t>(vw, lo, hi);
+          vo[2 * w] = lo, vo[2 * w + 1] = hi;
         }
+        const uint32_t at = (uint32_t)(r * ROW + ((piece + half) ^ tile_swz<HD>(r)) * 16);
+        lds_write_vec(k_base + at, ko);
+        lds_write_vec(v_base + at, vo);
       }
-      if (nan) sNan = 1;
+    }
+    if (nan) sNan = 1;
+  };
+  auto stage = [&](int k0) {
+    for (int i0 = tid; i0 < held * PIECES; i0 += 256 * AT_ONCE) {
+      stage_ask(k0, i0);
+      stage_put(i0);
     }
   };
   // where this lane's operands lie: of K row li, its pieces; of V four features of a row of four, and the row eight further down
@@ -590,9 +594,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
   };
 
-  if (ONE || held >= P) stage(0);
-  int have = 0;  // entries of the list that wait
-  for (int wb = w0; wb < w1; wb += kColumnWords) {
+  // the bits of kColumnWords words from wb on, spread out behind the `have` entries that the list has; returns how many it has then
+  auto spread = [&](int wb, int have) {
     uint32_t x = word;
     const int n = __popc(x);
     int upto = n;
@@ -616,24 +619,35 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
       x &= x - 1u;
     }
     __syncthreads();
+    return count;
+  };
+  if (!ONE && held >= P) stage(0);
+  if (ONE) stage_ask(0, tid);
+  int wb = w0, count = spread(w0, 0);
+  if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) ask(0, min(kColumnRows, count));
+  if (ONE) stage_put(tid);
+  __syncthreads();
+  while (true) {
     const bool end = wb + kColumnWords >= w1;
     int from = 0;
     auto turn_at = [&](int f) { return count - f >= kColumnRows || end ? min(kColumnRows, count - f) : 0; };  // entries of the turn that begins there
-    if (ONE && turn_at(0) > 0) ask(0, turn_at(0));
     for (int now = turn_at(0), then; now > 0; now = then) {
       then = turn_at(from + kColumnRows);
       if (!ONE) ask(from, now);
       turn(now, from + kColumnRows, then);
       from += kColumnRows;
     }
-    have = max(count - from, 0);
+    if (end) return;
+    const int have = max(count - from, 0);  // entries that wait
     __syncthreads();
     if (from > 0 && have > 0) {
       const uint16_t moved = tid < have ? sList[from + tid] : (uint16_t)0;
       __syncthreads();
       if (tid < have) sList[tid] = moved;
     }
-    __syncthreads();
+    wb += kColumnWords;
+    count = spread(wb, have);
+    if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) ask(0, min(kColumnRows, count));
   }
 }
 
