@@ -443,8 +443,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   // products with the keys are done (the registers of its queries are free then).
   Pack8 q[KS];
   int4 pages[2];
-  int row, g;
-  int64_t rowhead;
+  int row = 0, g = 0;
+  int64_t rowhead = (int64_t)q0 * a.heads + hk * G;
   auto ask = [&](int from, int count) {
     const int entry = sList[from + min(wave * 32 + li, count - 1)], w = w0 + (entry >> 5), rb = w / G;
     g = w - rb * G, row = rb * kTileRows + (entry & 31);
@@ -467,11 +467,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     for (int i = 8; i < p.topk4; i += 4) slot = among(sel[i >> 2], i, slot);
     return slot;
   };
-  // one turn: up to 128 entries of the list from `from` on, which were asked for; `next`: as many behind them follow
-  auto turn = [&](int count, int from_next, int next) {
-    if (ONE && wave * 32 >= count) return;  // (a last turn: nothing follows)
-    const bool there = wave * 32 + li < count;
-    const int lim = shift + row - c * P;  // last key of the page that the row sees
+  // What was asked for, taken over before anything is stored: a wait for loads is one for the stores in front of them too.
+  int64_t at_next = 0;
+  int lim_next = 0;
+  auto take_over = [&]() {
     q_rows_arrange<HD>(q, hh, D);
     if (q_sign != 0u) {
 #pragma unroll
@@ -479,8 +478,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[ks].w[i] ^= q_sign;
     }
-    int64_t at = 0;
-    if (!ONE) at = rowhead * p.topk4 + place();
+    at_next = rowhead * p.topk4 + place();
+    lim_next = shift + row - c * P;  // last key of the page that the row sees
+  };
+  // one turn: `count` entries of the list, which were asked for and taken over; then those of the next turn, `next` from `from_next` on
+  auto turn = [&](int count, int from_next, int next) {
+    if (ONE && wave * 32 >= count) return;  // (a last turn: nothing follows)
+    const bool there = wave * 32 + li < count;
+    const int lim = lim_next;
+    const int64_t at = at_next;
     f32x16 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -504,10 +510,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) s[t] = mfma32<T>(lds_read16(k_at[ks] + off + (uint32_t)(t * 32 * ROW)), q[ks], s[t]);
         }
-        if (ONE) {
-          at = rowhead * p.topk4 + place();
-          if (next > 0) ask(from_next, next);
-        }
+        if (ONE && next > 0) ask(from_next, next);
         const int left = lim - k0 - s0;  // last visible key of this step
         float mx = -INFINITY;
         if (__ballot(left < KT - 1) != 0ull) {
@@ -550,6 +553,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
         l += sum_xor32_f(sum);
       }
     }
+    if (ONE && next > 0) take_over();
     uint16_t *dst = p.part + at * D;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
@@ -625,7 +629,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   if (ONE) stage_ask(0, tid);
   int wb = w0, count = spread(w0, 0);
   if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) ask(0, min(kColumnRows, count));
-  if (ONE) stage_put(tid);
+  if (ONE) {
+    stage_put(tid);
+    take_over();  // (of nothing, if there is no turn yet)
+  }
   __syncthreads();
   while (true) {
     const bool end = wb + kColumnWords >= w1;
@@ -633,7 +640,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     auto turn_at = [&](int f) { return count - f >= kColumnRows || end ? min(kColumnRows, count - f) : 0; };  // entries of the turn that begins there
     for (int now = turn_at(0), then; now > 0; now = then) {
       then = turn_at(from + kColumnRows);
-      if (!ONE) ask(from, now);
+      if (!ONE) {
+        ask(from, now);
+        take_over();
+      }
       turn(now, from + kColumnRows, then);
       from += kColumnRows;
     }
@@ -647,7 +657,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
     wb += kColumnWords;
     count = spread(wb, have);
-    if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) ask(0, min(kColumnRows, count));
+    if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) {
+      ask(0, min(kColumnRows, count));
+      take_over();
+    }
   }
 }
 
