@@ -5,7 +5,7 @@
 //            A page is brought into LDS once for all of them, widened to 16 bits, exactly; its scales multiply scores and the result of a visit.
 //            Every visit leaves its output over the page and the logarithm of its sum.
 //   combine  adds a row's visits.
-// The weights of a visit are at most 1 and its output, in units of the page's scale, at most 448: both are kept in fp16, whatever the type of q (in bf16 each
+// The weights of a visit are at most 1 and its output, in units of the page's scale, at most 448 times their sum: both are kept in fp16, whatever the type of q (in bf16 each
 // would cost eight times its error; fp16 leaves 2^-12 of the output beside the 2^-9 of a bf16 one).
 #include "kv_attn.h"
 
@@ -21,8 +21,8 @@ struct ColumnPlan {
   int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
   uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
   float *scores;     // [block of 32 rows][head][32 rows][half of the wave][slot], where LDS does not hold them
-  float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum, scale of its page's values
-  uint16_t *part;    // [(row, head)][topk4][head_dim]: its output in units of that scale, fp16
+  float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum of weights, and what its output has to be multiplied by
+  uint16_t *part;    // [(row, head)][topk4][head_dim]: that output, fp16
   int32_t topk4;     // topk, rounded up to a multiple of four
   int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
   int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
@@ -555,8 +555,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
     if (ONE && next > 0) take_over();
     uint16_t *dst = p.part + at * D;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale);
+    // In one step of up to 128 keys the sums reach 128 * 448, which fp16 holds: they are divided by the weights' sum with the scale, else here.
+    const float inv = l == 0.f ? 0.f : 1.f / l, norm = ONE ? 1.f : inv;
+    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), ONE ? v_scale * inv : v_scale);
     {
       // Features 8 j + 4 hh .. of both halves to eight of one lane, then to four lanes with 64 bytes of a row, as the queries were loaded: stores of 16 bytes of 64
       // rows at a time take the caches a cycle for each.
@@ -568,7 +569,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) (j < 2 ? x : y)[(j & 1) * 2 + i] = pack2<f16_t>(o[d][4 * j + 2 * i] * inv, o[d][4 * j + 2 * i + 1] * inv);
+          for (int i = 0; i < 2; ++i) (j < 2 ? x : y)[(j & 1) * 2 + i] = pack2<f16_t>(o[d][4 * j + 2 * i] * norm, o[d][4 * j + 2 * i + 1] * norm);
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
