@@ -74,10 +74,27 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
 // One workgroup per (row, head): eight waves take the units of 64 keys of its pages side by side and merge in LDS.  16 bytes (features) a lane and load,
 // LPR lanes a key.
 // ------------------------------------------------------------------------------------
-constexpr int kRowWaves = 8, kUnitKeys = 64;
-constexpr int kOwnScores = 1024;  // candidates of a row that its workgroup scores itself, at most
-constexpr int kPickAlone = 256;  // candidates that one wave chooses from
+constexpr int kUnitKeys = 64;
+// Waves of a workgroup: eight, so that two of them share a compute unit; sixteen where there are not as many rows and heads as compute units.
+constexpr int kRowWaves = 8, kRowWavesFew = 16, kFewWorkgroups = 256;
+// Candidates of a row that its workgroup scores itself, at most.  Rows score for themselves what the heads of a group could share, from the L2, and spare a launch
+// between which everything waits: XX
+__host__ __device__ constexpr int own_limit(int waves) { return waves == kRowWavesFew ? 4096 : 1024; }
+constexpr int kPickAlone = 256;  // candidates that one wave chooses from (by the groups' cut 128 of them took 2 us longer)
+constexpr int kPickList = 512;  // candidates that are left when the cut of the groups is known, beyond which all are looked through again
 constexpr int kUnitsWithWeight = 1024;  // units of a row, at most: 64 pages of 1024 keys
+
+// the largest of N (8 or 16) consecutive lanes, in all of them
+template <int N>
+__device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));  // row_half_mirror
+  if constexpr (N == 16) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // row_mirror
+#endif
+  return x;
+}
 
 template <int LPR>
 __device__ __forceinline__ float sum_key_lanes(float x) {  // over the LPR consecutive lanes of a key
@@ -87,22 +104,26 @@ __device__ __forceinline__ float sum_key_lanes(float x) {  // over the LPR conse
 }
 
 // The scores of one row against its nc candidates by a whole workgroup: four lanes a page, 16 pages a wave, two of them in flight.
-template <typename T, int HD>
+template <typename T, int HD, int NW>
 __device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t, int h, int hk, int nc, const int32_t *table, uint32_t *key_hi, uint32_t *key_lo) {
-  constexpr int NP = HD / 32, TURN = kRowWaves * 16;
+  constexpr int NP = HD / 32, TURN = NW * 16;
   const int D = a.cache.head_dim, tid = threadIdx.x, part = tid & 3;
   const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)t * a.q_row_stride + (int64_t)h * a.q_head_stride + part * 8;
   Pack8 q[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) q[i] = i * 32 + part * 8 < D ? ld_global16(src + i * 32) : zero_pack8();
-  for (int c0 = 0; c0 < nc; c0 += 2 * TURN) {
-    int page[2];
-    Pack8 x[2][NP];
+  int page[2], page_next[2];
+  auto ask_pages = [&](int c0) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int c = c0 + u * TURN + (tid >> 2);
-      page[u] = c < nc ? table[c] : -1;
+      page_next[u] = c < nc ? table[c] : -1;
     }
+  };
+  ask_pages(0);
+  for (int c0 = 0; c0 < nc; c0 += 2 * TURN) {
+    Pack8 x[2][NP];
+    page[0] = page_next[0], page[1] = page_next[1];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const bool there = page[u] >= 0 && page[u] < a.cache.num_pages;
@@ -110,6 +131,7 @@ __device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t,
 #pragma unroll
       for (int i = 0; i < NP; ++i) x[u][i] = there && i * 32 + part * 8 < D ? ld_global16(mean + i * 32) : zero_pack8();
     }
+    ask_pages(c0 + 2 * TURN);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       double s = 0.0;
@@ -134,15 +156,15 @@ __device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t,
 }
 
 // SCORES: the workgroup scores its row's candidates itself, as cache_scores_kernel does, into LDS.
-template <typename T, typename H, int HD, bool WEIGHT, bool SCORES>
-__global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_row_kernel(CacheAttn p) {
+template <typename T, typename H, int HD, bool WEIGHT, bool SCORES, int NW>
+__global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kernel(CacheAttn p) {
   constexpr int LPR = HD / 16, KPI = 64 / LPR, NIN = kUnitKeys / KPI;
   const fmoba_cache_attn_args &a = p.a;
   __shared__ int sChosen[64], sCount, sPages[64];
   __shared__ float sScaleK[64], sScaleV[64];
-  __shared__ uint32_t sHi[kRowWaves * 64], sKeyHi[SCORES ? kOwnScores : 1], sKeyLo[SCORES ? kOwnScores : 1];
-  __shared__ int sPage[kRowWaves * 64];
-  __shared__ float sAcc[kRowWaves][HD], sM[kRowWaves], sL[kRowWaves];
+  __shared__ uint32_t sTop[64], sCut, sKeyHi[SCORES ? own_limit(NW) : 1], sKeyLo[SCORES ? own_limit(NW) : 1];
+  __shared__ int sPage[kPickList], sFound[NW];
+  __shared__ float sAcc[NW][HD], sM[NW], sL[NW];
   __shared__ float sUnitM[WEIGHT ? kUnitsWithWeight : 1], sUnitL[WEIGHT ? kUnitsWithWeight : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int t = blockIdx.x / a.heads, i = blockIdx.x - t * a.heads;
@@ -160,27 +182,74 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
   const int want = a.topk - 1;
   if constexpr (SCORES) {
     if (want > 0 && nc > 0) {
-      score_row<T, HD>(a, t, h, hk, nc, table, sKeyHi, sKeyLo);
+      score_row<T, HD, NW>(a, t, h, hk, nc, table, sKeyHi, sKeyLo);
       __syncthreads();
     }
   }
-  auto chosen = [&](int c, uint32_t, int i) { sChosen[i] = c; };
   int picked = 0;
-  if (nc <= kPickAlone) {
+  if (nc <= kPickAlone) {  // one wave, while the others ask for the query
     if (wave == 0)
-      picked = pick_best<kPickAlone / 64>(nc, want, lane, [&](int c) { return key_hi[c]; }, [&](int c) { return key_lo[c]; }, [](int c) { return c; }, chosen);
-  } else {  // the best of every eighth of the candidates, then the best of these
-    const int seg = ((nc + kRowWaves - 1) / kRowWaves + 63) / 64 * 64, c0 = wave * seg, n = min(seg, nc - c0);
-    auto hi = [&](int c) { return key_hi[c0 + c]; };
-    auto lo = [&](int c) { return key_lo[c0 + c]; };
-    auto id = [&](int c) { return c0 + c; };
-    auto take = [&](int c, uint32_t k, int i) { sHi[wave * 64 + i] = k, sPage[wave * 64 + i] = c0 + c; };
-    const int found = seg <= 256 ? pick_best<4>(n, want, lane, hi, lo, id, take) : seg <= 1024 ? pick_best<16>(n, want, lane, hi, lo, id, take) : pick_best<0>(n, want, lane, hi, lo, id, take);
-    for (int i = found + lane; i < 64; i += 64) sHi[wave * 64 + i] = 0u;
+      picked = pick_best<kPickAlone / 64>(nc, want, lane, [&](int c) { return key_hi[c]; }, [&](int c) { return key_lo[c]; }, [](int c) { return c; }, [&](int c, uint32_t, int at) { sChosen[at] = c; });
+  } else if (want > 0) {
+    // The candidates are 64 groups.  The want-th largest of the groups' largest keys is no larger than the want-th largest of all, so those at or above it are
+    // enough to choose from: a few more than are wanted.
+    uint32_t top = 0u;
+    for (int c = tid; c < nc; c += 64 * NW) top = max(top, key_hi[c]);
+    top = max_lanes<NW>(top);
+    if (lane % NW == 0) sTop[tid / NW] = top;
     __syncthreads();
-    if (wave == 0)
-      picked = pick_best<kRowWaves>(kRowWaves * 64, want, lane, [&](int i) { return sHi[i]; }, [&](int i) { return key_lo[sPage[i]]; }, [&](int i) { return sPage[i]; },
-                                    [&](int i, uint32_t, int at) { sChosen[at] = sPage[i]; });
+    if (wave == 0) {
+      const uint32_t mine = sTop[lane];
+      int at_least = 0;
+      for (int i = 0; i < 64; ++i) at_least += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) >= mine ? 1 : 0;
+      uint32_t cut = max(at_least >= want ? mine : 1u, 1u);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) cut = max(cut, (uint32_t)__shfl_xor((int)cut, o, 64));
+      if (lane == 0) sCut = cut;
+    }
+    __syncthreads();
+    const uint32_t cut = sCut;
+    int found = 0;
+    for (int c0 = wave * 64; c0 < nc; c0 += 64 * NW) found += __popcll(__ballot(c0 + lane < nc && key_hi[min(c0 + lane, nc - 1)] >= cut));
+    if (lane == 0) sFound[wave] = found;
+    __syncthreads();
+    int place = 0, m = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      place += w < wave ? sFound[w] : 0;
+      m += sFound[w];
+    }
+    for (int c0 = wave * 64; c0 < nc; c0 += 64 * NW) {
+      const int c = c0 + lane;
+      const bool in = c < nc && key_hi[min(c, nc - 1)] >= cut;
+      const unsigned long long mask = __ballot(in);
+      const int i = place + __popcll(mask & ((1ull << lane) - 1ull));
+      if (in && i < kPickList) sPage[i] = c;
+      place += __popcll(mask);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      if (m <= 64) {  // one a lane: its rank among them
+        const int c = lane < m ? sPage[lane] : 0;
+        const uint32_t hi = lane < m ? key_hi[c] : 0u, lo = key_lo[c];
+        int rank = 0;
+        for (int i = 0; i < m; ++i) {
+          const uint32_t h = (uint32_t)__builtin_amdgcn_readlane((int)hi, i), l = (uint32_t)__builtin_amdgcn_readlane((int)lo, i);
+          const int o = __builtin_amdgcn_readlane(c, i);
+          rank += h > hi || (h == hi && (l > lo || (l == lo && o > c))) ? 1 : 0;
+        }
+        const bool in = hi != 0u && rank < want;
+        if (in) sChosen[rank] = c;
+        picked = __popcll(__ballot(in));
+      } else if (m <= kPickList) {
+        picked = pick_best<kPickList / 64>(
+            m, want, lane, [&](int i) { return key_hi[sPage[i]]; }, [&](int i) { return key_lo[sPage[i]]; }, [&](int i) { return sPage[i]; },
+            [&](int i, uint32_t, int at) { sChosen[at] = sPage[i]; });
+      } else {
+        picked = pick_best<0>(
+            nc, want, lane, [&](int c) { return key_hi[c]; }, [&](int c) { return key_lo[c]; }, [](int c) { return c; }, [&](int c, uint32_t, int at) { sChosen[at] = c; });
+      }
+    }
   }
   if (wave == 0) {
     const int page = at.pos >= 0 && own < p.cols ? table[own] : -1;
@@ -214,7 +283,7 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
   float m = -INFINITY, l = 0.f, acc[16];  // l and acc: over this lane's keys (every KPI-th)
 #pragma unroll
   for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-  for (int u = wave; u < nunit; u += kRowWaves) {
+  for (int u = wave; u < nunit; u += NW) {
     const int n_page = u / upc, c = sChosen[n_page], in_page = (u - n_page * upc) * kUnitKeys;
     const int64_t page = sPages[n_page];
     if (c * P + in_page >= kend || page < 0) {
@@ -284,13 +353,14 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
   }
   if (lane == 0) sM[wave] = m, sL[wave] = l;
   __syncthreads();
+  if (wave * 64 >= max(HD, WEIGHT ? nunit : 0)) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) M = fmaxf(M, sM[w]);
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, sM[w]);
   const float Mref = M == -INFINITY ? 0.f : M;
   float L = 0.f, o = 0.f;
 #pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float f = __builtin_amdgcn_exp2f(sM[w] - Mref);
     L = fmaf(f, sL[w], L);
     if (tid < HD) o = fmaf(f, sAcc[w][tid], o);
@@ -299,7 +369,7 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
   if (tid < D) out[tid] = float_to_elem_bits<T>(empty ? 0.f : o / L);
   if (tid == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (M + __builtin_amdgcn_logf(L)) * 0.6931471805599453f;
   if constexpr (WEIGHT) {
-    for (int u = tid; u < nunit; u += 64 * kRowWaves) {
+    for (int u = tid; u < nunit; u += 64 * NW) {
       const float part = __builtin_amdgcn_exp2f(sUnitM[u] - Mref) * sUnitL[u] / L;  // (a unit past the row: 0)
       if (part > 0.f) atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)sPages[u / upc] * a.cache.heads_k + hk, (unsigned long long)rintf(part * 4294967296.f));
     }
@@ -309,25 +379,24 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
 static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
 // whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own
 static bool many_rows(const fmoba_cache_attn_args &a, int cols) { return cols > 0 && a.max_seqlen_q > kRowFormRows; }
-// whether the rows' workgroups score their pages themselves
-static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= kOwnScores; }
-
-template <typename T, typename H, bool WEIGHT, bool SCORES>
-static void launch_rows(const CacheAttn &p, hipStream_t s) {
-  const dim3 grid((uint32_t)p.a.total_q * p.a.heads), block(64 * kRowWaves);
-  if (p.a.cache.head_dim <= 64)
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 64, WEIGHT, SCORES>), grid, block, 0, s, p);
-  else if (p.a.cache.head_dim <= 128)
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 128, WEIGHT, SCORES>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((cache_attn_row_kernel<T, H, 256, WEIGHT, SCORES>), grid, block, 0, s, p);
+static int row_waves(const fmoba_cache_attn_args &a) {
+  return a.cache.head_dim <= 128 && (int64_t)a.total_q * a.heads <= kFewWorkgroups && cache_cols(a) - 1 <= own_limit(kRowWavesFew) ? kRowWavesFew : kRowWaves;
 }
-template <typename T, typename H>
-static void launch_rows_as(const CacheAttn &p, bool scores, hipStream_t s) {
-  if (p.a.add_weight)
-    scores ? launch_rows<T, H, true, true>(p, s) : launch_rows<T, H, true, false>(p, s);
-  else
-    scores ? launch_rows<T, H, false, true>(p, s) : launch_rows<T, H, false, false>(p, s);
+// whether the rows' workgroups score their pages themselves
+static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= own_limit(row_waves(a)); }
+
+template <typename T, typename H, bool WEIGHT>
+static void launch_rows(const CacheAttn &p, hipStream_t s) {
+  const int D = p.a.cache.head_dim, waves = row_waves(p.a);
+  const bool own = own_scores(p.a);
+  auto kern = D <= 64    ? (waves == kRowWavesFew ? cache_attn_row_kernel<T, H, 64, WEIGHT, true, kRowWavesFew>
+                            : own                 ? cache_attn_row_kernel<T, H, 64, WEIGHT, true, kRowWaves>
+                                                  : cache_attn_row_kernel<T, H, 64, WEIGHT, false, kRowWaves>)
+              : D <= 128 ? (waves == kRowWavesFew ? cache_attn_row_kernel<T, H, 128, WEIGHT, true, kRowWavesFew>
+                            : own                 ? cache_attn_row_kernel<T, H, 128, WEIGHT, true, kRowWaves>
+                                                  : cache_attn_row_kernel<T, H, 128, WEIGHT, false, kRowWaves>)
+                         : (own ? cache_attn_row_kernel<T, H, 256, WEIGHT, true, kRowWaves> : cache_attn_row_kernel<T, H, 256, WEIGHT, false, kRowWaves>);
+  hipLaunchKernelGGL(kern, dim3((uint32_t)p.a.total_q * p.a.heads), dim3(64 * waves), 0, s, p);
 }
 
 template <typename T, int HD>
@@ -348,15 +417,14 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
   if (many_rows(a, p.cols)) return run_cache_columns(p, s);
-  const bool own = own_scores(a);
-  if (!own && p.cols > 1 && a.topk > 1) {
+  if (!own_scores(a) && p.cols > 1 && a.topk > 1) {
     if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
     FMOBA_LAUNCH_CHECK("cache_scores_kernel");
   }
   if (a.cache.format == FMOBA_CACHE_E4M3)
-    launch_rows_as<T, HeldE4M3>(p, own, s);
+    a.add_weight ? launch_rows<T, HeldE4M3, true>(p, s) : launch_rows<T, HeldE4M3, false>(p, s);
   else
-    launch_rows_as<T, HeldInt8>(p, own, s);
+    a.add_weight ? launch_rows<T, HeldInt8, true>(p, s) : launch_rows<T, HeldInt8, false>(p, s);
   FMOBA_LAUNCH_CHECK("cache_attn_row_kernel");
   return 0;
 }
