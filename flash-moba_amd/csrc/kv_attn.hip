@@ -96,11 +96,36 @@ __device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
   return x;
 }
 
-template <int LPR>
-__device__ __forceinline__ float sum_key_lanes(float x) {  // over the LPR consecutive lanes of a key
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) x += __shfl_xor(x, o, 64);
+// lane permutations on the vector unit: CTRL of update_dpp
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+#else
   return x;
+#endif
+}
+// sum over the LPR (4, 8 or 16) consecutive lanes of a key, in all of them
+template <int LPR>
+__device__ __forceinline__ float sum_key_lanes(float x) {
+  x += dpp_f<0xb1>(x);   // quad_perm 1 0 3 2
+  x += dpp_f<0x4e>(x);   // quad_perm 2 3 0 1
+  if constexpr (LPR >= 8) x += dpp_f<0x141>(x);   // row_half_mirror
+  if constexpr (LPR >= 16) x += dpp_f<0x140>(x);  // row_mirror
+  return x;
+}
+// sum and maximum over the lanes of equal features: every LPR-th
+template <int LPR>
+__device__ __forceinline__ float sum_keys(float x) {
+  if constexpr (LPR == 4) x += dpp_f<0x124>(x);  // row_ror 4
+  if constexpr (LPR <= 8) x += dpp_f<0x128>(x);  // row_ror 8
+  return sum_rows4_f(x);
+}
+template <int LPR>
+__device__ __forceinline__ float max_keys(float x) {
+  if constexpr (LPR == 4) x = fmaxf(x, dpp_f<0x124>(x));
+  if constexpr (LPR <= 8) x = fmaxf(x, dpp_f<0x128>(x));
+  return max_rows4_f(x);
 }
 
 // The scores of one row against its nc candidates by a whole workgroup: four lanes a page, 16 pages a wave, two of them in flight.
@@ -314,8 +339,7 @@ __global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kern
       s[n] = r0 + n * KPI <= last ? d : -INFINITY;
       mu = fmaxf(mu, s[n]);
     }
-#pragma unroll
-    for (int o = LPR; o < 64; o <<= 1) mu = fmaxf(mu, __shfl_xor(mu, o, 64));
+    mu = max_keys<LPR>(mu);
     const float mn = fmaxf(m, mu), mref = mn == -INFINITY ? 0.f : mn;
     const float resc = __builtin_amdgcn_exp2f(m - mref);
     m = mn;
@@ -336,17 +360,13 @@ __global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kern
     }
     l = fmaf(l, resc, lu);
     if constexpr (WEIGHT) {
-#pragma unroll
-      for (int o = LPR; o < 64; o <<= 1) lu += __shfl_xor(lu, o, 64);
+      lu = sum_keys<LPR>(lu);
       if (lane == 0) sUnitM[u] = mref, sUnitL[u] = lu;
     }
   }
+  l = sum_keys<LPR>(l);
 #pragma unroll
-  for (int o = LPR; o < 64; o <<= 1) {
-    l += __shfl_xor(l, o, 64);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
-  }
+  for (int j = 0; j < 16; ++j) acc[j] = sum_keys<LPR>(acc[j]);
   if (lane < LPR) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) sAcc[wave][e + j] = acc[j];
