@@ -100,7 +100,7 @@ def test_refusals(change, message):
 def test_the_entry_point_refuses_without_a_gpu():
     lib = H.load_library()
     assert lib.fmoba_cache_evict(None, None) != 0
-    assert lib.fmoba_cache_evict_workspace_bytes(4, 8192) == 0 and lib.fmoba_cache_evict_workspace_bytes(4, 8193) == 4 * 8193 * 8
+    assert lib.fmoba_cache_evict_workspace_bytes(4, 1024) == 0 and lib.fmoba_cache_evict_workspace_bytes(4, 1025) == 4 * 1025 * 8
 
     def args(**kw):
         a = H.CacheEvictArgs()
