@@ -7,7 +7,7 @@ namespace fmoba {
 
 // E4M3 and INT8 as types for templates.
 //   unpack4: four values of a 32-bit word in units of their scale, exact in 32 bits
-//   pack4:   four values in units of their scale, rounded to nearest (ties to even), cut off at the largest
+//   pack4:   four values in units of their scale, rounded to nearest (ties to even), cut off at the largest; int8 holds a NaN as 0.  SURE: no NaN among them
 struct HeldE4M3 {
   static constexpr int kFormat = FMOBA_CACHE_E4M3;
   static __device__ __forceinline__ void unpack4(uint32_t w, float (&f)[4]) {
@@ -42,11 +42,20 @@ struct HeldE4M3 {
     const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;  // 1 in the bytes that are
     return w & ~(nan * 255u);
   }
-  static __device__ __forceinline__ float limit(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
+  template <bool SURE>
+  static __device__ __forceinline__ float limit(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float y = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
+    return !SURE && x != x ? x : y;
+#else
+    return x;
+#endif
+  }
+  template <bool SURE = false>
   static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(limit(a), limit(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(limit(c), limit(d), w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(limit<SURE>(a), limit<SURE>(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(limit<SURE>(c), limit<SURE>(d), w, true);
 #else
     (void)a, (void)b, (void)c, (void)d;
     return 0;
@@ -70,8 +79,25 @@ struct HeldInt8 {
   }
   static __device__ __forceinline__ bool any_nan4(uint32_t) { return false; }
   static __device__ __forceinline__ uint32_t without_nan4(uint32_t w) { return w; }
-  static __device__ __forceinline__ uint32_t pack1(float x) { return (uint32_t)(int)(x != x ? 0.f : rintf(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu; }
-  static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack1(a) | pack1(b) << 8 | pack1(c) << 16 | pack1(d) << 24; }
+  // 1.5 * 2^23 + x, |x| <= 127: the sum's unit is 1, so it is rounded to a whole number, whose low byte is x's
+  template <bool SURE>
+  static __device__ __forceinline__ uint32_t pack1(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const float y = __builtin_amdgcn_fmed3f(x, -127.f, 127.f);
+    return __float_as_uint((!SURE && x != x ? 0.f : y) + 12582912.f);
+#else
+    return (void)x, 0;
+#endif
+  }
+  template <bool SURE = false>
+  static __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t lo = __builtin_amdgcn_perm(pack1<SURE>(b), pack1<SURE>(a), 0x0c0c0400u), hi = __builtin_amdgcn_perm(pack1<SURE>(d), pack1<SURE>(c), 0x04000c0cu);
+    return lo | hi;
+#else
+    return (void)a, (void)b, (void)c, (void)d, 0;
+#endif
+  }
   // 127 = 1.984375 * 2^6
   static __device__ __forceinline__ int scale_exponent(float m, int x) { return x - 6 + (m > 1.984375f ? 1 : 0); }
 };
