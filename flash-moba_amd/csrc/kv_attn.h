@@ -120,7 +120,6 @@ __device__ __forceinline__ int pick_best(int n, int want, int lane, Hi hi, Lo lo
   return total;
 }
 
-constexpr int kRowFormRows = 8;  // rows of a sequence that are taken one by one
 // the form for many rows
 size_t column_workspace_bytes(const fmoba_cache_attn_args &a, int cols);
 int run_cache_columns(const CacheAttn &c, hipStream_t s);

@@ -10,23 +10,22 @@
 namespace fmoba {
 
 // ------------------------------------------------------------------------------------
-// Scores of NR (row, head of the group) pairs against 64 pages: four lanes share a page's mean, a quarter of the features each.  The pairs' queries
+// Scores of up to eight (row, head of the group) pairs against 64 pages: four lanes share a page's mean, a quarter of the features each.  The pairs' queries
 // lie in LDS as doubles.  A decode step reads every mean once and is bound by latency: the lengths, then the queries and the table, then the means, each once
-// and all of a lane's loads together (with the means asked for one after the other 13 us instead of XX, 16 requests with 512 to 32768 tokens, 8 key
-// heads of 128, 128-key pages).  Many rows are bound by the 64-bit products.
+// and all of a lane's loads together.  Many rows are bound by the 64-bit products.
 // ------------------------------------------------------------------------------------
-constexpr int kScorePages = 64;
-template <typename T, int HD, int NR>
+constexpr int kScorePages = 64, kScorePairs = 8;
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
-  __shared__ double sQ[NR * HD];
+  __shared__ double sQ[kScorePairs * HD];
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, tid = threadIdx.x;
   const int b = blockIdx.z / a.cache.heads_k, hk = blockIdx.z - b * a.cache.heads_k;
   const int c = blockIdx.x * kScorePages + (tid >> 2), part = tid & 3;
   const int page = c < p.cols - 1 ? a.block_table[(int64_t)b * a.table_stride + c] : -1;
   const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
-  const int R = min(q1, a.total_q) - q0, pair0 = blockIdx.y * NR;
-  const int npairs = (int)min((int64_t)NR, (int64_t)R * G - pair0);
+  const int R = min(q1, a.total_q) - q0, pair0 = blockIdx.y * kScorePairs;
+  const int npairs = (int)min((int64_t)kScorePairs, (int64_t)R * G - pair0);
   if (q0 < 0 || npairs <= 0) return;
   const int last_pos = len - (q1 - q0) + (pair0 + npairs - 1) / G;  // pairs: row by row, a row's heads one after the other
   const int npages = last_pos < 0 ? 0 : min(last_pos / P, p.cols - 1);  // that any of the rows can select beside its own
@@ -37,35 +36,38 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
   Pack8 x[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i) x[i] = there && i * 32 + part * 8 < D ? ld_global16(mean + i * 32 + part * 8) : zero_pack8();
-  for (int i = tid; i < NR * HD; i += 256) {
-    const int r = i / HD, e = i % HD, pair = pair0 + min(r, npairs - 1);
+  for (int i = tid; i < npairs * HD; i += 256) {
+    const int r = i / HD, e = i % HD, pair = pair0 + r;
     const int row = q0 + pair / G, h = hk * G + pair % G;
     sQ[i] = e < D ? (double)elem_to_float<T>(reinterpret_cast<const uint16_t *>(a.q)[(int64_t)row * a.q_row_stride + (int64_t)h * a.q_head_stride + e]) : 0.0;
   }
   __syncthreads();
-  double acc[NR];
+  constexpr int RC = HD > 128 ? 1 : 2;  // pairs at a time: all of them read ahead do not fit the registers
+#pragma unroll 1
+  for (int r0 = 0; r0 < npairs; r0 += RC) {
+    double s[RC];
 #pragma unroll
-  for (int r = 0; r < NR; ++r) acc[r] = 0.0;
+    for (int r = 0; r < RC; ++r) s[r] = 0.0;
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    float f[8];
-    unpack8<T>(x[i], f);
+    for (int i = 0; i < NP; ++i) {
+      float f[8];
+      unpack8<T>(x[i], f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int r = 0; r < NR; ++r) acc[r] = fma((double)f[j], sQ[r * HD + i * 32 + part * 8 + j], acc[r]);
-  }
+        for (int r = 0; r < RC; ++r) s[r] = fma((double)f[j], sQ[min(r0 + r, npairs - 1) * HD + i * 32 + part * 8 + j], s[r]);
+    }
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    double s = acc[r];
-    s += __shfl_xor(s, 1, 64);
-    s += __shfl_xor(s, 2, 64);
-    if (part == 0 && c < npages && r < npairs) {
-      const int pair = pair0 + r;
-      const int64_t at = ((int64_t)(q0 + pair / G) * a.heads + hk * G + pair % G) * p.cols + c;
-      const uint64_t key = there ? score_key(s) : 0ull;
-      p.key_hi[at] = (uint32_t)(key >> 32);
-      p.key_lo[at] = (uint32_t)key;
+    for (int r = 0; r < RC; ++r) {
+      s[r] += __shfl_xor(s[r], 1, 64);
+      s[r] += __shfl_xor(s[r], 2, 64);
+      if (part == 0 && c < npages && r0 + r < npairs) {
+        const int pair = pair0 + r0 + r;
+        const int64_t at = ((int64_t)(q0 + pair / G) * a.heads + hk * G + pair % G) * p.cols + c;
+        const uint64_t key = there ? score_key(s[r]) : 0ull;
+        p.key_hi[at] = (uint32_t)(key >> 32);
+        p.key_lo[at] = (uint32_t)key;
+      }
     }
   }
 }
@@ -75,23 +77,29 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
 // LPR lanes a key.
 // ------------------------------------------------------------------------------------
 constexpr int kUnitKeys = 64;
-// Waves of a workgroup: eight, so that two of them share a compute unit; sixteen where there are not as many rows and heads as compute units.
-constexpr int kRowWaves = 8, kRowWavesFew = 16, kFewWorkgroups = 256;
+constexpr int kRowWaves = 8;  // of a workgroup: two of them share a compute unit
+static_assert(kRowWaves == 8, "64 groups of candidates: eight threads each");
 // Candidates of a row that its workgroup scores itself, at most.  Rows score for themselves what the heads of a group could share, from the L2, and spare a launch
-// between which everything waits: XX
-__host__ __device__ constexpr int own_limit(int waves) { return waves == kRowWavesFew ? 4096 : 1024; }
+// that everything waits for: one row of each of 16 sequences, 32 over 8 heads, 1024 pages 33.5 instead of 44.0 us, of one 18.7 and 18.8; 2048 pages, 16 heads of 64, 16
+// sequences 30.2 and 42.3, four 25.3 and 25.1, one 21.8 and 19.2.
+constexpr int kOwnScores = 2048;
+// Rows share pages where there are kColumnRowsLeast (row, head) pairs or more and a page is selected by kVisitsOwn of them on average, or by kVisits if the scores are a
+// launch of their own; else the form for many rows takes longer, for its three launches and for pages that few rows visit.  Visits of a page, us of the form for many rows and of this
+// one, heads of 128, 8 pages a row: 16 sequences of 2048 tokens, 16 heads, 4 rows each 2: 91, 34; 8 rows 4: 93, 62; 16 rows 8: 94, 117; of 32768 tokens, 32 over 8
+// heads, 32 rows 4: 551, 513; of 8192 8 rows 4: 160, 122; 16 rows 8: 165, 233; a sequence of 100000 tokens 64 rows 2.6: 140, 103; 128 rows 5.2: 150, 191; 256 rows 10: 156, 364;
+// with its own launch for the scores, four sequences of 300000, 32 rows 0.4: 1007, 391; 128 rows 1.7: 1293, 1465.  Few pairs, 1536: 16 over 2 heads, 262 visits: 56, 49; 1024, 32
+// over 8 heads, 64: 30, 34; 2048, 16 heads, 16: 46, 61.
+constexpr int kColumnRowsLeast = 2048, kVisitsOwn = 5, kVisits = 2;
 constexpr int kPickAlone = 256;  // candidates that one wave chooses from (by the groups' cut 128 of them took 2 us longer)
 constexpr int kPickList = 512;  // candidates that are left when the cut of the groups is known, beyond which all are looked through again
 constexpr int kUnitsWithWeight = 1024;  // units of a row, at most: 64 pages of 1024 keys
 
-// the largest of N (8 or 16) consecutive lanes, in all of them
-template <int N>
-__device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
+// the largest of 8 consecutive lanes, in all of them
+__device__ __forceinline__ uint32_t max_lanes8(uint32_t x) {
 #if defined(__HIP_DEVICE_COMPILE__)
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true));   // quad_perm 2 3 0 1
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));  // row_half_mirror
-  if constexpr (N == 16) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // row_mirror
 #endif
   return x;
 }
@@ -129,9 +137,9 @@ __device__ __forceinline__ float max_keys(float x) {
 }
 
 // The scores of one row against its nc candidates by a whole workgroup: four lanes a page, 16 pages a wave, two of them in flight.
-template <typename T, int HD, int NW>
+template <typename T, int HD>
 __device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t, int h, int hk, int nc, const int32_t *table, uint32_t *key_hi, uint32_t *key_lo) {
-  constexpr int NP = HD / 32, TURN = NW * 16;
+  constexpr int NP = HD / 32, TURN = kRowWaves * 16;
   const int D = a.cache.head_dim, tid = threadIdx.x, part = tid & 3;
   const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)t * a.q_row_stride + (int64_t)h * a.q_head_stride + part * 8;
   Pack8 q[NP];
@@ -181,13 +189,13 @@ __device__ __forceinline__ void score_row(const fmoba_cache_attn_args &a, int t,
 }
 
 // SCORES: the workgroup scores its row's candidates itself, as cache_scores_kernel does, into LDS.
-template <typename T, typename H, int HD, bool WEIGHT, bool SCORES, int NW>
-__global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kernel(CacheAttn p) {
-  constexpr int LPR = HD / 16, KPI = 64 / LPR, NIN = kUnitKeys / KPI;
+template <typename T, typename H, int HD, bool WEIGHT, bool SCORES>
+__global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_row_kernel(CacheAttn p) {
+  constexpr int LPR = HD / 16, KPI = 64 / LPR, NW = kRowWaves, NIN = kUnitKeys / KPI;
   const fmoba_cache_attn_args &a = p.a;
   __shared__ int sChosen[64], sCount, sPages[64];
   __shared__ float sScaleK[64], sScaleV[64];
-  __shared__ uint32_t sTop[64], sCut, sKeyHi[SCORES ? own_limit(NW) : 1], sKeyLo[SCORES ? own_limit(NW) : 1];
+  __shared__ uint32_t sTop[64], sCut, sKeyHi[SCORES ? kOwnScores : 1], sKeyLo[SCORES ? kOwnScores : 1];
   __shared__ int sPage[kPickList], sFound[NW];
   __shared__ float sAcc[NW][HD], sM[NW], sL[NW];
   __shared__ float sUnitM[WEIGHT ? kUnitsWithWeight : 1], sUnitL[WEIGHT ? kUnitsWithWeight : 1];
@@ -207,7 +215,7 @@ __global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kern
   const int want = a.topk - 1;
   if constexpr (SCORES) {
     if (want > 0 && nc > 0) {
-      score_row<T, HD, NW>(a, t, h, hk, nc, table, sKeyHi, sKeyLo);
+      score_row<T, HD>(a, t, h, hk, nc, table, sKeyHi, sKeyLo);
       __syncthreads();
     }
   }
@@ -220,8 +228,8 @@ __global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kern
     // enough to choose from: a few more than are wanted.
     uint32_t top = 0u;
     for (int c = tid; c < nc; c += 64 * NW) top = max(top, key_hi[c]);
-    top = max_lanes<NW>(top);
-    if (lane % NW == 0) sTop[tid / NW] = top;
+    top = max_lanes8(top);
+    if (lane % 8 == 0) sTop[tid / 8] = top;
     __syncthreads();
     if (wave == 0) {
       const uint32_t mine = sTop[lane];
@@ -397,38 +405,32 @@ __global__ __launch_bounds__(64 * NW, HD > 128 ? 2 : 4) void cache_attn_row_kern
 }
 
 static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
-// whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own
-static bool many_rows(const fmoba_cache_attn_args &a, int cols) { return cols > 0 && a.max_seqlen_q > kRowFormRows; }
-static int row_waves(const fmoba_cache_attn_args &a) {
-  return a.cache.head_dim <= 128 && (int64_t)a.total_q * a.heads <= kFewWorkgroups && cache_cols(a) - 1 <= own_limit(kRowWavesFew) ? kRowWavesFew : kRowWaves;
-}
 // whether the rows' workgroups score their pages themselves
-static bool own_scores(const fmoba_cache_attn_args &a) { return cache_cols(a) - 1 <= own_limit(row_waves(a)); }
+static bool own_scores(int cols) { return cols - 1 <= kOwnScores; }
+// Whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own.
+static bool many_rows(const fmoba_cache_attn_args &a, int cols) {
+  const int64_t rows = (int64_t)a.total_q * a.heads;
+  return cols > 0 && rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
+}
 
 template <typename T, typename H, bool WEIGHT>
 static void launch_rows(const CacheAttn &p, hipStream_t s) {
-  const int D = p.a.cache.head_dim, waves = row_waves(p.a);
-  const bool own = own_scores(p.a);
-  auto kern = D <= 64    ? (waves == kRowWavesFew ? cache_attn_row_kernel<T, H, 64, WEIGHT, true, kRowWavesFew>
-                            : own                 ? cache_attn_row_kernel<T, H, 64, WEIGHT, true, kRowWaves>
-                                                  : cache_attn_row_kernel<T, H, 64, WEIGHT, false, kRowWaves>)
-              : D <= 128 ? (waves == kRowWavesFew ? cache_attn_row_kernel<T, H, 128, WEIGHT, true, kRowWavesFew>
-                            : own                 ? cache_attn_row_kernel<T, H, 128, WEIGHT, true, kRowWaves>
-                                                  : cache_attn_row_kernel<T, H, 128, WEIGHT, false, kRowWaves>)
-                         : (own ? cache_attn_row_kernel<T, H, 256, WEIGHT, true, kRowWaves> : cache_attn_row_kernel<T, H, 256, WEIGHT, false, kRowWaves>);
-  hipLaunchKernelGGL(kern, dim3((uint32_t)p.a.total_q * p.a.heads), dim3(64 * waves), 0, s, p);
+  const int D = p.a.cache.head_dim;
+  const bool own = own_scores(p.cols);
+  auto kern = D <= 64    ? (own ? cache_attn_row_kernel<T, H, 64, WEIGHT, true> : cache_attn_row_kernel<T, H, 64, WEIGHT, false>)
+              : D <= 128 ? (own ? cache_attn_row_kernel<T, H, 128, WEIGHT, true> : cache_attn_row_kernel<T, H, 128, WEIGHT, false>)
+                         : (own ? cache_attn_row_kernel<T, H, 256, WEIGHT, true> : cache_attn_row_kernel<T, H, 256, WEIGHT, false>);
+  hipLaunchKernelGGL(kern, dim3((uint32_t)p.a.total_q * p.a.heads), dim3(64 * kRowWaves), 0, s, p);
 }
 
 template <typename T, int HD>
 static int launch_scores(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int64_t pairs = (int64_t)a.max_seqlen_q * (a.heads / a.cache.heads_k);
-  const int nr = pairs <= 1 ? 1 : pairs <= 2 ? 2 : pairs <= 4 ? 4 : 8;
-  const int64_t turns = ceil_div64(pairs, nr), z = (int64_t)a.batch * a.cache.heads_k;
+  const int64_t turns = ceil_div64(pairs, kScorePairs), z = (int64_t)a.batch * a.cache.heads_k;
   FMOBA_REQUIRE(turns <= 65535 && z <= 65535, "cache_attn: too many rows, or sequences times heads, for the launch grid");
   const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)turns, (uint32_t)z);
-  auto kern = nr == 1 ? cache_scores_kernel<T, HD, 1> : nr == 2 ? cache_scores_kernel<T, HD, 2> : nr == 4 ? cache_scores_kernel<T, HD, 4> : cache_scores_kernel<T, HD, 8>;
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p);
+  hipLaunchKernelGGL((cache_scores_kernel<T, HD>), grid, dim3(256), 0, s, p);
   return 0;
 }
 
@@ -437,7 +439,7 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
   if (many_rows(a, p.cols)) return run_cache_columns(p, s);
-  if (!own_scores(a) && p.cols > 1 && a.topk > 1) {
+  if (!own_scores(p.cols) && p.cols > 1 && a.topk > 1) {
     if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
     FMOBA_LAUNCH_CHECK("cache_scores_kernel");
   }
@@ -457,7 +459,7 @@ extern "C" size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *
   const int cols = a->cache.num_pages > 0 ? cache_cols(*a) : 0;
   if (cols == 0) return 0;
   if (many_rows(*a, cols)) return column_workspace_bytes(*a, cols);
-  return own_scores(*a) ? 0 : (size_t)a->total_q * a->heads * cache_cols(*a) * 8;
+  return own_scores(cols) ? 0 : (size_t)a->total_q * a->heads * cols * 8;
 }
 
 extern "C" int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream) {

@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRo
 // gate: a workgroup takes 32 rows of a head, its waves a quarter of the pages each.  Scores^T = means q^T, so that a lane has half of a row's scores (the other half of the wave the others), 16 of a
 // product's 32 pages.  A score gives its lowest bits up for the page's number; eight groups of a lane's scores are known by their largest, and the best
 // are taken off one by one: the largest of eight, whose group is then looked through again.  About 60 instructions for one page of 32 rows, where counting
-// scores above a cut (a ballot per 64 scores and bit) takes 30 for one bit of one row: XX instead of 142 us, 8191 tokens, 16 heads, 64 pages.
+// scores above a cut (a ballot per 64 scores and bit) takes 30 for one bit of one row: 29 instead of 142 us, 8191 tokens, 16 heads, 64 pages.
 // ------------------------------------------------------------------------------------
 constexpr int kGateCols = 1024;   // pages whose scores of 32 rows LDS holds (135 KB); beyond, in the workspace
 constexpr int kGateGroups = 8;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   const int shift = len - (q1 - q0), G_tiles = (R + kTileRows - 1) / kTileRows * G;
   // the words of rows that can see the page, shared out evenly
   const int first = max(c * P - shift, 0) / kTileRows * G;
-  const int each = ((G_tiles - first + p.parts - 1) / p.parts + 31) / 32 * 32;
+  const int each = ((G_tiles - first + p.parts - 1) / p.parts + 7) / 8 * 8;
   const int w0 = first + part * each, w1 = min(w0 + each, G_tiles);
   if (w0 >= w1) return;
   const int keys = min(P, len - c * P);  // of the page that are there
@@ -872,7 +872,7 @@ static int run_columns_as(const ColumnPlan &p, hipStream_t s) {
 
 int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   const fmoba_cache_attn_args &a = c.a;
-  FMOBA_REQUIRE(c.cols <= kColumnCols, "cache_attn: %d pages per sequence; at most %d are supported for more than %d rows of a sequence", c.cols, kColumnCols, kRowFormRows);
+  FMOBA_REQUIRE(c.cols <= kColumnCols, "cache_attn: %d pages per sequence; at most %d are supported for that many rows", c.cols, kColumnCols);
   ColumnPlan p{};
   p.c = c;
   const ColumnSizes z = column_sizes(a, c.cols, p);
@@ -882,9 +882,11 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   p.scores = reinterpret_cast<float *>(at), at += z.scores;
   p.head = reinterpret_cast<float2 *>(at), at += z.head;
   p.part = reinterpret_cast<uint16_t *>(at);
-  // workgroups of a page: three turns of rows each, if rows choose evenly
+  // Workgroups of a page: four turns of rows each, if rows choose evenly, and an odd number: the last ones of a late page, which few rows see, have nothing to
+  // do, and would otherwise come to the same shader engines for every page (8191 tokens, 16 heads: 223 us even, 201 odd; 8192, 16 over 2 heads: 380 and 254;
+  // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
   const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
-  p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (3 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32));
+  p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 

@@ -1,4 +1,5 @@
 """The paged 8-bit cache in 64 bits on the CPU, written from its definition: a dict of tensors like MobaKVCache's fields, and what the functions do to it."""
+import itertools
 import math
 
 import torch
@@ -75,32 +76,40 @@ def attention(s, q, cu, seqlens_k, table, topk, scale=None):
     size, dot, most, count = torch.zeros_like(out), torch.zeros((heads, q.shape[0])).double(), torch.zeros((heads, q.shape[0])).double(), torch.zeros((heads, q.shape[0])).double()
     weight = torch.zeros(s["k_scale"].shape, dtype=torch.float64)
     for b in range(len(seqlens_k)):
-        for i in range(cu[b], cu[b + 1]):
-            pos = seqlens_k[b] - (cu[b + 1] - i)
-            if pos < 0:
+        n = min(-(-max(seqlens_k[b], 0) // P), len(table[b]))
+        if n == 0:
+            continue
+        pages = torch.tensor(table[b][:n])
+        there = (pages >= 0) & (pages < s["k"].shape[0])
+        pages = pages.where(there, torch.zeros_like(pages))
+        for h, i0 in itertools.product(range(heads), range(cu[b], cu[b + 1], 128)):
+            hk, rows = h // G, torch.arange(i0, min(i0 + 128, cu[b + 1]))
+            x, pos = q[rows, h].double(), seqlens_k[b] - (cu[b + 1] - rows)
+            own = torch.arange(n) == pos[:, None] // P
+            score = x @ s["k_mean"][pages, hk].T
+            score = score.where((torch.arange(n) < pos[:, None] // P) & there & (score > -math.inf), torch.tensor(-math.inf).double())
+            best = n - 1 - score.flip(1).argsort(dim=1, descending=True, stable=True)[:, :topk - 1]  # of equals the later page
+            chosen = torch.zeros_like(own).scatter(1, best, score.gather(1, best) > -math.inf) | (own & there)
+            seen = chosen.repeat_interleave(P, 1) & (torch.arange(n * P) <= pos[:, None])
+            used = chosen.any(0)  # (of the other pages nothing is needed)
+            seen, chosen = seen[:, used.repeat_interleave(P)], chosen[:, used]
+            k = (s["k"][pages[used], hk] * s["k_scale"][pages[used], hk][:, None, None]).reshape(-1, dim)
+            v = (s["v"][pages[used], hk] * s["v_scale"][pages[used], hk][:, None, None]).reshape(-1, dim)
+            some = seen.any(1)
+            if not bool(some.any()):
                 continue
-            for h in range(heads):
-                hk, x = h // G, q[i, h].double()
-                there = [c for c in range(pos // P + 1) if 0 <= table[b][c] < s["k"].shape[0]]
-                score = [((x @ s["k_mean"][table[b][c], hk]).item(), c) for c in there if c < pos // P]
-                score = sorted(e for e in score if e[0] > -math.inf)[::-1]
-                chosen = [c for _, c in score[:topk - 1]] + [c for c in there if c == pos // P]
-                parts, vs = [], []
-                for c in chosen:
-                    page, n = table[b][c], min(P, pos + 1 - c * P)
-                    k = s["k"][page, hk, :n] * s["k_scale"][page, hk]
-                    parts.append(k @ x * scale)
-                    dot[h, i] = max(dot[h, i].item(), (k.abs() @ x.abs()).max().item() * abs(scale))
-                    vs.append(s["v"][page, hk, :n] * s["v_scale"][page, hk])
-                if not chosen:
-                    continue
-                w = torch.cat(parts)
-                lse[h, i] = torch.logsumexp(w, 0)
-                p = torch.softmax(w, 0)
-                vs = torch.cat(vs)
-                out[i, h], size[i, h], most[h, i], count[h, i] = p @ vs, p @ vs.abs(), vs.abs().max(), len(w)
-                for c, part in zip(chosen, p.split([len(x) for x in parts])):
-                    weight[table[b][c], hk] += part.sum()
+            rows, x, seen = rows[some], x[some], seen[some]
+            w = (x @ k.T * scale).where(seen, torch.tensor(-math.inf).double())
+            lse[h, rows] = torch.logsumexp(w, 1)
+            p = torch.softmax(w, 1)
+            no_number = seen.double() @ v.isnan().double() > 0  # (a NaN that a row does not see is none of it)
+            fine = v.nan_to_num(0.0)
+            out[rows, h] = (p @ fine).masked_fill(no_number, math.nan)
+            size[rows, h] = p @ fine.abs()
+            most[h, rows] = fine.abs().amax(1).where(seen, torch.tensor(0.0).double()).amax(1)
+            dot[h, rows] = (x.abs() @ k.abs().T).where(seen, torch.tensor(0.0).double()).amax(1) * abs(scale)
+            count[h, rows] = seen.sum(1).double()
+            weight[:, hk].index_add_(0, pages[used], p.view(len(rows), -1, P).sum((0, 2)))
     return out, lse, weight, (size, dot, most, count)
 
 

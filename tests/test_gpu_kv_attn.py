@@ -77,6 +77,18 @@ CASES = [  # heads, heads_k, dim, page, lens_q, lens_k, topk
     (3, 3, 256, 128, [40], [700], 4),
     (8, 1, 32, 256, [50], [900], 1),                 # its own page alone
     (4, 2, 112, 64, [20, 9], [64 * 30, 64 * 21 + 1], 64),
+    # 2048 rows times heads and more, whose pages are shared
+    (4, 2, 64, 64, [600], [600], 2),
+    (4, 1, 128, 128, [700, 1, 0, 33], [900, 300, 9, 33], 3),
+    (2, 2, 80, 64, [1030, 64], [1500, 64], 9),
+    (3, 3, 256, 128, [700], [1400], 4),
+    (3, 1, 192, 64, [699], [700], 5),
+    (8, 1, 32, 256, [300], [900], 1),
+    (4, 2, 112, 64, [500, 30], [64 * 30, 64 * 21 + 1], 64),
+    (16, 8, 64, 320, [130], [1500], 3),
+    (32, 2, 128, 1024, [66], [3000], 2),
+    (7, 1, 48, 192, [290, 7], [64 * 40, 192 * 3], 7),
+    (2, 1, 16, 64, [5, 1100, 0, 40], [0, 1101, 77, 39], 17),
 ]
 
 
@@ -106,10 +118,10 @@ def test_outputs_are_the_definitions(held, dtype, heads, heads_k, dim, P, lens_q
 
 
 @gpu
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows", [1, 5, 40, 1100])
 def test_long_contexts_with_many_pages(rows):
-    """More pages than registers (256) and, for one row, than LDS (4096) hold; few are read."""
-    for n in (300, 5000 if rows == 1 else 1100):
+    """More pages than registers (256) and LDS (2048, 1024 where rows share pages) hold; few are read."""
+    for n in (300, 2049, 2050, 5000) if rows <= 5 else (300, 1100, 2100):
         lens_k = [64 * n - 7]
         cache, table, q, cu = setup(2, 1, 16, 64, [rows], lens_k, torch.bfloat16, torch.int8, seed=n)
         out, lse = call(cache, table, q, cu, lens_k, 6)
@@ -118,7 +130,7 @@ def test_long_contexts_with_many_pages(rows):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("rows", [1, 20, 1100])
 def test_ties_and_near_ties_are_decided_as_in_64_bits(rows):
     """Means that differ in the last bits of a sum: in 32 bits the order of its terms would decide.  Equal ones: the later page."""
     P, dim, n = 64, 64, 40
@@ -140,7 +152,7 @@ def test_ties_and_near_ties_are_decided_as_in_64_bits(rows):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [1, 33])
+@pytest.mark.parametrize("rows", [1, 33, 260])
 def test_what_lies_behind_a_row_is_not_seen(rows):
     """NaN in places behind a sequence's end and behind a row, in pages that are no one's, and table entries that are no page."""
     P, dim = 64, 64
@@ -178,9 +190,10 @@ def test_what_lies_behind_a_row_is_not_seen(rows):
 
 
 @gpu
-def test_rows_that_see_nothing_and_lengths_that_do_not_fit():
+@pytest.mark.parametrize("heads", [2, 160])
+def test_rows_that_see_nothing_and_lengths_that_do_not_fit(heads):
     P, dim = 64, 32
-    cache, table, q, cu = setup(2, 1, dim, P, [1, 12, 1], [1, 200, 64], torch.float16, torch.int8)
+    cache, table, q, cu = setup(heads, 1, dim, P, [1, 12, 1], [1, 200, 64], torch.float16, torch.int8)
     lens = [0, 5, -3]  # no token, fewer tokens than rows, less than none
     out, lse = call(cache, table, q, cu, lens, 4, max_k=200)
     want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens, table, 4)
@@ -192,14 +205,14 @@ def test_rows_that_see_nothing_and_lengths_that_do_not_fit():
     assert torch.equal(a[0][:1], b[0][:1]) and torch.equal(a[0][13:], b[0][13:])
     c = call(cache, table, q, cu, [1, 200, 64], 4, max_q=3)
     want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [1, 200, 64], table, 4)
-    check(c[0][:4], c[1][:, :4], want[:4], want_lse[:, :4], tuple(x[:4] if x.dim() == 3 else x[:, :4] for x in sizes), False)
+    check(c[0][:4], c[1][:, :4], want[:4], want_lse[:, :4], tuple(x[:4] if x.dim() == 3 else x[:, :4] for x in sizes), heads > 2)  # (160 heads are 2240 rows and heads: pages are shared)
     assert bool((c[0][4:13] == 0).all())
     call(cache, table, q, [0, 100, 7, 900], [9, 200, 64], 4, max_k=200, max_q=12)
     call(cache, table, q, [-5, 3, 8, 14], [9, 200, 64], 4, max_k=200, max_q=12)
     torch.cuda.synchronize()
     i32 = dict(dtype=torch.int32, device="cuda")
     none = flash_moba.flash_moba_cache_attn_func(q[:0], cache, torch.tensor([0, 0], **i32), 0, torch.tensor([9], **i32), 9, torch.tensor([[0]], **i32), 4)
-    assert none.shape == (0, 2, 32)
+    assert none.shape == (0, heads, 32)
     empty = flash_moba.MobaKVCache.allocate(0, P, 1, dim, torch.float16, torch.int8)
     out, lse = call(empty, [[0], [0], [0]], q, cu, [1, 12, 1], 4)
     assert bool((out == 0).all()) and bool(torch.isinf(lse).all())
@@ -208,25 +221,25 @@ def test_rows_that_see_nothing_and_lengths_that_do_not_fit():
 
 
 @gpu
-@pytest.mark.parametrize("rows", [2, 30])
-def test_values_that_are_no_ordinary_numbers(rows):
+@pytest.mark.parametrize("rows,pages", [(2, 6), (30, 6), (1030, 30)])
+def test_values_that_are_no_ordinary_numbers(rows, pages):
     P, dim = 64, 32
-    cache, table, q, cu = setup(2, 2, dim, P, [rows], [64 * 6], torch.bfloat16, torch.float8_e4m3fn)
+    cache, table, q, cu = setup(2, 2, dim, P, [rows], [64 * pages], torch.bfloat16, torch.float8_e4m3fn)
     q[0, 0, 0], q[1, 1, 3] = float("nan"), float("inf")
     cache.k_mean[table[0][2], 0, 5] = float("nan")   # selects nothing
     cache.k_mean[table[0][1], 0] = -float("inf")
-    out, lse = call(cache, table, q, cu, [64 * 6], 3)
+    out, lse = call(cache, table, q, cu, [64 * pages], 3)
     assert bool(out[0, 0].isnan().all()) and bool(lse[0, 0].isnan())
     assert not bool(out[0, 1].isnan().any())
     clean = [i for i in range(rows) if i > 1]
     s = R.state(cache)
-    s["k_mean"][table[0][1], 0] = -1e30  # (as a finite score below all others: 6 pages, so it is never among the best 2 of 5)
+    s["k_mean"][table[0][1], 0] = -1e30  # (as a finite score below all others: five pages or more before a row, so it is never among the best 2)
     s["k_mean"][table[0][2], 0] = float("nan")
     qs = q.clone()
     qs[0], qs[1] = 0, 0
     qa = qs.abs()  # with it the product with -1e30 is negative, as with -inf
-    out, lse = call(cache, table, qa, cu, [64 * 6], 3)
-    want, want_lse, _, sizes = R.attention(s, qa.cpu(), cu, [64 * 6], table, 3)
+    out, lse = call(cache, table, qa, cu, [64 * pages], 3)
+    want, want_lse, _, sizes = R.attention(s, qa.cpu(), cu, [64 * pages], table, 3)
     pick = lambda x: x[clean] if x.dim() == 3 else x[:, clean]  # noqa: E731
     if clean:
         check(out[clean], lse[:, clean], pick(want), pick(want_lse), tuple(map(pick, sizes)), rows > 8)
@@ -234,7 +247,7 @@ def test_values_that_are_no_ordinary_numbers(rows):
 
 @gpu
 @pytest.mark.parametrize("P", [64, 128, 256])
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows", [1, 40, 520])
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 4.0])
 def test_scales_of_any_sign_and_pages_without_any(scale, rows, P):
     cache, table, q, cu = setup(4, 2, 64, P, [rows], [P * 5 + 30], torch.bfloat16, torch.float8_e4m3fn)
@@ -286,6 +299,10 @@ def test_a_cache_whose_offsets_pass_32_bits():
     a = call(far, table, q, [0, 1, 31], [250, 256], 3)
     b = call(near, table, q, [0, 1, 31], [250, 256], 3)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    many = torch.randn((1 + 600, 4, dim), device="cuda").bfloat16()  # (rows that share pages; the first ones see nothing)
+    a = call(far, table, many, [0, 1, 601], [250, 256], 3)
+    b = call(near, table, many, [0, 1, 601], [250, 256], 3)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and bool((a[0][400:] != 0).any())
     k = torch.randn((5, 1, dim), device="cuda").bfloat16() * 100
     i32 = dict(dtype=torch.int32, device="cuda")
     for c in (far, near):
@@ -295,21 +312,22 @@ def test_a_cache_whose_offsets_pass_32_bits():
 
 
 @gpu
-@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("rows", [1, 12, 300])
 def test_a_step_replays_from_graphs_that_run_side_by_side(rows):
     """Positions, append, attention and weights captured twice (two graphs of the same call share nothing but the cache of each) and replayed while tokens come."""
     P, dim, heads, heads_k = 64, 64, 4, 2
     i32 = dict(dtype=torch.int32, device="cuda")
     lens = [200, 130]
-    table = torch.tensor(tables([400, 400], P, 20, 4), **i32)
-    caches = [filled_cache(20, heads_k, P, dim, torch.bfloat16, torch.float8_e4m3fn, 5) for _ in range(3)]
+    most = 400 + 4 * rows
+    table = torch.tensor(tables([most, most], P, most // 25 + 4, 4), **i32)
+    caches = [filled_cache(most // 25 + 4, heads_k, P, dim, torch.bfloat16, torch.float8_e4m3fn, 5) for _ in range(3)]
     cu = torch.tensor([0, rows, 2 * rows], **i32)
     seqlens = torch.tensor(lens, **i32)
     q, k, v = (torch.randn((2 * rows, h, dim), device="cuda").bfloat16() for h in (heads, heads_k, heads_k))
     positions = torch.arange(2 * rows, device="cuda")[None]
 
     def step(cache):
-        return flash_moba.flash_moba_with_cache_func(q, k, v, cache, cu, rows, seqlens, 400, table, 3, positions=positions, add_weight=True)
+        return flash_moba.flash_moba_with_cache_func(q, k, v, cache, cu, rows, seqlens, most, table, 3, positions=positions, add_weight=True)
 
     torch.cuda.synchronize()
     graphs, held = [], []
@@ -340,7 +358,7 @@ def test_a_step_replays_from_graphs_that_run_side_by_side(rows):
 @pytest.mark.parametrize("sections", [None, (8, 12, 12)])
 def test_a_program_that_serves(held, sections):
     """A prompt in two parts, decode steps, eviction, more decode steps, with the freed pages given out again: every step against the definition."""
-    P, dim, heads, heads_k, topk = 64, 64, 4, 2, 3
+    P, dim, heads, heads_k, topk = 64, 64, 8, 2, 3
     i32 = dict(dtype=torch.int32, device="cuda")
     cache = flash_moba.MobaKVCache.allocate(12, P, heads_k, dim, torch.bfloat16, held)
     s, free, table, length, position = R.state(cache), list(range(12)), [], 0, 0
