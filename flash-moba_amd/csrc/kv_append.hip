@@ -184,6 +184,7 @@ extern "C" int fmoba_cache_append(const fmoba_cache_append_args *a, void *stream
   FMOBA_REQUIRE((((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0, "cache_append: k and v must be 16-byte aligned");
   // the pages that max_seqlen_new tokens can touch, K and V apart
   const int64_t touched = std::min<int64_t>(ceil_div64(std::min<int64_t>(a->max_seqlen_new, a->total_new), a->cache.page_size) + 1, a->max_pages);
+  FMOBA_REQUIRE(2 * touched * a->cache.heads_k * kAppendThreads <= UINT32_MAX, "cache_append: too many tokens of a sequence for the launch grid");
   const dim3 grid((uint32_t)(2 * touched * a->cache.heads_k), a->batch), block(kAppendThreads);
   const bool bf16 = a->cache.dtype == FMOBA_DTYPE_BF16, e4m3 = a->cache.format == FMOBA_CACHE_E4M3;
   auto kern = bf16 ? (e4m3 ? cache_append_kernel<bf16_t, HeldE4M3> : cache_append_kernel<bf16_t, HeldInt8>)

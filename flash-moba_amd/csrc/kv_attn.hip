@@ -410,7 +410,7 @@ static bool own_scores(int cols) { return cols - 1 <= kOwnScores; }
 // Whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own.
 static bool many_rows(const fmoba_cache_attn_args &a, int cols) {
   const int64_t rows = (int64_t)a.total_q * a.heads;
-  return cols > 0 && rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
+  return cols > 0 && cols <= kColumnCols && rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
 }
 
 template <typename T, typename H, bool WEIGHT>
@@ -426,7 +426,7 @@ static void launch_rows(const CacheAttn &p, hipStream_t s) {
 template <typename T, int HD>
 static int launch_scores(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
-  const int64_t pairs = (int64_t)a.max_seqlen_q * (a.heads / a.cache.heads_k);
+  const int64_t pairs = (int64_t)std::min(a.max_seqlen_q, a.total_q) * (a.heads / a.cache.heads_k);
   const int64_t turns = ceil_div64(pairs, kScorePairs), z = (int64_t)a.batch * a.cache.heads_k;
   FMOBA_REQUIRE(turns <= 65535 && z <= 65535, "cache_attn: too many rows, or sequences times heads, for the launch grid");
   const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)turns, (uint32_t)z);
@@ -439,6 +439,7 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
   if (many_rows(a, p.cols)) return run_cache_columns(p, s);
+  FMOBA_REQUIRE((int64_t)a.total_q * a.heads * 64 * kRowWaves <= UINT32_MAX, "cache_attn: too many rows times heads for the launch grid");
   if (!own_scores(p.cols) && p.cols > 1 && a.topk > 1) {
     if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
     FMOBA_LAUNCH_CHECK("cache_scores_kernel");

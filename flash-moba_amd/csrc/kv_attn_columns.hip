@@ -13,7 +13,6 @@
 
 namespace fmoba {
 
-constexpr int kColumnCols = 32768;  // pages of a table, at most (a word of bits for each in LDS, and its number in a score)
 constexpr int kTileRows = 32;  // rows of a head that share a word of bits
 
 struct ColumnPlan {
@@ -832,7 +831,6 @@ static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
   const size_t bytes = (size_t)held * HD * 4;
   if (int rc = with_lds(kern, bytes, "cache_columns")) return rc;
   const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.parts;
-  FMOBA_REQUIRE(grid <= INT32_MAX, "cache_attn: too many pages for the launch grid");
   hipLaunchKernelGGL(kern, dim3((uint32_t)grid), dim3(256), bytes, s, p, held);
   FMOBA_LAUNCH_CHECK("cache_columns_kernel");
   return 0;
@@ -872,7 +870,6 @@ static int run_columns_as(const ColumnPlan &p, hipStream_t s) {
 
 int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   const fmoba_cache_attn_args &a = c.a;
-  FMOBA_REQUIRE(c.cols <= kColumnCols, "cache_attn: %d pages per sequence; at most %d are supported for that many rows", c.cols, kColumnCols);
   ColumnPlan p{};
   p.c = c;
   const ColumnSizes z = column_sizes(a, c.cols, p);
@@ -887,6 +884,7 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
   const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
   p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
+  FMOBA_REQUIRE((int64_t)a.batch * a.cache.heads_k * c.cols * p.parts * 256 <= UINT32_MAX, "cache_attn: too many sequences times pages for the launch grid");
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 

@@ -81,11 +81,15 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(fmoba_rotary_arg
   }
 }
 
-template <typename T>
-static void launch_rotary(const fmoba_rotary_args &a, hipStream_t s) {
-  // a thread an angle; fewer tokens where that leaves less than two workgroups per compute unit
+// of a workgroup: a thread an angle; fewer where that leaves less than two workgroups per compute unit
+static int rotary_tokens(const fmoba_rotary_args &a) {
   int tokens = std::max(1, kRotaryThreads / (a.rotary_dim / 2));
   while (tokens > 1 && a.total / tokens < 512) tokens /= 2;
+  return tokens;
+}
+template <typename T>
+static void launch_rotary(const fmoba_rotary_args &a, hipStream_t s) {
+  const int tokens = rotary_tokens(a);
   const dim3 grid((uint32_t)ceil_div64(a.total, tokens)), block(kRotaryThreads);
   if (a.interleaved)
     hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, s, a, tokens);
@@ -114,6 +118,7 @@ extern "C" int fmoba_rotary(const fmoba_rotary_args *a, void *stream) {
   FMOBA_REQUIRE(pairs == a->rotary_dim / 2, "rotary: the sections have %lld pairs, rotary_dim has %d", (long long)pairs, a->rotary_dim / 2);
   FMOBA_REQUIRE(a->log2_base >= 0.0 && a->log2_base <= 1024.0, "rotary: base must be a number from 1 on");
   if (a->total == 0) return 0;
+  FMOBA_REQUIRE(ceil_div64(a->total, rotary_tokens(*a)) * kRotaryThreads <= UINT32_MAX, "rotary: too many tokens for the launch grid");
   FMOBA_REQUIRE(a->positions && (a->heads == 0 || (a->q && a->q_out)) && (a->heads_k == 0 || (a->k && a->k_out)), "rotary: null pointer");
   FMOBA_REQUIRE(a->q_row_stride % 8 == 0 && a->q_head_stride % 8 == 0 && a->k_row_stride % 8 == 0 && a->k_head_stride % 8 == 0 && a->qo_row_stride % 8 == 0 &&
                     a->qo_head_stride % 8 == 0 && a->ko_row_stride % 8 == 0 && a->ko_head_stride % 8 == 0,

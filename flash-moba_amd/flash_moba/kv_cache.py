@@ -92,8 +92,8 @@ def flash_moba_cache_append_func(cache, k, v, cu_seqlens, max_seqlen, seqlens_k,
 
     k, v: (tokens, num_heads_k, head_size) of the dtype of cache.k_mean, any strides; cu_seqlens: (batch + 1,) int32, which of them are whose;
     max_seqlen: the most that a sequence gets; seqlens_k: (batch,) int32, tokens of every sequence WITH the new ones, which are its
-    last; block_table: (batch, n) int32, page of the tokens i * page_size and on of a sequence at [b, i].  Different sequences must
-    not get tokens in the same page.
+    last; block_table: (batch, n) int32, page of the tokens i * page_size and on of a sequence at [b, i].  A page may get
+    tokens of one sequence only, and has one place in its table.
 
     The scale of a page and head is the least power of two (2^-64 to 2^64) that brings the largest finite magnitude among its tokens to
     448 (e4m3) or 127 (int8) at most; infinities are held as that, NaN as NaN (int8: 0).  Where a later token needs a larger scale, the

@@ -252,7 +252,8 @@ def test_the_entry_point_refuses_without_a_gpu():
     for kw, message in BAD_CACHES:
         assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(**kw))), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
-    for kw, message in [(dict(batch=0), b"batch"), (dict(total_new=-1), b"sizes"), (dict(k=0), b"null"), (dict(block_table=0), b"null"), (dict(k_row_stride=4), b"strides"), (dict(v=4100), b"aligned")]:
+    for kw, message in [(dict(batch=0), b"batch"), (dict(total_new=-1), b"sizes"), (dict(k=0), b"null"), (dict(block_table=0), b"null"), (dict(k_row_stride=4), b"strides"), (dict(v=4100), b"aligned"),
+                        (dict(total_new=2 ** 31 - 1, max_seqlen_new=2 ** 31 - 1, max_pages=1 << 26), b"launch grid")]:
         assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(), **kw)), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
     assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(), total_new=0)), None) == 0

@@ -130,6 +130,29 @@ def test_long_contexts_with_many_pages(rows):
 
 
 @gpu
+@pytest.mark.parametrize("n", [32768, 33000])
+def test_the_longest_tables(n):
+    """The most pages that rows share, and more, chosen by many rows (most of them are the same page, and worth nothing), and a bound on the rows that says nothing."""
+    P, dim, rows = 64, 16, 2100
+    cache, _, q, cu = setup(1, 1, dim, P, [rows], [P * 200], torch.bfloat16, torch.float8_e4m3fn)
+    g = torch.Generator().manual_seed(8)
+    table = [[200] * n]
+    for i, c in enumerate(torch.randperm(n - 40, generator=g)[:160].tolist()):
+        table[0][c] = i
+    table[0][-40:] = list(range(160, 200))
+    q.abs_()
+    cache.k_mean.abs_()
+    cache.k_mean[200] = -1.0
+    cache.k[200] = 0
+    lens_k = [P * n - 5]
+    out, lse = call(cache, table, q, cu, lens_k, 64)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, 64)
+    check(out, lse, want, want_lse, sizes, True)
+    few, few_lse = call(cache, table, q[-2:], [0, 2], lens_k, 64, max_q=2 ** 31 - 1)
+    check(few, few_lse, want[-2:], want_lse[:, -2:], tuple(x[-2:] if x.dim() == 3 else x[:, -2:] for x in sizes), False)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 20, 1100])
 def test_ties_and_near_ties_are_decided_as_in_64_bits(rows):
     """Means that differ in the last bits of a sum: in 32 bits the order of its terms would decide.  Equal ones: the later page."""
@@ -451,8 +474,10 @@ def test_the_entry_point_refuses_without_a_gpu():
         assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(**kw))), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
     for kw, message in [(dict(batch=0), b"batch"), (dict(total_q=-1), b"sizes"), (dict(heads=3), b"divide"), (dict(topk=0), b"moba_topk"), (dict(topk=65), b"moba_topk"), (dict(q=0), b"null"),
-                        (dict(softmax_lse=0), b"null"), (dict(block_table=0), b"null"), (dict(q_row_stride=4), b"strides"), (dict(out=4100), b"aligned"), (dict(workspace_bytes=16), b"workspace"),
-                        (dict(workspace=4100), b"workspace"), (dict(total_q=1 << 30, heads=8), b"launch grid")]:
+                        (dict(softmax_lse=0), b"null"), (dict(block_table=0), b"null"), (dict(q_row_stride=4), b"strides"), (dict(out=4100), b"aligned"), (dict(workspace_bytes=16, total_q=4096), b"workspace"),
+                        (dict(workspace=4100), b"workspace"), (dict(total_q=1 << 30, heads=8), b"launch grid"),
+                        (dict(batch=65535, total_q=1 << 22, max_seqlen_k=65536, max_pages=1024), b"launch grid"),              # a workgroup a row and head
+                        (dict(batch=65535, total_q=1 << 26, max_seqlen_k=65536, max_pages=1024), b"times pages for the launch grid")]:
         assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(), **kw)), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
     assert lib.fmoba_cache_attn(ctypes.byref(args(cache_struct(weight=0), add_weight=1)), None) != 0

@@ -247,7 +247,7 @@ def test_the_entry_point_refuses_without_a_gpu():
     for kw, message in [(dict(dtype=2), b"fp16 and bf16"), (dict(total=-1), b"tokens"), (dict(heads=0, heads_k=0), b"heads"), (dict(head_dim=12), b"head_size"),
                         (dict(rotary_dim=128), b"rotary_dim"), (dict(rotary_dim=4), b"rotary_dim"), (dict(axes=0), b"axes"), (dict(axes=5), b"axes"), (dict(section=31), b"pairs"),
                         (dict(section=-1), b"negative"), (dict(log2_base=-1.0), b"base"), (dict(log2_base=math.nan), b"base"), (dict(q=0), b"null"), (dict(positions=0), b"null"),
-                        (dict(q_row_stride=4), b"strides"), (dict(k=4100), b"aligned")]:
+                        (dict(q_row_stride=4), b"strides"), (dict(k=4100), b"aligned"), (dict(total=2 ** 31 - 1), b"launch grid")]:
         assert lib.fmoba_rotary(ctypes.byref(args(**kw)), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
     assert lib.fmoba_rotary(ctypes.byref(args(total=0, q=0)), None) == 0  # no tokens: nothing to do
