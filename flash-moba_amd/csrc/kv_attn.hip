@@ -74,7 +74,9 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(CacheAttn p) {
 
 // ------------------------------------------------------------------------------------
 // One workgroup per (row, head): eight waves take the units of 64 keys of its pages side by side and merge in LDS.  16 bytes (features) a lane and load,
-// LPR lanes a key.
+// LPR lanes a key.  Every key and value that a row reads is read once (from the L2 again where heads of a group choose alike): 16 rows of 16 sequences with 512 to 32768 tokens, 32
+// over 8 heads of 128, 8 pages of 128: 22.7 us, 106 MB at 4.7 TB/s.  With fewer rows than compute units it is a chain: scores, choice, pages, merge (four rows of up to 262144
+// tokens, 16 heads of 64: 30 us on 64 units; sixteen waves instead of eight took 28.5 there and 14.5 instead of 12.7 for four of 8192, 32 heads).
 // ------------------------------------------------------------------------------------
 constexpr int kUnitKeys = 64;
 constexpr int kRowWaves = 8;  // of a workgroup: two of them share a compute unit

@@ -5,8 +5,9 @@
 //            A page is brought into LDS once for all of them, widened to 16 bits, exactly; its scales multiply scores and the result of a visit.
 //            Every visit leaves its output over the page and the logarithm of its sum.
 //   combine  adds a row's visits.
-// The weights of a visit are at most 1 and its output, in units of the page's scale, at most 448 times their sum: both are kept in fp16, whatever the type of q (in bf16 each
-// would cost eight times its error; fp16 leaves 2^-12 of the output beside the 2^-9 of a bf16 one).
+// The weights of a visit are at most 1 and go to the second product in fp16, whatever the type of q (2^-12 of each on average; in bf16 eight times that).  Its output is left in 16-bit
+// whole numbers, 32767 for the largest of its features: at most 2^-16 of that is lost, a quarter of what fp16 would lose of most features (which, beside the weights' rounding, cost
+// outputs in fp16 1.6 times their own rounding against 64 bits).
 #include "kv_attn.h"
 
 #include <algorithm>
@@ -15,13 +16,15 @@ namespace fmoba {
 
 constexpr int kTileRows = 32;  // rows of a head that share a word of bits
 
+constexpr int kNanPart = -32768;
+
 struct ColumnPlan {
   CacheAttn c;
   int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
   uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
   float *scores;     // [block of 32 rows][head][32 rows][half of the wave][slot], where LDS does not hold them
   float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum of weights, and what its output has to be multiplied by
-  uint16_t *part;    // [(row, head)][topk4][head_dim]: that output, fp16
+  uint16_t *part;    // [(row, head)][topk4][head_dim]: that output, int16; kNanPart is a NaN
   int32_t topk4;     // topk, rounded up to a multiple of four
   int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
   int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
@@ -36,8 +39,10 @@ __device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRo
 // product's 32 pages.  A score gives its lowest bits up for the page's number; eight groups of a lane's scores are known by their largest, and the best
 // are taken off one by one: the largest of eight, whose group is then looked through again.  About 60 instructions for one page of 32 rows, where counting
 // scores above a cut (a ballot per 64 scores and bit) takes 30 for one bit of one row: 29 instead of 142 us, 8191 tokens, 16 heads, 64 pages.
+// Bound by latency: 2825 rows of three sequences, 32 heads, up to 258 pages take 58 us, of which a workgroup spends a fifth on its queries' way, two fifths on the scores and a third on the
+// best (the other waves wait); LDS has room for three of them a compute unit.  Page numbers a tile ahead and means fetched 64 bytes of a row at a time changed nothing.
 // ------------------------------------------------------------------------------------
-constexpr int kGateCols = 1024;   // pages whose scores of 32 rows LDS holds (135 KB); beyond, in the workspace
+constexpr int kGateCols = 1024;   // pages whose scores of 32 rows LDS holds (135 KB); beyond, in the workspace (258 pages, whole calls: 94 us in LDS, 156 in the workspace)
 constexpr int kGateGroups = 8;
 
 // row . mean of a page in 64 bits, by 16 lanes (four pages a wave)
@@ -335,12 +340,25 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
 }
 
 // ------------------------------------------------------------------------------------
-// columns
+// columns: a workgroup of four waves keeps a page in LDS and takes 128 of its rows a turn, what a turn needs of memory on its way during the one before.  Products and softmax of a turn
+// would take a third of what it does: of a workgroup's 33 thousand clocks (1.9 turns a page) 16 thousand are gone before its first product, on lengths and table,
+// words of bits and the page, the rows, one after the other, and two waves a SIMD (254 registers) hide little of it.  2825 rows of three sequences of 9216 to 33000
+// tokens, 32 over 8 heads of 128: 150 us, 385 MB at 2.6 TB/s; 8191 rows, 16 heads: 147 us, 0.47 PFLOP/s.
 // ------------------------------------------------------------------------------------
 constexpr int kColumnRows = 128;  // of a turn: 32 a wave
 constexpr int kColumnWords = 128;  // words of bits that are spread out at a time: 32 a wave
 constexpr int kColumnList = kColumnRows + kColumnWords * 32;
 constexpr int kColumnPart = 2048;  // words of a workgroup, at most: an entry of its list has 16 bits
+
+// two numbers of [-1, 1] as int16, rounded to nearest
+__device__ __forceinline__ uint32_t pack_part(float x, float y) {
+  uint32_t w = 0u;
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto two = __builtin_amdgcn_cvt_pknorm_i16(x, y);
+  __builtin_memcpy(&w, &two, 4);
+#endif
+  return w;
+}
 
 // ONE: the page is one step of KT keys, which LDS holds
 template <typename T, typename H, int HD, int KT, bool ONE>  // KT: keys of a softmax step
@@ -554,9 +572,14 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     }
     if (ONE && next > 0) take_over();
     uint16_t *dst = p.part + at * D;
-    // In one step of up to 128 keys the sums reach 128 * 448, which fp16 holds: they are divided by the weights' sum with the scale, else here.
-    const float inv = l == 0.f ? 0.f : 1.f / l, norm = ONE ? 1.f : inv;
-    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), ONE ? v_scale * inv : v_scale);
+    float most = 1e-36f;  // (a NaN is none; smaller sums are nothing beside the others')
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(o[d][i]));
+    most = max_xor32_f(most);
+    const float inv = l == 0.f ? 0.f : 1.f / l, norm = __builtin_amdgcn_rcpf(most);
+    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale * (inv * most * (1.f / 32767.f)));
     {
       // Features 8 j + 4 hh .. of both halves to eight of one lane, then to four lanes with 64 bytes of a row, as the queries were loaded: stores of 16 bytes of 64
       // rows at a time take the caches a cycle for each.
@@ -568,7 +591,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) (j < 2 ? x : y)[(j & 1) * 2 + i] = pack2<f16_t>(o[d][4 * j + 2 * i] * norm, o[d][4 * j + 2 * i + 1] * norm);
+          for (int i = 0; i < 2; ++i) (j < 2 ? x : y)[(j & 1) * 2 + i] = pack_part(o[d][4 * j + 2 * i] * norm, o[d][4 * j + 2 * i + 1] * norm);
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -593,7 +616,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
         const int last = min(lim, keys - 1);
         for (int e = hh; e < D; e += 2)
           for (int k = 0; k <= last; ++k)
-            if ((vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) dst[e] = 0x7e00;
+            if ((vg[(int64_t)k * a.cache.v_token_stride + e] & 0x7f) == 0x7f) dst[e] = (uint16_t)kNanPart;
       }
     }
   };
@@ -665,13 +688,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 }
 
 // ------------------------------------------------------------------------------------
-// combine: LPR lanes a (row, head), eight features each
+// combine: LPR lanes a (row, head), eight features each.  Bound by memory: two bytes a feature and visit (2825 rows, 32 heads of 128, 8 pages a row: 40 us, 206 MB at
+// 5.1 TB/s; 46 with as many registers as the compiler takes, for five waves a SIMD instead of six).
 // ------------------------------------------------------------------------------------
 // WEIGHT: what pages receive is added up in LDS for the 64 rows of the workgroup first (integers, so in no order): rows next to each other choose alike, and
 // atomics on few addresses of memory are slow (a million of them 180 us).
 constexpr int kCombineRows = 64, kCombineCols = 2048;
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 template <typename T, int LPR, bool WEIGHT>
-__global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
+__global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(ColumnPlan p) {
   constexpr int NS = 64 / LPR, AT_ONCE = 8;  // slots of a lane; rows asked for together
   __shared__ unsigned long long sWeight[WEIGHT ? kCombineCols : 1];
   const fmoba_cache_attn_args &a = p.c.a;
@@ -687,86 +712,97 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(ColumnPlan p) {
     __syncthreads();
   }
   for (int t = t0 + tid / LPR; t < min(t0 + kCombineRows, a.total_q); t += 256 / LPR) {
-  const int64_t rowhead = (int64_t)t * a.heads + h;
-  const int32_t *sel = p.sel + rowhead * p.topk4;
-  const float2 *head = p.head + rowhead * p.topk4;
-  const uint16_t *part = p.part + rowhead * p.topk4 * D;
-  const RowPlace at = find_row_lane(a, t);
-  // the row's visits, one or more a lane: their pages fill the slots from the first on
-  int page_of[NS];
-  float w[NS], vs[NS], m = -INFINITY;
+    const int64_t rowhead = (int64_t)t * a.heads + h;
+    const int32_t *sel = p.sel + rowhead * p.topk4;
+    const float2 *head = p.head + rowhead * p.topk4;
+    const uint16_t *part = p.part + rowhead * p.topk4 * D;
+    const RowPlace at = find_row_lane(a, t);
+    // the row's visits, one or more a lane: their pages fill the slots from the first on
+    int page_of[NS];
+    float w[NS], vs[NS], m = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    const int s = j * LPR + li;
-    page_of[j] = s < p.topk4 && at.pos >= 0 ? sel[s] : -1;
-  }
+    for (int j = 0; j < NS; ++j) {
+      const int s = j * LPR + li;
+      page_of[j] = s < p.topk4 && at.pos >= 0 ? sel[s] : -1;
+    }
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    const float2 x = page_of[j] >= 0 ? head[j * LPR + li] : make_float2(-INFINITY, 0.f);
-    w[j] = x.x, vs[j] = x.y;
-    m = x.x > m ? x.x : m;
-  }
+    for (int j = 0; j < NS; ++j) {
+      const float2 x = page_of[j] >= 0 ? head[j * LPR + li] : make_float2(-INFINITY, 0.f);
+      w[j] = x.x, vs[j] = x.y;
+      m = x.x > m ? x.x : m;
+    }
 #pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  int n = 0;
+    for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    int n = 0;
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    w[j] = __builtin_amdgcn_exp2f(w[j] - ref);
-    l += w[j];
-    vs[j] *= w[j];
-    n += page_of[j] >= 0 ? 1 : 0;
-  }
+    for (int j = 0; j < NS; ++j) {
+      w[j] = __builtin_amdgcn_exp2f(w[j] - ref);
+      l += w[j];
+      vs[j] *= w[j];
+      n += page_of[j] >= 0 ? 1 : 0;
+    }
 #pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64), n += __shfl_xor(n, o, 64);
-  const int e = li * 8;
-  float acc[8];
+    for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64), n += __shfl_xor(n, o, 64);
+    const int e = li * 8;
+    float acc[8];
+    i16x2 least = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
 #pragma unroll
-  for (int j = 0; j < NS; ++j) {
-    if (j * LPR >= p.topk4) break;
-    for (int i0 = 0; i0 < LPR && j * LPR + i0 < p.topk4; i0 += AT_ONCE) {
-      Pack8 x[AT_ONCE];
+    for (int j = 0; j < NS; ++j) {
+      if (j * LPR >= p.topk4) break;
+      for (int i0 = 0; i0 < LPR && j * LPR + i0 < p.topk4; i0 += AT_ONCE) {
+        Pack8 x[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const int s = j * LPR + i0 + i;
-        x[i] = s < n && e < D ? ld_stream16(part + (int64_t)s * D + e) : zero_pack8();
-      }
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int s = j * LPR + i0 + i;
+          x[i] = s < n && e < D ? ld_stream16(part + (int64_t)s * D + e) : zero_pack8();
+        }
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const float wv = __shfl(vs[j], group + i0 + i, 64);
-        float f[8];
-        unpack8<f16_t>(x[i], f);
-        if (j * LPR + i0 + i < n && wv != 0.f) {
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const float of_visit = __shfl(vs[j], group + i0 + i, 64), wv = j * LPR + i0 + i < n ? of_visit : 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] = fmaf(wv, f[k], acc[k]);
+          for (int k = 0; k < 4; ++k) {
+            i16x2 two;
+            __builtin_memcpy(&two, &x[i].w[k], 4);
+            least = __builtin_elementwise_min(least, two);
+            acc[2 * k] = fmaf(wv, (float)two.x, acc[2 * k]);
+            acc[2 * k + 1] = fmaf(wv, (float)two.y, acc[2 * k + 1]);
+          }
         }
       }
     }
-  }
-  const bool empty = l == 0.f;
-  const float inv = empty ? 0.f : 1.f / l;
-  if (e < D) {
-    Pack8 o;
+    if (min(least.x, least.y) == kNanPart) {  // (seldom: of the visits that count, once more)
+      for (int s = 0; s < n; ++s) {
+        if (__builtin_amdgcn_exp2f(head[s].x - ref) == 0.f) continue;
+        const Pack8 again = ld_global16(part + (int64_t)s * D + e);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o.w[j] = pack2<T>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-    *reinterpret_cast<Pack8 *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t)t * a.o_row_stride + (int64_t)h * a.o_head_stride + e) = o;
-  }
-  if (li == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-  if constexpr (WEIGHT) {
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const float part_of = w[j] * inv;
-      if (!(part_of > 0.f) || page_of[j] < 0) continue;
-      const unsigned long long x = (unsigned long long)rintf(part_of * 4294967296.f);
-      if (at.b == b0 && page_of[j] < cols)
-        atomicAdd(&sWeight[page_of[j]], x);
-      else
-        receive(at.b, page_of[j], x);
+        for (int k = 0; k < 8; ++k) acc[k] = (int16_t)(again.w[k >> 1] >> (16 * (k & 1))) == kNanPart ? NAN : acc[k];
+      }
     }
-  }
+    const bool empty = l == 0.f;
+    const float inv = empty ? 0.f : 1.f / l;
+    if (e < D) {
+      Pack8 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o.w[j] = pack2<T>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+      *reinterpret_cast<Pack8 *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t)t * a.o_row_stride + (int64_t)h * a.o_head_stride + e) = o;
+    }
+    if (li == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    if constexpr (WEIGHT) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const float part_of = w[j] * inv;
+        if (!(part_of > 0.f) || page_of[j] < 0) continue;
+        const unsigned long long x = (unsigned long long)rintf(part_of * 4294967296.f);
+        if (at.b == b0 && page_of[j] < cols)
+          atomicAdd(&sWeight[page_of[j]], x);
+        else
+          receive(at.b, page_of[j], x);
+      }
+    }
   }
   if constexpr (WEIGHT) {
     __syncthreads();
@@ -820,6 +856,7 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   while ((1 << page_bits) < p.c.cols) ++page_bits;
   auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
   if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
+  // whole calls, us with one wave, two, four: 64 pages 270, 274, 293; 256 pages 124, 121, 127; 512 188, 169, 164; 1024 395, 320, 286
   const int waves = p.c.cols <= 64 ? 1 : p.c.cols <= 320 ? 2 : 4;
   hipLaunchKernelGGL(kern, grid, dim3(64 * waves), bytes, s, p, page_bits);
   FMOBA_LAUNCH_CHECK("cache_gate_kernel");
@@ -838,7 +875,8 @@ static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
 template <typename T, typename H, int HD>
 static int launch_columns(const ColumnPlan &p, hipStream_t s) {
   const int P = p.c.a.cache.page_size;
-  // the whole page where two workgroups find room on a compute unit, else 64 keys at a time
+  // the whole page where two workgroups find room on a compute unit, else 64 keys at a time; pages of 64 and (of heads up to 128, whose 128 scores a row fit the registers) 128 keys are
+  // one step, which nothing before it has to be scaled for, and whose next rows can be on their way
   const int held = P * HD * 4 <= 64 * 1024 ? P : 64;
   if constexpr (HD <= 128) {
     if (P == 128) return launch_columns_as<T, H, HD, 128, true>(p, held, s);

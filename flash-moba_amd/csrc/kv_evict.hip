@@ -3,14 +3,17 @@
 //
 // Bound by latency: 8 heads_k bytes per page are gathered once.  One histogram of the weights in bins of a 32nd of a power of two says in which bin the cut
 // lies; of the few weights there the last one to stay is the one of the right rank, or, if they are many, is found byte by byte.  The pages kept and the pages
-// let go are written in order, every wave a stretch of the table.
+// let go are written in order, every wave a stretch of the table.  16 tables of up to 768 pages 9.3 us, 64 of up to 4096 22.6 (34 with one workgroup for all of a table's
+// sums, and byte by byte from the first bit on).
 #include "fmoba_common.h"
 
 namespace fmoba {
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictPages = 8192;  // pages of a sequence whose weights are kept in LDS (64 KB); beyond, in the workspace
-constexpr int kEvictAlone = 1024;  // pages of a table that the sequence's workgroup sums itself; with more a launch before it does
+// Pages of a table that the sequence's workgroup sums itself; with more a launch before it does.  us alone and with the launch, 16 tables of 8 heads: 512 pages 9.1, 10.4; 1024 11.2, 11.7; 2048
+// 16.4, 13.7; 4096 26.8, 18.5.
+constexpr int kEvictAlone = 1024;
 
 // Bin of a key: the place of its highest bit and the five bits behind it (a key below 32 is its own bin), so that the bins of weights of any size hold alike.
 constexpr int kEvictBins = 32 * 60;

@@ -3,8 +3,8 @@
 Which pages a row reads is decided as in 64 bits, so nothing is left out of the comparison for near-ties.  Error of an output: a score of D
 products in 32 bits is off by at most (D + 8) 2^-24 of scale sum |q| |k| (8: the scales, the change of base and the exponential's argument), the exponential
 by 2^-22, a sum of n weights by n 2^-24; weights are off by twice the first two, relatively, and an output by that times sum p |v|, and by half a
-step of its type.  Where many rows share a page, its weights and its part of an output are rounded to fp16 (2^-11 each; weights below 2^-14 by 2^-25 of the
-largest)."""
+step of its type.  Where many rows share a page, its weights are rounded to fp16 (2^-11; weights below 2^-14 by 2^-25 of the largest), and its part of an
+output to 32767ths of its largest feature: half a step of each of the parts, whose weights add up to 1, is up to max |v| 2^-16."""
 import ctypes
 import math
 
@@ -19,12 +19,12 @@ from test_gpu_kv_append import BAD_CACHES, cache_struct, random_cache, tables
 gpu = pytest.mark.gpu
 
 
-def check(got, lse, want, want_lse, sizes, fp16_parts):
+def check(got, lse, want, want_lse, sizes, parts):
     size, dot, most, count = sizes
     D = got.shape[2]
     delta = ((D + 8) * 2.0 ** -24 * dot + 2.0 ** -22)
-    weights = (2 * delta + count * 2.0 ** -24 + (2 * 2.0 ** -11 if fp16_parts else 0.0)).t()[:, :, None]
-    tol = want.abs() * torch.finfo(got.dtype).eps / 2 * 1.01 + size * weights + (2.0 ** -25 * (count * most).t()[:, :, None] if fp16_parts else 0.0) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    weights = (2 * delta + count * 2.0 ** -24 + (2.0 ** -11 if parts else 0.0)).t()[:, :, None]
+    tol = want.abs() * torch.finfo(got.dtype).eps / 2 * 1.01 + size * weights + (((2.0 ** -25 * count + 2.0 ** -16 * 1.01) * most).t()[:, :, None] if parts else 0.0) + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
     err = (got.float().cpu().double() - want).abs()
     assert bool((err <= tol).all()), f"out {(err - tol).max().item():.3e} over, largest error {err.max().item():.3e}"
     lse = lse.cpu().double()
