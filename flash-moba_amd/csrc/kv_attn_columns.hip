@@ -691,16 +691,16 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 // combine: LPR lanes a (row, head), eight features each.  Bound by memory: two bytes a feature and visit (2825 rows, 32 heads of 128, 8 pages a row: 40 us, 206 MB at
 // 5.1 TB/s; 46 with as many registers as the compiler takes, for five waves a SIMD instead of six).
 // ------------------------------------------------------------------------------------
-// WEIGHT: what pages receive is added up in LDS for the 64 rows of the workgroup first (integers, so in no order): rows next to each other choose alike, and
+// WEIGHT: what pages receive is added up in LDS for the rows of the workgroup first (integers, so in no order): rows next to each other choose alike, and
 // atomics on few addresses of memory are slow (a million of them 180 us).
-constexpr int kCombineRows = 64, kCombineCols = 2048;
+constexpr int kCombineCols = 2048;
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 template <typename T, int LPR, bool WEIGHT>
-__global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(ColumnPlan p) {
+__global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(ColumnPlan p, int rows) {  // rows: of a workgroup
   constexpr int NS = 64 / LPR, AT_ONCE = 8;  // slots of a lane; rows asked for together
   __shared__ unsigned long long sWeight[WEIGHT ? kCombineCols : 1];
   const fmoba_cache_attn_args &a = p.c.a;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim, h = blockIdx.y, t0 = blockIdx.x * kCombineRows;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim, h = blockIdx.y, t0 = blockIdx.x * rows;
   const int hk = h / (a.heads / a.cache.heads_k), cols = min(p.c.cols, kCombineCols);
   const int b0 = WEIGHT ? find_row_lane(a, t0).b : 0;
   auto receive = [&](int b, int c, unsigned long long x) {
@@ -711,7 +711,7 @@ __global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(Co
     for (int i = tid; i < cols; i += 256) sWeight[i] = 0ull;
     __syncthreads();
   }
-  for (int t = t0 + tid / LPR; t < min(t0 + kCombineRows, a.total_q); t += 256 / LPR) {
+  for (int t = t0 + tid / LPR; t < min(t0 + rows, a.total_q); t += 256 / LPR) {
     const int64_t rowhead = (int64_t)t * a.heads + h;
     const int32_t *sel = p.sel + rowhead * p.topk4;
     const float2 *head = p.head + rowhead * p.topk4;
@@ -886,11 +886,15 @@ static int launch_columns(const ColumnPlan &p, hipStream_t s) {
 }
 template <typename T, int LPR>
 static void launch_combine(const ColumnPlan &p, hipStream_t s) {
-  const dim3 grid(ceil_div(p.c.a.total_q, kCombineRows), p.c.a.heads);
+  const int64_t pairs = (int64_t)p.c.a.total_q * p.c.a.heads;
+  // Rows of a workgroup: fewer where there are few, more spare the weights' atomics.  Whole calls, us with 16, 32, 64, 128 rows, heads of 128 without weights and with: 2048 pairs 35, 38, 44, 56
+  // and 40, 42, 50, 64; 8192 49, 51, 56, 68 and 62, 59, 61, 75; 32768 78, 76, 80, 87 and 117, 99, 91, 96; 131056 219, 213, 212, 213 and 277, 243, 229, 225.
+  const int rows = std::max(pairs <= 4096 ? 16 : pairs <= 16384 ? 32 : 64, 256 / LPR);
+  const dim3 grid(ceil_div(p.c.a.total_q, rows), p.c.a.heads);
   if (p.c.a.add_weight)
-    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, true>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, true>), grid, dim3(256), 0, s, p, rows);
   else
-    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, false>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((cache_combine_kernel<T, LPR, false>), grid, dim3(256), 0, s, p, rows);
 }
 template <typename T, int HD>
 static int run_columns_hd(const ColumnPlan &p, hipStream_t s) {
