@@ -23,9 +23,12 @@ struct ColumnPlan {
   int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
   uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
   float *scores;     // [block of 32 rows][head][32 rows][half of the wave][slot], where LDS does not hold them
-  float2 *head;      // [(row, head)][topk4]: log2 of a visit's sum of weights, and what its output has to be multiplied by
-  uint16_t *part;    // [(row, head)][topk4][head_dim]: that output, int16; kNanPart is a NaN
+  float2 *head;      // [(row, head)][slots]: log2 of a visit's sum of weights, and what its output has to be multiplied by
+  uint16_t *part;    // [(row, head)][slots][head_dim]: that output, int16; kNanPart is a NaN
   int32_t topk4;     // topk, rounded up to a multiple of four
+  int32_t steps;     // a page's, each a column of its own with step_keys keys (or 1)
+  int32_t step_keys;
+  int32_t slots;     // visits of a row, at most: pages times steps
   int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
   int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
   int32_t parts;     // workgroups of a page
@@ -360,7 +363,7 @@ __device__ __forceinline__ uint32_t pack_part(float x, float y) {
   return w;
 }
 
-// ONE: the page is one step of KT keys, which LDS holds
+// ONE: the column is one step of KT keys, which LDS holds
 template <typename T, typename H, int HD, int KT, bool ONE>  // KT: keys of a softmax step
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
   constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, ROW = HD * 2;  // (LDS rows of exactly HD elements, their pieces swizzled: tile_swz)
@@ -370,21 +373,22 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k, cols = p.c.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
-  const PairItem item = xcd_pair_item(blockIdx.x, a.batch * a.cache.heads_k, cols * p.parts);
-  const int b = item.pair / a.cache.heads_k, hk = item.pair - b * a.cache.heads_k, c = item.idx / p.parts, part = item.idx - c * p.parts;
+  const PairItem item = xcd_pair_item(blockIdx.x, a.batch * a.cache.heads_k, cols * p.steps * p.parts);
+  const int b = item.pair / a.cache.heads_k, hk = item.pair - b * a.cache.heads_k, nth = item.idx / p.parts, part = item.idx - nth * p.parts;
+  const int c = nth / p.steps, step = nth - c * p.steps, key0 = ONE ? step * KT : 0;  // page of the table, and the first of its keys that are this column's
   const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b], page = a.block_table[(int64_t)b * a.table_stride + c];  // (asked for together)
   const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q);
-  if (q0 < 0 || R <= 0 || (int64_t)c * P >= len || page < 0 || page >= a.cache.num_pages) return;
+  if (q0 < 0 || R <= 0 || (int64_t)c * P + key0 >= len || page < 0 || page >= a.cache.num_pages) return;
   const int shift = len - (q1 - q0), G_tiles = (R + kTileRows - 1) / kTileRows * G;
   // the words of rows that can see the page, shared out evenly
-  const int first = max(c * P - shift, 0) / kTileRows * G;
+  const int first = max(c * P + key0 - shift, 0) / kTileRows * G;
   const int each = ((G_tiles - first + p.parts - 1) / p.parts + 7) / 8 * 8;
   const int w0 = first + part * each, w1 = min(w0 + each, G_tiles);
   if (w0 >= w1) return;
-  const int keys = min(P, len - c * P);  // of the page that are there
+  const int keys = min(ONE ? KT : P, len - c * P - key0);  // that are there
   const uint32_t *bits = p.bits + ((int64_t)hk * p.blocks + block_of(q0, b)) * G * cols + c;
-  const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + (int64_t)page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride;
-  const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + (int64_t)page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride;
+  const uint8_t *kg = reinterpret_cast<const uint8_t *>(a.cache.k) + (int64_t)page * a.cache.k_page_stride + (int64_t)hk * a.cache.k_head_stride + (int64_t)key0 * a.cache.k_token_stride;
+  const uint8_t *vg = reinterpret_cast<const uint8_t *>(a.cache.v) + (int64_t)page * a.cache.v_page_stride + (int64_t)hk * a.cache.v_head_stride + (int64_t)key0 * a.cache.v_token_stride;
   const int my_word = wave * 32 + li;
   uint32_t word = hh == 0 && w0 + my_word < w1 ? bits[(int64_t)(w0 + my_word) * cols] : 0u;  // (those of the next turn of words, always)
   // the scale of a score, its sign with q (the largest product is the largest score), and not 0 (times which a masked product would be no number)
@@ -495,8 +499,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[ks].w[i] ^= q_sign;
     }
-    at_next = rowhead * p.topk4 + place();
-    lim_next = shift + row - c * P;  // last key of the page that the row sees
+    at_next = rowhead * p.slots + place() * p.steps + step;
+    lim_next = shift + row - c * P - key0;  // last key that the row sees (of its own page's later steps none, and the combine looks at none)
   };
   // one turn: `count` entries of the list, which were asked for and taken over; then those of the next turn, `next` from `from_next` on
   auto turn = [&](int count, int from_next, int next) {
@@ -689,20 +693,21 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
 
 // ------------------------------------------------------------------------------------
 // combine: LPR lanes a (row, head), eight features each.  Bound by memory: two bytes a feature and visit (2825 rows, 32 heads of 128, 8 pages a row: 40 us, 206 MB at
-// 5.1 TB/s; 46 with as many registers as the compiler takes, for five waves a SIMD instead of six).
+// 5.1 TB/s; 46 with as many registers as the compiler takes, for five waves a SIMD instead of six; with weights, or heads of 64, the smaller number spills).
 // ------------------------------------------------------------------------------------
 // WEIGHT: what pages receive is added up in LDS for the rows of the workgroup first (integers, so in no order): rows next to each other choose alike, and
 // atomics on few addresses of memory are slow (a million of them 180 us).
-constexpr int kCombineCols = 2048;
+constexpr int kCombineCols = 2048, kCombineSlots = 64;
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 template <typename T, int LPR, bool WEIGHT>
-__global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(ColumnPlan p, int rows) {  // rows: of a workgroup
-  constexpr int NS = 64 / LPR, AT_ONCE = 8;  // slots of a lane; rows asked for together
+__global__ __launch_bounds__(256, !WEIGHT && LPR == 16 ? 6 : 4) void cache_combine_kernel(ColumnPlan p, int rows) {  // rows: of a workgroup
+  constexpr int AT_ONCE = 8;  // parts asked for together
   __shared__ unsigned long long sWeight[WEIGHT ? kCombineCols : 1];
   const fmoba_cache_attn_args &a = p.c.a;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim, h = blockIdx.y, t0 = blockIdx.x * rows;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane % LPR, group = lane - li, D = a.cache.head_dim, P = a.cache.page_size, h = blockIdx.y, t0 = blockIdx.x * rows;
   const int hk = h / (a.heads / a.cache.heads_k), cols = min(p.c.cols, kCombineCols);
   const int b0 = WEIGHT ? find_row_lane(a, t0).b : 0;
+  const uint32_t per_step = (65535u + (uint32_t)p.steps) / (uint32_t)p.steps;  // s / steps = s per_step >> 16 for s below 64 and up to 16 steps
   auto receive = [&](int b, int c, unsigned long long x) {
     const int page = a.block_table[(int64_t)b * a.table_stride + c];
     if (page >= 0 && page < a.cache.num_pages) atomicAdd(reinterpret_cast<unsigned long long *>(a.cache.weight) + (int64_t)page * a.cache.heads_k + hk, x);
@@ -714,55 +719,54 @@ __global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(Co
   for (int t = t0 + tid / LPR; t < min(t0 + rows, a.total_q); t += 256 / LPR) {
     const int64_t rowhead = (int64_t)t * a.heads + h;
     const int32_t *sel = p.sel + rowhead * p.topk4;
-    const float2 *head = p.head + rowhead * p.topk4;
-    const uint16_t *part = p.part + rowhead * p.topk4 * D;
+    const float2 *head = p.head + rowhead * p.slots;
+    const uint16_t *part = p.part + rowhead * p.slots * D;
     const RowPlace at = find_row_lane(a, t);
-    // the row's visits, one or more a lane: their pages fill the slots from the first on
-    int page_of[NS];
-    float w[NS], vs[NS], m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const int s = j * LPR + li;
-      page_of[j] = s < p.topk4 && at.pos >= 0 ? sel[s] : -1;
-    }
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      const float2 x = page_of[j] >= 0 ? head[j * LPR + li] : make_float2(-INFINITY, 0.f);
-      w[j] = x.x, vs[j] = x.y;
+    // visit s of the row: its page (or -1), the logarithm of its weights' sum (-inf if there is none) and its output's factor
+    auto visit = [&](int s, int &c, float2 &x) {
+      const int nth = (int)((uint32_t)s * per_step >> 16), page = s < p.slots && at.pos >= 0 ? sel[nth] : -1;
+      c = page >= 0 && at.pos - page * P >= (s - nth * p.steps) * p.step_keys ? page : -1;  // (its own page is a row's last, and has the steps up to its place)
+      x = c >= 0 ? head[s] : make_float2(-INFINITY, 0.f);
+    };
+    // They fill the slots from the first on, LPR of them at a time, one a lane; most rows have no more, and are asked for once.
+    int c_first, n = 0;
+    float2 x_first;
+    float m = -INFINITY, l = 0.f;
+    visit(li, c_first, x_first);
+#pragma unroll 1
+    for (int s0 = 0; s0 < p.slots; s0 += LPR) {
+      int c = c_first;
+      float2 x = x_first;
+      if (s0 > 0) visit(s0 + li, c, x);
       m = x.x > m ? x.x : m;
+      n += c >= 0 ? 1 : 0;
     }
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64)), n += __shfl_xor(n, o, 64);
     const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      w[j] = __builtin_amdgcn_exp2f(w[j] - ref);
-      l += w[j];
-      vs[j] *= w[j];
-      n += page_of[j] >= 0 ? 1 : 0;
-    }
-#pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64), n += __shfl_xor(n, o, 64);
     const int e = li * 8;
     float acc[8];
     i16x2 least = {0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-      if (j * LPR >= p.topk4) break;
-      for (int i0 = 0; i0 < LPR && j * LPR + i0 < p.topk4; i0 += AT_ONCE) {
+#pragma unroll 1
+    for (int s0 = 0; s0 < p.slots; s0 += LPR) {
+      int c = c_first;
+      float2 x_head = x_first;
+      if (s0 > 0) visit(s0 + li, c, x_head);
+      const float w = __builtin_amdgcn_exp2f(x_head.x - ref), vs = w * x_head.y;
+      l += w;
+#pragma unroll 1
+      for (int i0 = 0; i0 < LPR && s0 + i0 < p.slots; i0 += AT_ONCE) {
         Pack8 x[AT_ONCE];
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-          const int s = j * LPR + i0 + i;
+          const int s = s0 + i0 + i;
           x[i] = s < n && e < D ? ld_stream16(part + (int64_t)s * D + e) : zero_pack8();
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-          const float of_visit = __shfl(vs[j], group + i0 + i, 64), wv = j * LPR + i0 + i < n ? of_visit : 0.f;
+          const float of_visit = __shfl(vs, group + i0 + i, 64), wv = s0 + i0 + i < n ? of_visit : 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             i16x2 two;
@@ -774,6 +778,8 @@ __global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(Co
         }
       }
     }
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64);
     if (min(least.x, least.y) == kNanPart) {  // (seldom: of the visits that count, once more)
       for (int s = 0; s < n; ++s) {
         if (__builtin_amdgcn_exp2f(head[s].x - ref) == 0.f) continue;
@@ -792,15 +798,18 @@ __global__ __launch_bounds__(256, LPR == 8 ? 5 : 6) void cache_combine_kernel(Co
     }
     if (li == 0) a.softmax_lse[(int64_t)h * a.total_q + t] = empty ? INFINITY : (ref + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     if constexpr (WEIGHT) {
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const float part_of = w[j] * inv;
-        if (!(part_of > 0.f) || page_of[j] < 0) continue;
-        const unsigned long long x = (unsigned long long)rintf(part_of * 4294967296.f);
-        if (at.b == b0 && page_of[j] < cols)
-          atomicAdd(&sWeight[page_of[j]], x);
+  #pragma unroll 1
+    for (int s0 = 0; s0 < p.slots; s0 += LPR) {
+        int c = c_first;
+        float2 x = x_first;
+        if (s0 > 0) visit(s0 + li, c, x);
+        const float part_of = __builtin_amdgcn_exp2f(x.x - ref) * inv;
+        if (!(part_of > 0.f) || c < 0) continue;
+        const unsigned long long whole = (unsigned long long)rintf(part_of * 4294967296.f);
+        if (at.b == b0 && c < cols)
+          atomicAdd(&sWeight[c], whole);
         else
-          receive(at.b, page_of[j], x);
+          receive(at.b, c, whole);
       }
     }
   }
@@ -823,12 +832,21 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   p.topk4 = (a.topk + 3) / 4 * 4;
   p.blocks = a.total_q / kTileRows + a.batch;
   p.tiles = ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows) * (a.heads / a.cache.heads_k);
+  // Pages of one step (64 keys, or 128 of heads up to 128, whose scores of a row fit the registers): nothing before it has to be scaled for, and its next rows can be on their way.  Larger pages are
+  // several columns of one step each, as far as the combine has places for a row's visits; else one column of many steps, whose keys come into LDS 64 at a time, again for every turn,
+  // where two workgroups do not find room for all.  (8191 tokens, 16 over 4 heads of 128, pages of 256 keys, four a row: 260 us in two steps, 526 in one column; of 512, two a row: 245 and 670;
+  // heads of 256, pages of 128, eight a row: 785 and 1013.)
+  const int pages = std::min(a.topk, cols);
+  p.step_keys = a.cache.head_dim <= 128 && a.cache.page_size % 128 == 0 ? 128 : 64;
+  p.steps = a.cache.page_size / p.step_keys;
+  if (pages * p.steps > kCombineSlots) p.steps = 1, p.step_keys = a.cache.page_size;
+  p.slots = pages * p.steps;
   ColumnSizes z;
   z.sel = up(rowheads * p.topk4 * 4);
   z.bits = up((size_t)a.heads * p.blocks * cols * 4);
   z.scores = cols > kGateCols ? up((size_t)a.heads * p.blocks * kTileRows * 2 * gate_stride(cols) * 4) : 0;
-  z.head = up(rowheads * p.topk4 * 8);
-  z.part = up(rowheads * p.topk4 * a.cache.head_dim * 2);
+  z.head = up(rowheads * p.slots * 8);
+  z.part = up(rowheads * p.slots * a.cache.head_dim * 2);
   z.total = z.sel + z.bits + z.scores + z.head + z.part;
   return z;
 }
@@ -867,7 +885,7 @@ static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
   auto kern = cache_columns_kernel<T, H, HD, KT, ONE>;
   const size_t bytes = (size_t)held * HD * 4;
   if (int rc = with_lds(kern, bytes, "cache_columns")) return rc;
-  const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.parts;
+  const int64_t grid = (int64_t)p.c.a.batch * p.c.a.cache.heads_k * p.c.cols * p.steps * p.parts;
   hipLaunchKernelGGL(kern, dim3((uint32_t)grid), dim3(256), bytes, s, p, held);
   FMOBA_LAUNCH_CHECK("cache_columns_kernel");
   return 0;
@@ -875,14 +893,11 @@ static int launch_columns_as(const ColumnPlan &p, int held, hipStream_t s) {
 template <typename T, typename H, int HD>
 static int launch_columns(const ColumnPlan &p, hipStream_t s) {
   const int P = p.c.a.cache.page_size;
-  // the whole page where two workgroups find room on a compute unit, else 64 keys at a time; pages of 64 and (of heads up to 128, whose 128 scores a row fit the registers) 128 keys are
-  // one step, which nothing before it has to be scaled for, and whose next rows can be on their way
-  const int held = P * HD * 4 <= 64 * 1024 ? P : 64;
   if constexpr (HD <= 128) {
-    if (P == 128) return launch_columns_as<T, H, HD, 128, true>(p, held, s);
+    if (p.step_keys == 128) return launch_columns_as<T, H, HD, 128, true>(p, 128, s);
   }
-  if (P == 64) return launch_columns_as<T, H, HD, 64, true>(p, held, s);
-  return launch_columns_as<T, H, HD, 64, false>(p, held, s);
+  if (p.step_keys == 64) return launch_columns_as<T, H, HD, 64, true>(p, 64, s);
+  return launch_columns_as<T, H, HD, 64, false>(p, P * HD * 4 <= 64 * 1024 ? P : 64, s);
 }
 template <typename T, int LPR>
 static void launch_combine(const ColumnPlan &p, hipStream_t s) {
@@ -926,7 +941,7 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
   const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
   p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
-  FMOBA_REQUIRE((int64_t)a.batch * a.cache.heads_k * c.cols * p.parts * 256 <= UINT32_MAX, "cache_attn: too many sequences times pages for the launch grid");
+  FMOBA_REQUIRE((int64_t)a.batch * a.cache.heads_k * c.cols * p.steps * p.parts * 256 <= UINT32_MAX, "cache_attn: too many sequences times pages for the launch grid");
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 

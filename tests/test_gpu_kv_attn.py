@@ -89,6 +89,11 @@ CASES = [  # heads, heads_k, dim, page, lens_q, lens_k, topk
     (32, 2, 128, 1024, [66], [3000], 2),
     (7, 1, 48, 192, [290, 7], [64 * 40, 192 * 3], 7),
     (2, 1, 16, 64, [5, 1100, 0, 40], [0, 1101, 77, 39], 17),
+    (4, 2, 96, 384, [40, 500], [384 * 4, 901], 3),
+    # and more steps of their pages than the last launch has places for
+    (1, 1, 32, 256, [2200], [256 * 40 + 10], 40),
+    (4, 1, 128, 1024, [3, 550], [1000, 1024 * 9 + 5], 9),
+    (4, 4, 256, 128, [530], [128 * 34 - 1], 33),
 ]
 
 
