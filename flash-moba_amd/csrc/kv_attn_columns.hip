@@ -7,7 +7,7 @@
 //   combine  adds a row's visits.
 // The weights of a visit are at most 1 and go to the second product in fp16, whatever the type of q (2^-12 of each on average; in bf16 eight times that).  Its output is left in 16-bit
 // whole numbers, 32767 for the largest of its features: at most 2^-16 of that is lost, a quarter of what fp16 would lose of most features (which, beside the weights' rounding, cost
-// outputs in fp16 1.6 times their own rounding against 64 bits).
+// outputs in fp16 1.6 times their own rounding against 64 bits).  Features far below the largest lose more of themselves, but a page's values are eight bits of one scale to begin with.
 #include "kv_attn.h"
 
 #include <algorithm>
@@ -346,7 +346,8 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
 // columns: a workgroup of four waves keeps a page in LDS and takes 128 of its rows a turn, what a turn needs of memory on its way during the one before.  Products and softmax of a turn
 // would take a third of what it does: of a workgroup's 33 thousand clocks (1.9 turns a page) 16 thousand are gone before its first product, on lengths and table,
 // words of bits and the page, the rows, one after the other, and two waves a SIMD (254 registers) hide little of it.  2825 rows of three sequences of 9216 to 33000
-// tokens, 32 over 8 heads of 128: 150 us, 385 MB at 2.6 TB/s; 8191 rows, 16 heads: 147 us, 0.47 PFLOP/s.
+// tokens, 32 over 8 heads of 128: 155 us, 385 MB at 2.5 TB/s; 8191 rows, 16 heads: 147 us, 0.47 PFLOP/s.  (Two pages a workgroup, the second one's bytes on their way during the first one's last
+// turn, in the registers of the rows: 185 and 206.)
 // ------------------------------------------------------------------------------------
 constexpr int kColumnRows = 128;  // of a turn: 32 a wave
 constexpr int kColumnWords = 128;  // words of bits that are spread out at a time: 32 a wave
