@@ -180,10 +180,11 @@ def test_ties_and_near_ties_are_decided_as_in_64_bits(rows):
 
 
 @gpu
+@pytest.mark.parametrize("P", [64, 256])
 @pytest.mark.parametrize("rows", [1, 33, 260])
-def test_what_lies_behind_a_row_is_not_seen(rows):
+def test_what_lies_behind_a_row_is_not_seen(rows, P):
     """NaN in places behind a sequence's end and behind a row, in pages that are no one's, and table entries that are no page."""
-    P, dim = 64, 64
+    dim = 64
     lens_k = [P * 5 + 40, 70]
     cache, table, q, cu = setup(4, 2, dim, P, [rows, rows], lens_k, torch.bfloat16, torch.float8_e4m3fn, spare=3)
     s = R.state(cache)
