@@ -7,7 +7,7 @@
 // workgroup takes whole tokens, as many as give each of its threads an angle, and keeps their cosines and sines in LDS.  An angle is formed in
 // 64 bits as a number of turns and reduced there (positions reach 2^31; in 32 bits position 262144 would be off by 0.01 radians), sine and cosine of the rest
 // are taken in 32 bits.  24571 tokens, 16 and 16 heads of 128, there and back: 150 us, 0.8 GB at 5.4 TB/s; one token of each of 16 requests: 5.4 us.
-#include "fmoba_common.h"
+#include "rotary.h"
 
 #include <algorithm>
 
@@ -15,35 +15,6 @@ namespace fmoba {
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryPairs = 128;  // of a head, at most (rotary_dim <= 256)
-
-// W: features of a vector, 8, or 4 where half of rotary_dim is no multiple of 8
-template <typename T, int W, bool INTERLEAVED>
-__device__ __forceinline__ void rotate_piece(const uint16_t *src, uint16_t *dst, const float2 *cs, int piece, int half) {
-  constexpr int NW = W / 2;  // 32-bit words of a vector
-  typedef uint32_t vec __attribute__((ext_vector_type(NW)));
-  auto value = [](uint32_t w, int i) { return elem_to_float<T>((uint16_t)(w >> (16 * i))); };
-  if constexpr (INTERLEAVED) {
-    vec x = *reinterpret_cast<const vec *>(src + piece * W);
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const float2 c = cs[piece * NW + i];
-      const float a = value(x[i], 0), b = value(x[i], 1);
-      x[i] = pack2<T>(a * c.x - b * c.y, a * c.y + b * c.x);
-    }
-    *reinterpret_cast<vec *>(dst + piece * W) = x;
-  } else {
-    vec x = *reinterpret_cast<const vec *>(src + piece * W), y = *reinterpret_cast<const vec *>(src + half + piece * W);
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const float2 c0 = cs[piece * W + 2 * i], c1 = cs[piece * W + 2 * i + 1];
-      const float a0 = value(x[i], 0), a1 = value(x[i], 1), b0 = value(y[i], 0), b1 = value(y[i], 1);
-      x[i] = pack2<T>(a0 * c0.x - b0 * c0.y, a1 * c1.x - b1 * c1.y);
-      y[i] = pack2<T>(a0 * c0.y + b0 * c0.x, a1 * c1.y + b1 * c1.x);
-    }
-    *reinterpret_cast<vec *>(dst + piece * W) = x;
-    *reinterpret_cast<vec *>(dst + half + piece * W) = y;
-  }
-}
 
 template <typename T, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(fmoba_rotary_args a, int tokens) {  // tokens: of a workgroup
@@ -53,14 +24,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(fmoba_rotary_arg
   const int nt = (int)min((int64_t)tokens, a.total - t0);
   for (int i = tid; i < nt * pairs; i += kRotaryThreads) {
     const int t = i / pairs, j = i - t * pairs;
-    int axis = 0, end = a.sections[0];
-    while (axis + 1 < a.axes && j >= end) end += a.sections[++axis];
-    const int64_t at = axis * a.pos_axis_stride + t0 + t;
-    const double pos = a.positions_64 ? (double)reinterpret_cast<const int64_t *>(a.positions)[at] : (double)reinterpret_cast<const int32_t *>(a.positions)[at];
-    const double turns = pos * (exp2(a.log2_base * (-2.0 * j / a.rotary_dim)) * 0.15915494309189533577);
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    sTurn[i] = make_float2(c, a.inverse ? -s : s);
+    sTurn[i] = turn_of(a, t0 + t, j);
   }
   __syncthreads();
   const int turned = INTERLEAVED ? a.rotary_dim / W : pairs / W, copied = (a.head_dim - a.rotary_dim) / 8;
@@ -99,10 +63,7 @@ static void launch_rotary(const fmoba_rotary_args &a, hipStream_t s) {
     hipLaunchKernelGGL((rotary_kernel<T, 4, false>), grid, block, 0, s, a, tokens);
 }
 
-}  // namespace fmoba
-
-extern "C" int fmoba_rotary(const fmoba_rotary_args *a, void *stream) {
-  using namespace fmoba;
+int check_rotary_args(const fmoba_rotary_args *a, bool k_out) {
   FMOBA_REQUIRE(a != nullptr, "rotary: null args");
   FMOBA_REQUIRE(a->dtype == FMOBA_DTYPE_F16 || a->dtype == FMOBA_DTYPE_BF16, "FlashMoBA only supports fp16 and bf16 data types");
   FMOBA_REQUIRE(a->total >= 0 && a->total <= INT32_MAX && a->heads >= 0 && a->heads_k >= 0 && a->heads + a->heads_k >= 1 && a->heads <= 65535 && a->heads_k <= 65535,
@@ -119,11 +80,20 @@ extern "C" int fmoba_rotary(const fmoba_rotary_args *a, void *stream) {
   FMOBA_REQUIRE(a->log2_base >= 0.0 && a->log2_base <= 1024.0, "rotary: base must be a number from 1 on");
   if (a->total == 0) return 0;
   FMOBA_REQUIRE(ceil_div64(a->total, rotary_tokens(*a)) * kRotaryThreads <= UINT32_MAX, "rotary: too many tokens for the launch grid");
-  FMOBA_REQUIRE(a->positions && (a->heads == 0 || (a->q && a->q_out)) && (a->heads_k == 0 || (a->k && a->k_out)), "rotary: null pointer");
+  FMOBA_REQUIRE(a->positions && (a->heads == 0 || (a->q && a->q_out)) && (a->heads_k == 0 || (a->k && (a->k_out || !k_out))), "rotary: null pointer");
   FMOBA_REQUIRE(a->q_row_stride % 8 == 0 && a->q_head_stride % 8 == 0 && a->k_row_stride % 8 == 0 && a->k_head_stride % 8 == 0 && a->qo_row_stride % 8 == 0 &&
                     a->qo_head_stride % 8 == 0 && a->ko_row_stride % 8 == 0 && a->ko_head_stride % 8 == 0,
                 "rotary: strides must be multiples of 8 elements");
   FMOBA_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->q_out | (uintptr_t)a->k_out) % 16) == 0, "rotary: q and k must be 16-byte aligned");
+  return 0;
+}
+
+}  // namespace fmoba
+
+extern "C" int fmoba_rotary(const fmoba_rotary_args *a, void *stream) {
+  using namespace fmoba;
+  if (int rc = check_rotary_args(a, true)) return rc;
+  if (a->total == 0) return 0;
   if (a->dtype == FMOBA_DTYPE_BF16)
     launch_rotary<bf16_t>(*a, (hipStream_t)stream);
   else

@@ -57,30 +57,40 @@ void check_rotary(const Tensor &q, const Tensor &k, const Tensor &positions, con
   require(pairs == f.rotary_dim / 2, "the sections must have rotary_dim / 2 pairs together");
 }
 
+// the positions of x's tokens and how they turn; pos: a tensor that keeps them alive
+fmoba_rotary_args rotary_args(const Tensor &x, const Tensor &positions, const RotaryForm &f, Tensor &pos) {
+  fmoba_rotary_args a{};
+  pos = positions.size(1) > 1 && positions.stride(1) != 1 ? positions.contiguous() : positions;
+  a.positions = pos.data_ptr(), a.positions_64 = pos.scalar_type() == at::kLong, a.pos_axis_stride = pos.stride(0);
+  a.log2_base = std::log2(f.base), a.total = x.size(0), a.head_dim = x.size(2), a.rotary_dim = f.rotary_dim;
+  a.axes = f.sections.size();
+  for (int i = 0; i < a.axes; ++i) a.sections[i] = f.sections[i];
+  a.interleaved = f.interleaved, a.inverse = f.inverse, a.dtype = x.scalar_type() == at::kBFloat16 ? FMOBA_DTYPE_BF16 : FMOBA_DTYPE_F16;
+  return a;
+}
+// dense queries and the place of the turned ones
+Tensor rotary_queries(fmoba_rotary_args &a, Tensor &q) {
+  q = as_rows(q);
+  const Tensor qo = at::empty(q.sizes(), q.options());
+  a.q = q.data_ptr(), a.q_out = qo.data_ptr(), a.heads = q.size(1);
+  a.q_row_stride = q.stride(0), a.q_head_stride = q.stride(1), a.qo_row_stride = qo.stride(0), a.qo_head_stride = qo.stride(1);
+  return qo;
+}
+
 // q and k, or only one of them (the other undefined): what is given comes back turned
 std::pair<Tensor, Tensor> turn(Tensor q, Tensor k, const Tensor &positions, const RotaryForm &f) {
   const Tensor &x = q.defined() ? q : k;
   const c10::DeviceGuard guard(x.device());
   check_device(x.device().index());
-  fmoba_rotary_args a{};
-  Tensor qo, ko, pos = positions.size(1) > 1 && positions.stride(1) != 1 ? positions.contiguous() : positions;
-  if (q.defined()) {
-    q = as_rows(q);
-    qo = at::empty(q.sizes(), q.options());
-    a.q = q.data_ptr(), a.q_out = qo.data_ptr(), a.heads = q.size(1);
-    a.q_row_stride = q.stride(0), a.q_head_stride = q.stride(1), a.qo_row_stride = qo.stride(0), a.qo_head_stride = qo.stride(1);
-  }
+  Tensor qo, ko, pos;
+  fmoba_rotary_args a = rotary_args(x, positions, f, pos);
+  if (q.defined()) qo = rotary_queries(a, q);
   if (k.defined()) {
     k = as_rows(k);
     ko = at::empty(k.sizes(), k.options());
     a.k = k.data_ptr(), a.k_out = ko.data_ptr(), a.heads_k = k.size(1);
     a.k_row_stride = k.stride(0), a.k_head_stride = k.stride(1), a.ko_row_stride = ko.stride(0), a.ko_head_stride = ko.stride(1);
   }
-  a.positions = pos.data_ptr(), a.positions_64 = pos.scalar_type() == at::kLong, a.pos_axis_stride = pos.stride(0);
-  a.log2_base = std::log2(f.base), a.total = x.size(0), a.head_dim = x.size(2), a.rotary_dim = f.rotary_dim;
-  a.axes = f.sections.size();
-  for (int i = 0; i < a.axes; ++i) a.sections[i] = f.sections[i];
-  a.interleaved = f.interleaved, a.inverse = f.inverse, a.dtype = x.scalar_type() == at::kBFloat16 ? FMOBA_DTYPE_BF16 : FMOBA_DTYPE_F16;
   check(fmoba_rotary(&a, current_stream(x)));
   return {qo, ko};
 }
@@ -215,7 +225,8 @@ void check_inference(std::initializer_list<const Tensor *> ts) {
     require(!(at::GradMode::is_enabled() && t->requires_grad()), "the cache functions have no backward pass: call them under torch.no_grad(), or with detached tensors");
 }
 
-void append_raw(const Cache &c, const Tensor &k_in, const Tensor &v_in, const Tensor &cu, int64_t max_seqlen, const Tensor &seqlens_k, const Tensor &table) {
+// turn: the queries and positions, if the keys are to be turned first
+void append_raw(const Cache &c, const Tensor &k_in, const Tensor &v_in, const Tensor &cu, int64_t max_seqlen, const Tensor &seqlens_k, const Tensor &table, fmoba_rotary_args *turn = nullptr) {
   fmoba_cache_append_args a{};
   a.cache = cache_view(c);
   const at::Device dev = c.k.device();
@@ -233,7 +244,12 @@ void append_raw(const Cache &c, const Tensor &k_in, const Tensor &v_in, const Te
   a.total_new = k.size(0), a.max_seqlen_new = max_seqlen, a.max_pages = table.size(1);
   const c10::DeviceGuard guard(dev);
   check_device(dev.index());
-  check(fmoba_cache_append(&a, current_stream(c.k)));
+  if (turn) {
+    turn->k = a.k, turn->heads_k = k.size(1), turn->k_row_stride = a.k_row_stride, turn->k_head_stride = a.k_head_stride;
+    check(fmoba_cache_append_turned(&a, turn, current_stream(c.k)));
+  } else {
+    check(fmoba_cache_append(&a, current_stream(c.k)));
+  }
 }
 
 struct AttnForm {
@@ -367,11 +383,17 @@ py::object cache_step(const py::handle &hq, const py::handle &hk, const py::hand
     cache_view(c);  // (what the attention would refuse is refused before the cache changes)
     check_attn(q, c, attn);
     check_inference({&k});
-    if (turned) {
-      check_rotary(q, k, unpack(hp), f);
-      std::tie(q, k) = turn(q, k, unpack(hp), f);
+    if (turned) check_rotary(q, k, unpack(hp), f);
+    if (turned && max_q <= FMOBA_TURN_ROWS) {
+      Tensor pos;
+      fmoba_rotary_args a = rotary_args(q, unpack(hp), f, pos);
+      const Tensor qo = rotary_queries(a, q);
+      append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable), &a);
+      q = qo;
+    } else {
+      if (turned) std::tie(q, k) = turn(q, k, unpack(hp), f);
+      append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable));
     }
-    append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable));
     r = attn_raw(q, c, unpack(hcu), unpack(hlen), unpack(htable), attn);
   }
   return py::make_tuple(wrap(r.first), wrap(r.second));

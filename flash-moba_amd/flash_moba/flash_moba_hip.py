@@ -159,6 +159,7 @@ EXPORTS = {
     "fmoba_attn_bwd_phases": (c_i32, [ctypes.POINTER(AttnBwdArgs), c_i32, c_vp]),
     "fmoba_rotary": (c_i32, [ctypes.POINTER(RotaryArgs), c_vp]),
     "fmoba_cache_append": (c_i32, [ctypes.POINTER(CacheAppendArgs), c_vp]),
+    "fmoba_cache_append_turned": (c_i32, [ctypes.POINTER(CacheAppendArgs), ctypes.POINTER(RotaryArgs), c_vp]),
     "fmoba_cache_attn_workspace_bytes": (c_sz, [ctypes.POINTER(CacheAttnArgs)]),
     "fmoba_cache_attn": (c_i32, [ctypes.POINTER(CacheAttnArgs), c_vp]),
     "fmoba_cache_evict_workspace_bytes": (c_sz, [c_i32, c_i32]),

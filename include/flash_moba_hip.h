@@ -360,6 +360,10 @@ typedef struct {
   int32_t batch, total_new, max_seqlen_new, max_pages; /* max_pages: entries of a sequence's table */
 } fmoba_cache_append_args;
 int fmoba_cache_append(const fmoba_cache_append_args *a, void *stream);
+/* The same with fmoba_rotary of q and k in front, in one launch: the keys are turned on their way into the pages, the queries into turn->q_out.  The two
+ * agree on the tokens, the dtype and the keys (turn->k_out is not used); up to FMOBA_TURN_ROWS new tokens of a sequence.  Tokens of no sequence are not turned. */
+#define FMOBA_TURN_ROWS 8
+int fmoba_cache_append_turned(const fmoba_cache_append_args *a, const fmoba_rotary_args *turn, void *stream);
 
 /* Gated attention of query rows over the cache.  The rows of sequence b, cu_seqlens_q[b + 1] - cu_seqlens_q[b] of them, are its last tokens: row i has
  * position p = seqlens_k[b] - rows + i and sees the keys up to p of the pages that it selects: its own, p / page_size, and of the pages before

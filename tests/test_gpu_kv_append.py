@@ -257,6 +257,23 @@ def test_the_entry_point_refuses_without_a_gpu():
         assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(), **kw)), None) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
     assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(), total_new=0)), None) == 0
+
+    def turn(**kw):
+        r = H.RotaryArgs()
+        r.total, r.heads, r.heads_k, r.head_dim, r.rotary_dim, r.axes, r.log2_base, r.dtype = 16, 4, 2, 64, 64, 1, 13.0, 1
+        r.sections[0] = 32
+        r.q = r.k = r.q_out = r.positions = 4096
+        r.k_row_stride = r.k_head_stride = 64
+        for n, v in kw.items():
+            setattr(r, n, v)
+        return r
+
+    assert lib.fmoba_cache_append_turned(ctypes.byref(args(cache_struct())), None, None) != 0 and lib.fmoba_cache_append_turned(None, ctypes.byref(turn()), None) != 0
+    for kw, r, message in [(dict(max_seqlen_new=9), {}, b"up to 8"), (dict(total_new=15), {}, b"not the keys"), ({}, dict(heads_k=1), b"not the keys"), ({}, dict(k=8192), b"not the keys"),
+                           ({}, dict(k_row_stride=128), b"not the keys"), ({}, dict(dtype=0), b"not the keys"), ({}, dict(q_out=0), b"null"), ({}, dict(rotary_dim=128), b"rotary_dim"),
+                           (dict(v=0), {}, b"null"), (dict(batch=0), {}, b"batch")]:
+        assert lib.fmoba_cache_append_turned(ctypes.byref(args(cache_struct(), **kw)), ctypes.byref(turn(**r)), None) != 0, (kw, r)
+        assert message in lib.fmoba_last_error(), (kw, r, lib.fmoba_last_error())
     assert lib.fmoba_cache_append(ctypes.byref(args(cache_struct(num_pages=0, k=0))), None) == 0
 
 

@@ -420,6 +420,33 @@ def test_a_program_that_serves(held, sections):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,held", [(torch.bfloat16, torch.int8), (torch.float16, torch.float8_e4m3fn)])
+@pytest.mark.parametrize("dim,rotary_dim,sections,interleaved", [(64, None, None, False), (64, 40, None, False), (128, 64, (8, 12, 12), False), (256, None, None, True), (96, 48, (4, 20), True),
+                                                                 (16, 8, None, False)])
+def test_a_step_is_its_parts(dtype, held, dim, rotary_dim, sections, interleaved):
+    """Positions on the way into the cache: the bits of the three functions one after the other; tokens across a page's end, of no sequence, and before a sequence's beginning."""
+    P, heads, heads_k = 64, 6, 2
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new, lens_k = [1, 8, 0, 3, 5, 1], [1, 131, 70, 66, 3, 128]
+    cache, table, q, cu = setup(heads, heads_k, dim, P, new + [2], lens_k, dtype, held)
+    cu = cu[:-1]
+    other = flash_moba.MobaKVCache(*[t.clone() for t in cache])
+    g = torch.Generator(device="cuda").manual_seed(11)
+    kv = torch.randn((sum(new) + 2, 2, heads_k, dim), generator=g, device="cuda").to(dtype)  # (strided: both in one tensor)
+    k, v = kv[:, 0], kv[:, 1]
+    at = torch.randint(0, 10 ** 6, (len(sections) if sections else 1, sum(new) + 2), generator=g, device="cuda")
+    turn = dict(sections=sections, base=5e5, rotary_dim=rotary_dim, interleaved=interleaved)
+    for positions in (at, at.int()):
+        args = (torch.tensor(cu, **i32), 8, torch.tensor(lens_k, **i32), max(lens_k), torch.tensor(table, **i32), 3)
+        out, lse = flash_moba.flash_moba_with_cache_func(q, k, v, cache, *args, positions=positions, add_weight=True, return_lse=True, **turn)
+        tq, tk = flash_moba.flash_moba_rotary_func(q, k, positions, sections, 5e5, rotary_dim, interleaved)
+        flash_moba.flash_moba_cache_append_func(other, tk, v, args[0], 8, args[2], args[4])
+        want, want_lse = flash_moba.flash_moba_cache_attn_func(tq, other, *args, add_weight=True, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, other))
+
+
+@gpu
 def test_step_and_attention_from_traced_graphs():
     P, dim = 64, 32
     cache, table, q, cu = setup(4, 2, dim, P, [3], [200], torch.bfloat16, torch.int8)
