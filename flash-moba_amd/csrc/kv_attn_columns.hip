@@ -653,7 +653,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
     __syncthreads();
     return count;
   };
-  if (!ONE && held >= P) stage(0);
+  if (!ONE && held >= P) {
+    __syncthreads();  // (sNan is cleared before any wave sets it: the others have a barrier of their own before they store)
+    stage(0);
+  }
   if (ONE) stage_ask(0, tid);
   int wb = w0, count = spread(w0, 0);
   if (ONE && (count >= kColumnRows || wb + kColumnWords >= w1) && count > 0) ask(0, min(kColumnRows, count));

@@ -1,0 +1,52 @@
+"""The two forms of flash_moba_cache_attn_func, each where it runs: what a caller sees of a value must not depend on how many rows a call has.
+
+Tolerances are those of test_gpu_kv_attn.py, with the bound of the form that the call takes."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import cache_reference as R
+import flash_moba
+from flash_moba import flash_moba_hip as H
+from test_gpu_kv_attn import call, check, setup
+from test_gpu_kv_append import cache_struct
+
+gpu = pytest.mark.gpu
+
+
+def shares_pages(heads, heads_k, dim, P, lens_q, lens_k, topk, max_pages):
+    """Whether a call is of the form for many rows: it alone has a workspace for tables of up to 2049 pages."""
+    a = H.CacheAttnArgs()
+    a.cache = cache_struct(page_size=P, heads_k=heads_k, head_dim=dim)
+    a.batch, a.total_q, a.heads, a.max_seqlen_q, a.max_seqlen_k, a.max_pages, a.topk = len(lens_q), sum(lens_q), heads, max(lens_q), max(lens_k), max_pages, topk
+    assert min(-(-max(lens_k) // P), max_pages) <= 2049
+    return H.load_library().fmoba_cache_attn_workspace_bytes(ctypes.byref(a)) > 0
+
+
+def check_with_nans(out, lse, want, want_lse, sizes, parts):
+    assert torch.equal(out.isnan().cpu(), want.isnan())
+    check(out.nan_to_num(0.0), lse, want.nan_to_num(0.0), want_lse, sizes, parts)
+
+
+@gpu
+@pytest.mark.parametrize("heads,heads_k,dim,P,rows,length,topk,parts", [
+    (1, 1, 32, 256, 2200, 256 * 40 + 10, 40, True),     # a page of several steps, all of it in LDS
+    (2, 1, 64, 192, 1100, 192 * 30 - 1, 24, True),
+    (4, 1, 128, 1024, 550, 1024 * 9 + 5, 9, True),      # and 64 keys of it at a time
+    (4, 2, 256, 128, 520, 128 * 34, 33, True),
+    (4, 2, 64, 64, 600, 900, 5, True),                  # a page of one step
+    (4, 2, 128, 256, 600, 2000, 5, True),               # pages of several columns
+    (4, 2, 128, 128, 20, 2000, 5, False),
+])
+def test_a_row_has_the_nans_of_the_values_that_it_sees(heads, heads_k, dim, P, rows, length, topk, parts):
+    cache, table, q, cu = setup(heads, heads_k, dim, P, [rows], [length], torch.bfloat16, torch.float8_e4m3fn)
+    assert shares_pages(heads, heads_k, dim, P, [rows], [length], topk, len(table[0])) == parts
+    used = (length + P - 1) // P
+    for c, place, hk, e in ((0, 3, 0, 5), (used // 2, P - 1, heads_k - 1, dim - 1), (used - 1, (length - 1) % P // 2, 0, 0), (used - 2, 70 % P, 0, dim // 2)):
+        cache.v.view(torch.int8)[table[0][c], hk, place, e] = -1 if c & 1 else 0x7F  # (of either sign)
+    out, lse = call(cache, table, q, cu, [length], topk)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [length], table, topk)
+    assert bool(want.isnan().any()) and not bool(want.isnan().all())
+    check_with_nans(out, lse, want, want_lse, sizes, parts)
