@@ -5,9 +5,9 @@
 //            A page is brought into LDS once for all of them, widened to 16 bits, exactly; its scales multiply scores and the result of a visit.
 //            Every visit leaves its output over the page and the logarithm of its sum.
 //   combine  adds a row's visits.
-// The weights of a visit are at most 1 and go to the second product in fp16, whatever the type of q (2^-12 of each on average; in bf16 eight times that).  Its output is left in 16-bit
-// whole numbers, 32767 for the largest of its features: at most 2^-16 of that is lost, a quarter of what fp16 would lose of most features (which, beside the weights' rounding, cost
-// outputs in fp16 1.6 times their own rounding against 64 bits).  Features far below the largest lose more of themselves, but a page's values are eight bits of one scale to begin with.
+// The weights of a visit go to the second product as two fp16 numbers each (split_weights).  Its output is summed in 32 bits and left in 16-bit whole numbers, 32767 for the largest of
+// its features: at most 2^-16 of that is lost, a quarter of what fp16 would lose of most features.  Features far below the largest lose more of themselves, but a
+// page's values are eight bits of one scale to begin with.
 #include "kv_attn.h"
 
 #include <algorithm>
@@ -364,6 +364,21 @@ __device__ __forceinline__ uint32_t pack_part(float x, float y) {
   return w;
 }
 
+// Weights are formed as 2^15 of themselves and go to the second product as two fp16 numbers each, the second what the first cuts off: what is lost is 2^-20 of a weight, or 2^-39
+// of the largest.  (As one fp16 number, 2^-11 of a weight, outputs in fp16 were 1.3 times as far from 64 bits as their own rounding; it costs 6 %.  The remainder by one mixed
+// multiply-add instead of a conversion and a subtraction: the registers spill, no time gained.)
+constexpr float kWeightBits = 15.f, kOneWeight = 1.f / 32768.f;
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t &two, uint32_t &rest) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto cut = __builtin_amdgcn_cvt_pkrtz(x, y);
+  const auto left = __builtin_amdgcn_cvt_pkrtz(x - (float)cut[0], y - (float)cut[1]);
+  __builtin_memcpy(&two, &cut, 4);
+  __builtin_memcpy(&rest, &left, 4);
+#else
+  (void)x, (void)y, (void)two, (void)rest;
+#endif
+}
+
 // ONE: the column is one step of KT keys, which LDS holds
 template <typename T, typename H, int HD, int KT, bool ONE>  // KT: keys of a softmax step
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(ColumnPlan p, int held) {  // held: keys of a page that LDS holds at a time
@@ -556,21 +571,26 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
             for (int i = 0; i < 16; ++i) o[d][i] *= resc;
         }
         m = mn;
+        const float base = kWeightBits - ref;
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < ST; ++t)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            Pack8 pk;
+            Pack8 pk, rest;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-              const float x = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i], k_scale, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i + 1], k_scale, -ref));
+              const float x = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i], k_scale, base)), y = __builtin_amdgcn_exp2f(fmaf(s[t][8 * u + i + 1], k_scale, base));
               sum += x + y;
-              pk.w[i >> 1] = pack2<f16_t>(x, y);
+              split_weights(x, y, pk.w[i >> 1], rest.w[i >> 1]);
             }
             const uint32_t rows = off + (uint32_t)((t * 32 + 16 * u) * ROW);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = mfma32<f16_t>(lds_tr8(v_lo[d] + rows, v_hi[d] + rows), pk, o[d]);
+            for (int d = 0; d < DT; ++d) {
+              const Pack8 vt = lds_tr8(v_lo[d] + rows, v_hi[d] + rows);
+              o[d] = mfma32<f16_t>(vt, pk, o[d]);
+              o[d] = mfma32<f16_t>(vt, rest, o[d]);
+            }
           }
         l += sum_xor32_f(sum);
       }
@@ -584,7 +604,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void cache_columns_kernel(Co
       for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(o[d][i]));
     most = max_xor32_f(most);
     const float inv = l == 0.f ? 0.f : 1.f / l, norm = __builtin_amdgcn_rcpf(most);
-    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l), v_scale * (inv * most * (1.f / 32767.f)));
+    if (there && hh == 0) p.head[at] = make_float2(l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l * kOneWeight), v_scale * (inv * most * (1.f / 32767.f)));
     {
       // Features 8 j + 4 hh .. of both halves to eight of one lane, then to four lanes with 64 bytes of a row, as the queries were loaded: stores of 16 bytes of 64
       // rows at a time take the caches a cycle for each.

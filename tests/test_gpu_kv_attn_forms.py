@@ -1,6 +1,8 @@
 """The two forms of flash_moba_cache_attn_func, each where it runs: what a caller sees of a value must not depend on how many rows a call has.
 
-Tolerances are those of test_gpu_kv_attn.py, with the bound of the form that the call takes."""
+The row form is held to the bound of test_gpu_kv_attn.py.  Of the form for many rows: a weight goes to the second product as two fp16 numbers, of which the second is what the
+first cuts off (2^-10) and is cut off itself (2^-10 of that), and less than 2^-14 of 2^-15 is a multiple of 2^-39: 2^-20 of a weight and 2^-39 a key of max |v|; sums of n weights and of n products
+are off by n 2^-24 each; a visit's output is off by half a step of 32767ths of its largest feature, which is at most max |v|, and the visits' weights add up to 1: 2^-16 of it."""
 import ctypes
 import math
 
@@ -10,7 +12,7 @@ import torch
 import cache_reference as R
 import flash_moba
 from flash_moba import flash_moba_hip as H
-from test_gpu_kv_attn import call, check, setup
+from test_gpu_kv_attn import CASES, call, check, setup
 from test_gpu_kv_append import cache_struct
 
 gpu = pytest.mark.gpu
@@ -25,9 +27,21 @@ def shares_pages(heads, heads_k, dim, P, lens_q, lens_k, topk, max_pages):
     return H.load_library().fmoba_cache_attn_workspace_bytes(ctypes.byref(a)) > 0
 
 
+def check_form(got, lse, want, want_lse, sizes, parts):
+    if not parts:
+        return check(got, lse, want, want_lse, sizes, False)
+    size, dot, most, count = sizes
+    delta = (got.shape[2] + 8) * 2.0 ** -24 * dot + 2.0 ** -22
+    weights = (2 * delta + 2 * count * 2.0 ** -24 + 2.0 ** -20).t()[:, :, None]
+    tol = want.abs() * torch.finfo(got.dtype).eps / 2 * 1.01 + size * weights + ((2.0 ** -39 * count + 2.0 ** -16 * 1.01) * most).t()[:, :, None] + (2.0 ** -25 if got.dtype == torch.float16 else 0.0)
+    err = (got.float().cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"out {(err - tol).max().item():.3e} over, largest error {err.max().item():.3e}"
+    check(got, lse, want, want_lse, sizes, True)  # (and the log-sum-exp)
+
+
 def check_with_nans(out, lse, want, want_lse, sizes, parts):
     assert torch.equal(out.isnan().cpu(), want.isnan())
-    check(out.nan_to_num(0.0), lse, want.nan_to_num(0.0), want_lse, sizes, parts)
+    check_form(out.nan_to_num(0.0), lse, want.nan_to_num(0.0), want_lse, sizes, parts)
 
 
 @gpu
@@ -50,3 +64,14 @@ def test_a_row_has_the_nans_of_the_values_that_it_sees(heads, heads_k, dim, P, r
     want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [length], table, topk)
     assert bool(want.isnan().any()) and not bool(want.isnan().all())
     check_with_nans(out, lse, want, want_lse, sizes, parts)
+
+
+@gpu
+@pytest.mark.parametrize("held", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,heads_k,dim,P,lens_q,lens_k,topk", CASES)
+def test_every_call_keeps_the_bound_of_its_form(held, dtype, heads, heads_k, dim, P, lens_q, lens_k, topk):
+    cache, table, q, cu = setup(heads, heads_k, dim, P, lens_q, lens_k, dtype, held, seed=21)
+    out, lse = call(cache, table, q, cu, lens_k, topk)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, topk)
+    check_form(out, lse, want, want_lse, sizes, shares_pages(heads, heads_k, dim, P, lens_q, lens_k, topk, len(table[0])))
