@@ -804,9 +804,8 @@ __global__ __launch_bounds__(256, !WEIGHT && LPR == 16 ? 6 : 4) void cache_combi
     }
 #pragma unroll
     for (int o = 1; o < LPR; o <<= 1) l += __shfl_xor(l, o, 64);
-    if (min(least.x, least.y) == kNanPart) {  // (seldom: of the visits that count, once more)
+    if (min(least.x, least.y) == kNanPart && l != 0.f) {  // (seldom: once more; a NaN that a row sees is one whatever its weight, in this form as in the other)
       for (int s = 0; s < n; ++s) {
-        if (__builtin_amdgcn_exp2f(head[s].x - ref) == 0.f) continue;
         const Pack8 again = ld_global16(part + (int64_t)s * D + e);
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] = (int16_t)(again.w[k >> 1] >> (16 * (k & 1))) == kNanPart ? NAN : acc[k];

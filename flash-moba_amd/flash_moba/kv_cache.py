@@ -116,7 +116,8 @@ def flash_moba_cache_attn_func(q, cache, cu_seqlens_q, max_seqlen_q, seqlens_k, 
     Row i of a sequence has position seqlens_k - rows + i.  It sees, up to its position, the keys of its own page and of the
     moba_topk - 1 (at most 63) pages before it whose mean key has the largest product with it, decided as in 64 bits, of equals the
     later page; a product that is NaN or -inf selects nothing, and neither does a table entry that is no page.
-    softmax_scale defaults to head_size ** -0.5.  Rows that see no key produce 0 (and a log-sum-exp of +inf).
+    softmax_scale defaults to head_size ** -0.5.  Rows that see no key produce 0 (and a log-sum-exp of +inf).  A value that is NaN makes
+    its feature NaN for every row that sees it, whatever its weight.
 
     With add_weight=True the part of a row's softmax that a page holds is added to cache.weight (64-bit integers in units of 2^-32, so that
     the sums do not depend on an order), which flash_moba_cache_evict_func chooses by.

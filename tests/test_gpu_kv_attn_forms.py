@@ -75,3 +75,24 @@ def test_every_call_keeps_the_bound_of_its_form(held, dtype, heads, heads_k, dim
     out, lse = call(cache, table, q, cu, lens_k, topk)
     want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, lens_k, table, topk)
     check_form(out, lse, want, want_lse, sizes, shares_pages(heads, heads_k, dim, P, lens_q, lens_k, topk, len(table[0])))
+
+
+@gpu
+@pytest.mark.parametrize("P", [64, 256])
+@pytest.mark.parametrize("rows,parts", [(1, False), (40, False), (1100, True)])
+def test_a_nan_under_a_weight_that_vanishes(rows, parts, P):
+    """The row form multiplies every value that a row sees; where rows share pages a visit whose weights vanish beside the others' counts as much."""
+    dim, length = 64, P * 3 + max(rows, 20)
+    cache, table, q, cu = setup(2, 1, dim, P, [rows], [length], torch.bfloat16, torch.float8_e4m3fn)
+    topk = len(table[0])
+    assert shares_pages(2, 1, dim, P, [rows], [length], topk, topk) == parts
+    q.abs_()
+    q += 0.5
+    cache.k_scale.fill_(0.25)
+    cache.k.copy_(torch.ones(cache.k.shape, device="cuda").to(cache.k.dtype))
+    cache.k[table[0][1]] = torch.full(cache.k.shape[1:], -448.0, device="cuda").to(cache.k.dtype)  # scores 400 and more below the others: their exponential is 0
+    cache.v.view(torch.int8)[table[0][1], 0, 7, 11] = 0x7F
+    out, lse = call(cache, table, q, cu, [length], topk)
+    want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [length], table, topk)
+    assert bool(want[:, :, 11].isnan().all()) and want.isnan().sum().item() == rows * 2
+    check_with_nans(out, lse, want, want_lse, sizes, parts)
