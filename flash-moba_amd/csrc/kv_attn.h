@@ -123,6 +123,7 @@ __device__ __forceinline__ int pick_best(int n, int want, int lane, Hi hi, Lo lo
 // the form for many rows
 constexpr int kColumnCols = 32768;  // pages of a table, at most (a word of bits for each in LDS, and its number in a score)
 size_t column_workspace_bytes(const fmoba_cache_attn_args &a, int cols);
+bool column_grid_fits(const fmoba_cache_attn_args &a, int cols);
 int run_cache_columns(const CacheAttn &c, hipStream_t s);
 
 }  // namespace fmoba

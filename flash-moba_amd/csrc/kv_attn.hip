@@ -406,13 +406,26 @@ __global__ __launch_bounds__(64 * kRowWaves, HD > 128 ? 2 : 4) void cache_attn_r
   }
 }
 
-static int cache_cols(const fmoba_cache_attn_args &a) { return std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages); }
+// pages of a sequence, at most
+static int call_cols(const fmoba_cache_attn_args &a) {
+  return a.max_seqlen_k > 0 && a.max_pages > 0 && a.cache.num_pages > 0 ? std::min(ceil_div(a.max_seqlen_k, a.cache.page_size), a.max_pages) : 0;
+}
 // whether the rows' workgroups score their pages themselves
 static bool own_scores(int cols) { return cols - 1 <= kOwnScores; }
-// Whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own.
+// whether the row form's launches fit their grids
+static int64_t score_turns(const fmoba_cache_attn_args &a) { return ceil_div64((int64_t)std::min(a.max_seqlen_q, a.total_q) * (a.heads / a.cache.heads_k), kScorePairs); }
+static bool has_scores(const fmoba_cache_attn_args &a, int cols) { return !own_scores(cols) && cols > 1 && a.topk > 1; }
+static bool rows_grid_fits(const fmoba_cache_attn_args &a) { return (int64_t)a.total_q * a.heads * 64 * kRowWaves <= UINT32_MAX; }
+static bool scores_grid_fits(const fmoba_cache_attn_args &a, int cols) {
+  return !has_scores(a, cols) || (score_turns(a) <= 65535 && (int64_t)a.batch * a.cache.heads_k <= 65535);
+}
+// Whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own; where the launch grid has no room for the one, the other.
 static bool many_rows(const fmoba_cache_attn_args &a, int cols) {
+  if (cols <= 0 || cols > kColumnCols) return false;
   const int64_t rows = (int64_t)a.total_q * a.heads;
-  return cols > 0 && cols <= kColumnCols && rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
+  const bool shared = rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
+  const bool alone_fits = rows_grid_fits(a) && scores_grid_fits(a, cols), shared_fits = column_grid_fits(a, cols);
+  return shared ? shared_fits || !alone_fits : shared_fits && !alone_fits;
 }
 
 template <typename T, typename H, bool WEIGHT>
@@ -426,14 +439,10 @@ static void launch_rows(const CacheAttn &p, hipStream_t s) {
 }
 
 template <typename T, int HD>
-static int launch_scores(const CacheAttn &p, hipStream_t s) {
+static void launch_scores(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
-  const int64_t pairs = (int64_t)std::min(a.max_seqlen_q, a.total_q) * (a.heads / a.cache.heads_k);
-  const int64_t turns = ceil_div64(pairs, kScorePairs), z = (int64_t)a.batch * a.cache.heads_k;
-  FMOBA_REQUIRE(turns <= 65535 && z <= 65535, "cache_attn: too many rows, or sequences times heads, for the launch grid");
-  const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)turns, (uint32_t)z);
+  const dim3 grid(ceil_div(p.cols - 1, kScorePages), (uint32_t)score_turns(a), (uint32_t)(a.batch * a.cache.heads_k));
   hipLaunchKernelGGL((cache_scores_kernel<T, HD>), grid, dim3(256), 0, s, p);
-  return 0;
 }
 
 template <typename T>
@@ -441,9 +450,8 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.a;
   const int D = a.cache.head_dim;
   if (many_rows(a, p.cols)) return run_cache_columns(p, s);
-  FMOBA_REQUIRE((int64_t)a.total_q * a.heads * 64 * kRowWaves <= UINT32_MAX, "cache_attn: too many rows times heads for the launch grid");
-  if (!own_scores(p.cols) && p.cols > 1 && a.topk > 1) {
-    if (int rc = D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s)) return rc;
+  if (has_scores(a, p.cols)) {
+    D <= 64 ? launch_scores<T, 64>(p, s) : D <= 128 ? launch_scores<T, 128>(p, s) : launch_scores<T, 256>(p, s);
     FMOBA_LAUNCH_CHECK("cache_scores_kernel");
   }
   if (a.cache.format == FMOBA_CACHE_E4M3)
@@ -458,14 +466,14 @@ static int run_cache_attn(const CacheAttn &p, hipStream_t s) {
 
 extern "C" size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *a) {
   using namespace fmoba;
-  if (a == nullptr || a->total_q <= 0 || a->heads <= 0 || a->max_seqlen_k <= 0 || a->max_pages <= 0 || a->cache.page_size <= 0) return 0;
-  const int cols = a->cache.num_pages > 0 ? cache_cols(*a) : 0;
+  if (a == nullptr || a->total_q <= 0 || a->heads <= 0 || a->cache.heads_k <= 0 || a->cache.page_size <= 0) return 0;
+  const int cols = call_cols(*a);
   if (cols == 0) return 0;
   if (many_rows(*a, cols)) return column_workspace_bytes(*a, cols);
   return own_scores(cols) ? 0 : (size_t)a->total_q * a->heads * cols * 8;
 }
 
-extern "C" int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream) {
+extern "C" int fmoba_cache_attn_check(const fmoba_cache_attn_args *a) {
   using namespace fmoba;
   FMOBA_REQUIRE(a != nullptr, "cache_attn: null args");
   FMOBA_CHECK_CACHE(a->cache);
@@ -480,9 +488,23 @@ extern "C" int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream) {
   FMOBA_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->out) % 16) == 0, "cache_attn: q and out must be 16-byte aligned");
   const size_t need = fmoba_cache_attn_workspace_bytes(a);
   FMOBA_REQUIRE(a->workspace_bytes >= need && (a->workspace || need == 0) && (uintptr_t)a->workspace % 256 == 0, "cache_attn: workspace too small (%zu < %zu) or not 256-byte aligned", a->workspace_bytes, need);
+  const int cols = call_cols(*a);
+  if (many_rows(*a, cols)) {
+    FMOBA_REQUIRE(column_grid_fits(*a, cols), "cache_attn: too many sequences times pages for the launch grid");
+  } else {
+    FMOBA_REQUIRE(rows_grid_fits(*a), "cache_attn: too many rows times heads for the launch grid");
+    FMOBA_REQUIRE(scores_grid_fits(*a, cols), "cache_attn: too many rows, or sequences times heads, for the launch grid");
+  }
+  return 0;
+}
+
+extern "C" int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream) {
+  using namespace fmoba;
+  if (int rc = fmoba_cache_attn_check(a)) return rc;
+  if (a->total_q == 0) return 0;
   CacheAttn p{};
   p.a = *a;
-  p.cols = a->max_seqlen_k > 0 && a->max_pages > 0 && a->cache.num_pages > 0 ? cache_cols(*a) : 0;
+  p.cols = call_cols(*a);
   p.key_hi = reinterpret_cast<uint32_t *>(a->workspace);
   p.key_lo = p.key_hi + (size_t)a->total_q * a->heads * p.cols;
   return a->cache.dtype == FMOBA_DTYPE_BF16 ? run_cache_attn<bf16_t>(p, (hipStream_t)stream) : run_cache_attn<f16_t>(p, (hipStream_t)stream);

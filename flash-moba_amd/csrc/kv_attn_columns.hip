@@ -864,6 +864,11 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   p.steps = a.cache.page_size / p.step_keys;
   if (pages * p.steps > kCombineSlots) p.steps = 1, p.step_keys = a.cache.page_size;
   p.slots = pages * p.steps;
+  // Workgroups of a page: four turns of rows each, if rows choose evenly, and an odd number: the last ones of a late page, which few rows see, have nothing to
+  // do, and would otherwise come to the same shader engines for every page (8191 tokens, 16 heads: 223 us even, 201 odd; 8192, 16 over 2 heads: 380 and 254;
+  // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
+  const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, cols) / cols;
+  p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
   ColumnSizes z;
   z.sel = up(rowheads * p.topk4 * 4);
   z.bits = up((size_t)a.heads * p.blocks * cols * 4);
@@ -876,6 +881,12 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
 size_t column_workspace_bytes(const fmoba_cache_attn_args &a, int cols) {
   ColumnPlan p{};
   return column_sizes(a, cols, p).total;
+}
+
+bool column_grid_fits(const fmoba_cache_attn_args &a, int cols) {
+  ColumnPlan p{};
+  column_sizes(a, cols, p);
+  return (int64_t)a.batch * a.cache.heads_k * cols * p.steps * p.parts * 256 <= UINT32_MAX;
 }
 
 template <typename K>
@@ -959,12 +970,6 @@ int run_cache_columns(const CacheAttn &c, hipStream_t s) {
   p.scores = reinterpret_cast<float *>(at), at += z.scores;
   p.head = reinterpret_cast<float2 *>(at), at += z.head;
   p.part = reinterpret_cast<uint16_t *>(at);
-  // Workgroups of a page: four turns of rows each, if rows choose evenly, and an odd number: the last ones of a late page, which few rows see, have nothing to
-  // do, and would otherwise come to the same shader engines for every page (8191 tokens, 16 heads: 223 us even, 201 odd; 8192, 16 over 2 heads: 380 and 254;
-  // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
-  const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, c.cols) / c.cols;
-  p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
-  FMOBA_REQUIRE((int64_t)a.batch * a.cache.heads_k * c.cols * p.steps * p.parts * 256 <= UINT32_MAX, "cache_attn: too many sequences times pages for the launch grid");
   return a.cache.dtype == FMOBA_DTYPE_BF16 ? run_columns_as<bf16_t>(p, s) : run_columns_as<f16_t>(p, s);
 }
 

@@ -162,6 +162,7 @@ EXPORTS = {
     "fmoba_cache_append_turned": (c_i32, [ctypes.POINTER(CacheAppendArgs), ctypes.POINTER(RotaryArgs), c_vp]),
     "fmoba_cache_attn_workspace_bytes": (c_sz, [ctypes.POINTER(CacheAttnArgs)]),
     "fmoba_cache_attn": (c_i32, [ctypes.POINTER(CacheAttnArgs), c_vp]),
+    "fmoba_cache_attn_check": (c_i32, [ctypes.POINTER(CacheAttnArgs)]),
     "fmoba_cache_evict_workspace_bytes": (c_sz, [c_i32, c_i32]),
     "fmoba_cache_evict": (c_i32, [ctypes.POINTER(CacheEvictArgs), c_vp]),
 }

@@ -386,6 +386,8 @@ typedef struct {
 } fmoba_cache_attn_args;
 size_t fmoba_cache_attn_workspace_bytes(const fmoba_cache_attn_args *a);
 int fmoba_cache_attn(const fmoba_cache_attn_args *a, void *stream);
+/* 0 if fmoba_cache_attn would launch this call; else what it would refuse (what stands in the buffers is not looked at).  For callers that change the cache in between. */
+int fmoba_cache_attn_check(const fmoba_cache_attn_args *a);
 
 /* Which pages a sequence keeps when it has more than `keep`: its first `sink`, its last `recent` (one at least: the page that is being filled), and of the
  * others those with the most weight, summed over heads; of equals the first.  Their order stays.  new_table and freed (batch, max_pages), dense: pages
