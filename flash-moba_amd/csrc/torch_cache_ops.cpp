@@ -269,8 +269,14 @@ void check_attn(const Tensor &q, const Cache &c, const AttnForm &f) {
   require(!f.add_weight || c.weight.defined(), "the cache keeps no weight");
 }
 
-std::pair<Tensor, Tensor> attn_raw(const Tensor &q_in, const Cache &c, const Tensor &cu, const Tensor &seqlens_k, const Tensor &table, const AttnForm &f) {
+// A call that has passed every check, with all that it needs: nothing is refused any more when it is launched.
+struct AttnCall {
   fmoba_cache_attn_args a{};
+  Tensor q, out, lse, ws;
+};
+AttnCall attn_call(const Tensor &q_in, const Cache &c, const Tensor &cu, const Tensor &seqlens_k, const Tensor &table, const AttnForm &f) {
+  AttnCall call;
+  fmoba_cache_attn_args &a = call.a;
   a.cache = cache_view(c);
   const at::Device dev = c.k.device();
   check_attn(q_in, c, f);
@@ -278,18 +284,27 @@ std::pair<Tensor, Tensor> attn_raw(const Tensor &q_in, const Cache &c, const Ten
   require(cu.defined(), "cu_seqlens must be given");
   const c10::DeviceGuard guard(dev);
   check_device(dev.index());
-  const Tensor q = as_rows(q_in);
-  const Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  a.q = q.data_ptr(), a.out = out.data_ptr(), a.softmax_lse = lse.data_ptr<float>();
+  const Tensor q = call.q = as_rows(q_in);
+  const Tensor out = call.out = at::empty(q.sizes(), q.options());
+  call.lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  a.q = q.data_ptr(), a.out = out.data_ptr(), a.softmax_lse = call.lse.data_ptr<float>();
   a.cu_seqlens_q = cu.data_ptr<int32_t>(), a.seqlens_k = seqlens_k.data_ptr<int32_t>(), a.block_table = table.data_ptr<int32_t>();
   a.q_row_stride = q.stride(0), a.q_head_stride = q.stride(1), a.o_row_stride = out.stride(0), a.o_head_stride = out.stride(1), a.table_stride = table.stride(0);
   a.total_q = q.size(0), a.heads = q.size(1), a.max_seqlen_q = f.max_q, a.max_seqlen_k = f.max_k, a.max_pages = table.size(1), a.topk = f.topk, a.add_weight = f.add_weight;
   a.softmax_scale = static_cast<float>(f.scale ? *f.scale : std::pow(static_cast<double>(q.size(2)), -0.5));
   a.workspace_bytes = fmoba_cache_attn_workspace_bytes(&a);
-  const Tensor ws = bytes_like(q, a.workspace_bytes + 255);
-  a.workspace = reinterpret_cast<void *>(up256(reinterpret_cast<size_t>(ws.data_ptr())));
-  check(fmoba_cache_attn(&a, current_stream(c.k)));
-  return {out, lse};
+  call.ws = bytes_like(q, a.workspace_bytes + 255);
+  a.workspace = reinterpret_cast<void *>(up256(reinterpret_cast<size_t>(call.ws.data_ptr())));
+  check(fmoba_cache_attn_check(&a));
+  return call;
+}
+std::pair<Tensor, Tensor> launch(const AttnCall &call) {
+  const c10::DeviceGuard guard(call.q.device());
+  check(fmoba_cache_attn(&call.a, current_stream(call.q)));
+  return {call.out, call.lse};
+}
+std::pair<Tensor, Tensor> attn_raw(const Tensor &q, const Cache &c, const Tensor &cu, const Tensor &seqlens_k, const Tensor &table, const AttnForm &f) {
+  return launch(attn_call(q, c, cu, seqlens_k, table, f));
 }
 
 std::vector<Tensor> evict_raw(const Tensor &weight, const Tensor &seqlens_k, const Tensor &table, int64_t page_size, int64_t keep, int64_t sink, int64_t recent) {
@@ -378,23 +393,25 @@ py::object cache_step(const py::handle &hq, const py::handle &hk, const py::hand
   {
     py::gil_scoped_release nogil;
     at::AutoDispatchBelowADInplaceOrView below;
-    Tensor q = unpack(hq), k = unpack(hk);
+    Tensor q = unpack(hq), k = unpack(hk), q_rows;
     const AttnForm attn{max_q, max_k, topk, scale, add_weight};
-    cache_view(c);  // (what the attention would refuse is refused before the cache changes)
+    cache_view(c);
     check_attn(q, c, attn);
     check_inference({&k});
     if (turned) check_rotary(q, k, unpack(hp), f);
-    if (turned && max_q <= FMOBA_TURN_ROWS) {
-      Tensor pos;
-      fmoba_rotary_args a = rotary_args(q, unpack(hp), f, pos);
-      const Tensor qo = rotary_queries(a, q);
-      append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable), &a);
-      q = qo;
-    } else {
-      if (turned) std::tie(q, k) = turn(q, k, unpack(hp), f);
-      append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable));
+    // (the attention is checked, and has its memory, before the cache changes: a step that is refused can be made again)
+    const bool in_append = turned && max_q <= FMOBA_TURN_ROWS;
+    Tensor pos;
+    fmoba_rotary_args a{};
+    if (in_append) {
+      a = rotary_args(q, unpack(hp), f, pos);
+      q_rows = q, q = rotary_queries(a, q_rows);
+    } else if (turned) {
+      std::tie(q, k) = turn(q, k, unpack(hp), f);
     }
-    r = attn_raw(q, c, unpack(hcu), unpack(hlen), unpack(htable), attn);
+    const AttnCall call = attn_call(q, c, unpack(hcu), unpack(hlen), unpack(htable), attn);
+    append_raw(c, k, unpack(hv), unpack(hcu), max_q, unpack(hlen), unpack(htable), in_append ? &a : nullptr);
+    r = launch(call);
   }
   return py::make_tuple(wrap(r.first), wrap(r.second));
 }

@@ -1,4 +1,4 @@
-"""What one form of the attention has no launch grid for takes the other, and what neither has is known before anything runs."""
+"""A serving step that is refused leaves the cache as it was, and what one form of the attention has no launch grid for takes the other."""
 import ctypes
 
 import pytest
@@ -42,6 +42,68 @@ def test_the_check_says_what_the_call_would():
     assert ok(**big) == 0
     # and 300000 rows of 64 heads, which are 2^33 threads of a workgroup each: shared pages, though a page is selected twice on average
     assert ok(batch=1, heads_k=64, heads=64, total_q=300000, max_seqlen_q=300000, max_seqlen_k=64 * 30000, max_pages=30000, topk=1) == 0
+
+
+def step_inputs(batch, rows, heads, cols, positions):
+    """Sequences of cols pages of 64, of which the table has the last page only."""
+    P, dim = 64, 16
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = flash_moba.MobaKVCache.allocate(4, P, 1, dim)
+    cache.k_sum.normal_()
+    cache.weight.random_(0, 1 << 40)
+    table = torch.full((batch, cols), -1, **i32)
+    table[0, -1] = 2
+    q = torch.randn((batch * rows, heads, dim), device="cuda", dtype=torch.bfloat16)
+    k = torch.randn((batch * rows, 1, dim), device="cuda", dtype=torch.bfloat16)
+    cu = torch.arange(batch + 1, **i32) * rows
+    lens = torch.full((batch,), cols * P - 5, **i32)
+    pos = torch.arange(batch * rows, device="cuda") if positions else None
+    return cache, (q, k, k, cache, cu, rows, lens, cols * P, table, 1), dict(positions=pos, add_weight=True)
+
+
+def unchanged(cache, before):
+    return all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(cache, before))
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,positions", [(16, 64, False), (16, 64, True), (8, 128, True)])
+def test_a_step_refused_for_its_launch_grid_leaves_the_cache(rows, heads, positions):
+    cache, args, kw = step_inputs(8400, rows, heads, 2000, positions)
+    before = [t.clone() for t in cache]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="launch grid"):
+            flash_moba.flash_moba_with_cache_func(*args, **kw)
+    torch.cuda.synchronize()
+    assert unchanged(cache, before)
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,positions", [(8192, 64, False), (4096, 64, True)])
+def test_a_step_without_memory_leaves_the_cache_and_can_be_made_again(rows, heads, positions):
+    cache, args, kw = step_inputs(1, rows, heads, 200, positions)
+    args = args[:-1] + (64,)  # (top-k: a visit has a place in the workspace)
+    flash_moba.flash_moba_cache_append_func(cache, args[1][:30], args[1][:30], torch.tensor([0, 30], dtype=torch.int32, device="cuda"), 30,
+                                            torch.tensor([200 * 64 - 20], dtype=torch.int32, device="cuda"), args[8])
+    before = [t.clone() for t in cache]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (96 << 20)) / total)
+        with pytest.raises(torch.OutOfMemoryError):
+            flash_moba.flash_moba_with_cache_func(*args, **kw)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    torch.cuda.synchronize()
+    assert unchanged(cache, before)
+    twin = flash_moba.MobaKVCache(*[t.clone() for t in cache])
+    out = flash_moba.flash_moba_with_cache_func(*args, **kw)
+    q, k = args[:2]
+    if positions:
+        q, k = flash_moba.flash_moba_rotary_func(q, k, kw["positions"])
+    flash_moba.flash_moba_cache_append_func(twin, k, args[2], *args[4:7], args[8])
+    assert torch.equal(out, flash_moba.flash_moba_cache_attn_func(q, twin, *args[4:], add_weight=True))
+    assert unchanged(cache, twin)
 
 
 @gpu
