@@ -414,14 +414,14 @@ static int call_cols(const fmoba_cache_attn_args &a) {
 static bool own_scores(int cols) { return cols - 1 <= kOwnScores; }
 // whether the row form's launches fit their grids
 static int64_t score_turns(const fmoba_cache_attn_args &a) { return ceil_div64((int64_t)std::min(a.max_seqlen_q, a.total_q) * (a.heads / a.cache.heads_k), kScorePairs); }
-static bool has_scores(const fmoba_cache_attn_args &a, int cols) { return !own_scores(cols) && cols > 1 && a.topk > 1; }
+static bool has_scores(const fmoba_cache_attn_args &a, int cols) { return !own_scores(cols) && cols > 1 && a.topk > 1 && a.max_seqlen_q > 0; }
 static bool rows_grid_fits(const fmoba_cache_attn_args &a) { return (int64_t)a.total_q * a.heads * 64 * kRowWaves <= UINT32_MAX; }
 static bool scores_grid_fits(const fmoba_cache_attn_args &a, int cols) {
   return !has_scores(a, cols) || (score_turns(a) <= 65535 && (int64_t)a.batch * a.cache.heads_k <= 65535);
 }
 // Whether rows share the pages that they select (kv_attn_columns.hip), or every (row, head) reads its own; where the launch grid has no room for the one, the other.
 static bool many_rows(const fmoba_cache_attn_args &a, int cols) {
-  if (cols <= 0 || cols > kColumnCols) return false;
+  if (cols <= 0 || cols > kColumnCols || a.max_seqlen_q <= 0) return false;  // (no row of any sequence, rows that are padding: nothing to launch but what writes their outputs)
   const int64_t rows = (int64_t)a.total_q * a.heads;
   const bool shared = rows >= kColumnRowsLeast && rows * std::min(a.topk, cols) >= (own_scores(cols) ? kVisitsOwn : kVisits) * (int64_t)a.batch * a.cache.heads_k * cols;
   const bool alone_fits = rows_grid_fits(a) && scores_grid_fits(a, cols), shared_fits = column_grid_fits(a, cols);

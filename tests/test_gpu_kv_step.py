@@ -126,3 +126,19 @@ def test_where_a_workgroup_a_page_does_not_fit_the_grid_rows_read_their_own():
         length -= 1 if t == 300001 else 0
         want, want_lse, _, sizes = R.attention(s, q[t:t + 1].cpu(), [0, 1], [length], [table[-1].tolist()], 64)
         check(out[t:t + 1], lse[:, t:t + 1], want, want_lse, sizes, False)
+
+
+@gpu
+@pytest.mark.parametrize("pages", [6, 2100])
+@pytest.mark.parametrize("rows", [3, 2100])
+def test_rows_that_are_all_padding(rows, pages):
+    """No sequence has a row, and max_seqlen_q says so: both forms, and the scores' own launch, would have an empty grid."""
+    P, dim = 64, 32
+    cache, table, q, _ = setup(4, 2, dim, P, [rows], [P * pages], torch.bfloat16, torch.int8)
+    before = [t.clone() for t in cache]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    args = (torch.tensor([0, 0], **i32), 0, torch.tensor([P * pages], **i32), P * pages, torch.tensor(table, **i32), 3)
+    out, lse = flash_moba.flash_moba_cache_attn_func(q, cache, *args, return_lse=True)
+    assert bool((out == 0).all()) and bool(torch.isposinf(lse).all())
+    out, lse = flash_moba.flash_moba_with_cache_func(q, q[:, :2], q[:, :2], cache, *args, positions=torch.arange(rows, device="cuda"), add_weight=True, return_lse=True)
+    assert bool((out == 0).all()) and bool(torch.isposinf(lse).all()) and unchanged(cache, before)
