@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   const int tiles = (nscore + 31) / 32, per_group = (tiles + kGateGroups - 1) / kGateGroups;
   const uint32_t number = (1u << page_bits) - 1u;
   float top[kGateGroups], q2 = 0.f, mean2 = 0.f;
+  uint32_t q_bits = 0u;  // 0: a row of zeros
   if (nscore > 0) {
     Pack8 q[KS], k[KS];
     bool there = false;
@@ -153,6 +154,9 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q2 = add_squares<T>(q[ks], q2);
     q2 = sum_xor32_f(q2);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q_bits |= (q[ks].w[0] | q[ks].w[1] | q[ks].w[2] | q[ks].w[3]) & 0x7fff7fffu;
+    q_bits |= (uint32_t)__shfl_xor((int)q_bits, 32, 64);
     for (int g = wave; g < kGateGroups; g += nw) {  // the groups of a wave
       const int end = min((g + 1) * per_group, tiles);
       float best = -INFINITY;
@@ -193,10 +197,13 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   if (wave == 0) {
     float err = 0.f;
     // A score of D products in 32 bits, in whatever order and with whatever is cut off between the steps of the matrix unit, is off by less than D 2^-23 of
-    // |q| |mean| (and these by less than 2^-10): scores further apart than twice that are in the order of 64 bits.
+    // |q| |mean| (and these by less than 2^-10): scores further apart than twice that are in the order of 64 bits.  What is too small for 32 bits is lost beside that: up to 2^-126 of an
+    // element, a product and a sum, whatever of it the matrix unit keeps, and of the whole where the page's number is in its place; of a square up to that of the least normal element.
     if (nscore > 0) {
       for (int w = 0; w < nw; ++w) mean2 = fmaxf(mean2, sMean2[w]);
-      err = (float)D * (1.192092896e-7f * 1.002f) * sqrtf(q2) * sqrtf(mean2);
+      const float lost = (float)(D + 1) * 0x1p-126f, lost2 = std::is_same<T, bf16_t>::value ? lost : (float)D * 0x1p-28f;
+      const float q_size = sqrtf(q2 + lost2), mean_size = sqrtf(mean2 + lost2);
+      err = (float)D * (1.192092896e-7f * 1.002f) * q_size * mean_size + 2.f * lost * (1.f + q_size + mean_size);
     }
 #pragma unroll
     for (int g = 0; g < kGateGroups; ++g) top[g] = nscore > 0 ? sTop[g][lane] : -INFINITY;
@@ -237,12 +244,11 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
         out = best;
       }
     }
-    // Rows whose cut is too close for 32 bits.  (The page's number in a score: less than 2^(page_bits - 23) of it.  Products of zeros are equal, and of them the
+    // Rows whose cut is too close for 32 bits.  (The page's number in a score: less than 2^(page_bits - 23) of it.  The scores of a row of zeros are equal, and of them the
     // later pages came first.)
     const float near = 2.f * err + ldexpf(2.f * fmaxf(fabsf(in), fabsf(out)), page_bits - 23);
-    const bool zeros = err == 0.f && ((__float_as_uint(in) | __float_as_uint(out)) & ~number) == 0u;
-    const bool sized = err < 1e30f && (err > 0.f || zeros);  // (else sizes overflow or vanish, or are no numbers: all pages decide in 64 bits)
-    const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && !zeros && !(in - out > near)));
+    const bool sized = err < 1e30f;  // (else sizes overflow, or are no numbers: all pages decide in 64 bits)
+    const bool unsure = li < rows && want > 0 && (!sized || (out > -INFINITY && q_bits != 0u && !(in - out > near)));
     if (hh == 0) sPicked[li] = picked, sLow[li] = in - near;
     const uint32_t unsure_rows = (uint32_t)__ballot(unsure), all_rows = (uint32_t)__ballot(!sized);
     if (lane == 0) sUnsure = unsure_rows, sAll = all_rows;

@@ -96,3 +96,41 @@ def test_a_nan_under_a_weight_that_vanishes(rows, parts, P):
     want, want_lse, _, sizes = R.attention(R.state(cache), q.cpu(), cu, [length], table, topk)
     assert bool(want[:, :, 11].isnan().all()) and want.isnan().sum().item() == rows * 2
     check_with_nans(out, lse, want, want_lse, sizes, parts)
+
+
+@gpu
+@pytest.mark.parametrize("rows,parts", [(3, False), (1100, True)])
+@pytest.mark.parametrize("power", [-62, -66, -70, -90])
+def test_scores_too_small_for_32_bits_are_decided_as_in_64(power, rows, parts):
+    """Queries and means whose products are subnormal in 32 bits, or nothing: every page has another score all the same."""
+    P, dim, n, topk = 64, 64, 40, 5
+    cache, table, q, cu = setup(2, 1, dim, P, [rows], [P * n], torch.bfloat16, torch.float8_e4m3fn)
+    assert shares_pages(2, 1, dim, P, [rows], [P * n], topk, len(table[0])) == parts
+    q *= 2.0 ** power
+    cache.k_mean.mul_(2.0 ** power)
+    q[-1, 1] = 0  # (equal scores: the later pages)
+    assert bool((q[:-1] != 0).any(-1).all())
+    w = cache.weight.clone()
+    out, lse = call(cache, table, q, cu, [P * n], topk, add_weight=True)
+    want, want_lse, weight, sizes = R.attention(R.state(cache), q.cpu(), cu, [P * n], table, topk)
+    check_form(out, lse, want, want_lse, sizes, parts)
+    assert torch.equal((cache.weight > w).cpu(), weight > 0)
+
+
+@gpu
+@pytest.mark.parametrize("rows,parts", [(3, False), (1100, True)])
+def test_subnormal_features_count(rows, parts):
+    """fp16: the only normal feature of a row says the opposite of the others, which are subnormal."""
+    P, dim, n, topk = 64, 64, 40, 5
+    cache, table, q, cu = setup(2, 1, dim, P, [rows], [P * n], torch.float16, torch.int8)
+    assert shares_pages(2, 1, dim, P, [rows], [P * n], topk, len(table[0])) == parts
+    q[:] = 2.0 ** -15
+    q[:, :, 0] = 2.0 ** -14
+    for c in range(n):
+        cache.k_mean[table[0][c]] = (c - 16) * 2.0 ** -6
+        cache.k_mean[table[0][c], :, 0] = (16 - c) * 2.0 ** -6
+    w = cache.weight.clone()
+    out, lse = call(cache, table, q, cu, [P * n], topk, add_weight=True)
+    want, want_lse, weight, sizes = R.attention(R.state(cache), q.cpu(), cu, [P * n], table, topk)
+    check_form(out, lse, want, want_lse, sizes, parts)
+    assert torch.equal((cache.weight > w).cpu(), weight > 0)
