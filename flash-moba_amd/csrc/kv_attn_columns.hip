@@ -22,7 +22,7 @@ struct ColumnPlan {
   CacheAttn c;
   int32_t *sel;      // [(row, head)][topk4]: pages, -1 behind them
   uint32_t *bits;    // [key head][block of 32 rows][head of the group][page]: a bit for each of the rows
-  float *scores;     // [block of 32 rows][head][32 rows][half of the wave][slot], where LDS does not hold them
+  float *scores;     // [workgroup of the gate][32 rows][half of the wave][slot], where LDS does not hold them
   float2 *head;      // [(row, head)][slots]: log2 of a visit's sum of weights, and what its output has to be multiplied by
   uint16_t *part;    // [(row, head)][slots][head_dim]: that output, int16; kNanPart is a NaN
   int32_t topk4;     // topk, rounded up to a multiple of four
@@ -30,6 +30,8 @@ struct ColumnPlan {
   int32_t step_keys;
   int32_t slots;     // visits of a row, at most: pages times steps
   int32_t blocks;    // blocks of 32 rows, all sequences (block_of)
+  int32_t row_blocks;  // of a sequence, at most
+  int32_t gates;     // workgroups of the gate, where LDS does not hold their scores
   int32_t tiles;     // words of a page in a sequence, at most: its blocks times the heads of a group
   int32_t parts;     // workgroups of a page
 };
@@ -46,6 +48,9 @@ __device__ __forceinline__ int64_t block_of(int q0, int b) { return q0 / kTileRo
 // best (the other waves wait); LDS has room for three of them a compute unit.  Page numbers a tile ahead and means fetched 64 bytes of a row at a time changed nothing.
 // ------------------------------------------------------------------------------------
 constexpr int kGateCols = 1024;   // pages whose scores of 32 rows LDS holds (135 KB); beyond, in the workspace (258 pages, whole calls: 94 us in LDS, 156 in the workspace)
+// Bytes of the workspace for them, about: of a whole number of workgroups a compute unit (1 of tables of 32768 pages, 15 of 2048).  409 workgroups instead of 256, 1024 rows, 16 heads, 20000
+// pages: 3710 and 3210 us; 1677, 2048 rows, 5000 pages: 1086, a workgroup for each of the 2048 blocks 1140.
+constexpr int64_t kGateScores = int64_t(1) << 30;
 constexpr int kGateGroups = 8;
 
 // row . mean of a page in 64 bits, by 16 lanes (four pages a wave)
@@ -96,8 +101,10 @@ __device__ __forceinline__ int gate_half(int c) { return (c >> 2) & 1; }
 __device__ __forceinline__ int gate_slot(int c) { return (c >> 5) * 16 + ((c >> 3) & 3) * 4 + (c & 3); }
 __host__ __device__ __forceinline__ int gate_stride(int cols) { return (cols + 31) / 32 * 16 + 4; }  // floats of a lane (four more: 16 lanes' reads of 16 bytes meet all banks once)
 
+static int64_t gate_score_bytes(int cols) { return (int64_t)kTileRows * 2 * gate_stride(cols) * 4; }
+// 32 rows of a head: block rb of sequence b.  scores: (without LDS) a place for them that is no other workgroup's
 template <typename T, int HD, bool LDS>
-__global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_bits) {
+__device__ __forceinline__ void gate_block(const ColumnPlan &p, int page_bits, int rb, int h, int b, float *scores) {
   constexpr int KS = HD / 16;
   __shared__ float sTop[kGateGroups][64], sMean2[4], sLow[kTileRows];
   __shared__ int sPicked[kTileRows], sCandidate[4][64];
@@ -106,7 +113,7 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   const fmoba_cache_attn_args &a = p.c.a;
   const int D = a.cache.head_dim, P = a.cache.page_size, G = a.heads / a.cache.heads_k;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, li = lane & 31;
-  const int rb = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / G, cols = p.c.cols;
+  const int hk = h / G, cols = p.c.cols;
   const int q0 = a.cu_seqlens_q[b], q1 = a.cu_seqlens_q[b + 1], len = a.seqlens_k[b];
   const int R = min(min(q1, a.total_q) - q0, a.max_seqlen_q), row0 = rb * kTileRows;
   if (q0 < 0 || row0 >= R) return;
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   const int nscore = last < 0 || a.topk <= 1 ? 0 : min(last / P, cols - 1);                // that any of the rows can select beside its own
   const int32_t *table = a.block_table + (int64_t)b * a.table_stride;
   const int stride = gate_stride(cols);
-  float *scores = LDS ? gate_smem : p.scores + ((block_of(q0, b) + rb) * a.heads + h) * kTileRows * 2 * stride;
+  if (LDS) scores = gate_smem;
   uint32_t *sBits = reinterpret_cast<uint32_t *>(gate_smem + (LDS ? kTileRows * 2 * stride : 0));
   float *mine = scores + (li * 2 + hh) * stride;
   const uint16_t *qh = reinterpret_cast<const uint16_t *>(a.q) + (int64_t)(q0 + row0) * a.q_row_stride + (int64_t)h * a.q_head_stride;
@@ -346,6 +353,25 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
   __syncthreads();
   uint32_t *bits = p.bits + (((int64_t)hk * p.blocks + block_of(q0, b) + rb) * G + (h - hk * G)) * cols;
   for (int i = tid; i < npages; i += blockDim.x) bits[i] = sBits[i];
+}
+
+// A workgroup a block where LDS holds its scores; else as many workgroups as the device runs at a time, each with a place in the workspace that its blocks share one after the other: for
+// rows of a long prompt, all of whose scores together are rows times pages.  Every other head's blocks come from the last on, so that a workgroup has early and late ones.
+template <typename T, int HD, bool LDS>
+__global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_bits) {
+  if constexpr (LDS) {
+    gate_block<T, HD, true>(p, page_bits, blockIdx.x, blockIdx.y, blockIdx.z, nullptr);
+  } else {
+    const int heads = p.c.a.heads;
+    const int64_t all = (int64_t)p.row_blocks * heads * p.c.a.batch;
+    float *scores = p.scores + (int64_t)blockIdx.x * kTileRows * 2 * gate_stride(p.c.cols);
+    for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+      const int64_t nth = i / p.row_blocks;  // head of a sequence
+      const int rb = (int)(i - nth * p.row_blocks), b = (int)(nth / heads), h = (int)(nth - (int64_t)b * heads);
+      if (i != blockIdx.x) __syncthreads();  // (what the block before has in LDS and in the workspace is read)
+      gate_block<T, HD, false>(p, page_bits, nth & 1 ? p.row_blocks - 1 - rb : rb, h, b, scores);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------
@@ -860,7 +886,9 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   const size_t rowheads = (size_t)a.total_q * a.heads;
   p.topk4 = (a.topk + 3) / 4 * 4;
   p.blocks = a.total_q / kTileRows + a.batch;
-  p.tiles = ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows) * (a.heads / a.cache.heads_k);
+  p.row_blocks = ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows);
+  p.tiles = p.row_blocks * (a.heads / a.cache.heads_k);
+  p.gates = (int)std::min<int64_t>((int64_t)p.row_blocks * a.heads * a.batch, std::max<int64_t>(kGateScores / gate_score_bytes(cols) / 256, 1) * 256);
   // Pages of one step (64 keys, or 128 of heads up to 128, whose scores of a row fit the registers): nothing before it has to be scaled for, and its next rows can be on their way.  Larger pages are
   // several columns of one step each, as far as the combine has places for a row's visits; else one column of many steps, whose keys come into LDS 64 at a time, again for every turn,
   // where two workgroups do not find room for all.  (8191 tokens, 16 over 4 heads of 128, pages of 256 keys, four a row: 260 us in two steps, 526 in one column; of 512, two a row: 245 and 670;
@@ -878,7 +906,7 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   ColumnSizes z;
   z.sel = up(rowheads * p.topk4 * 4);
   z.bits = up((size_t)a.heads * p.blocks * cols * 4);
-  z.scores = cols > kGateCols ? up((size_t)a.heads * p.blocks * kTileRows * 2 * gate_stride(cols) * 4) : 0;
+  z.scores = cols > kGateCols ? up(p.gates * gate_score_bytes(cols)) : 0;
   z.head = up(rowheads * p.slots * 8);
   z.part = up(rowheads * p.slots * a.cache.head_dim * 2);
   z.total = z.sel + z.bits + z.scores + z.head + z.part;
@@ -907,8 +935,8 @@ static int with_lds(K kern, size_t bytes, const char *what) {
 template <typename T, int HD>
 static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   const fmoba_cache_attn_args &a = p.c.a;
-  const dim3 grid(ceil_div(std::min(a.max_seqlen_q, a.total_q), kTileRows), a.heads, a.batch);
   const bool lds = p.c.cols <= kGateCols;
+  const dim3 grid = lds ? dim3(p.row_blocks, a.heads, a.batch) : dim3(p.gates);
   const size_t bytes = ((size_t)p.c.cols + (lds ? (size_t)kTileRows * 2 * gate_stride(p.c.cols) : 0)) * 4;
   int page_bits = 1;
   while ((1 << page_bits) < p.c.cols) ++page_bits;

@@ -142,3 +142,39 @@ def test_rows_that_are_all_padding(rows, pages):
     assert bool((out == 0).all()) and bool(torch.isposinf(lse).all())
     out, lse = flash_moba.flash_moba_with_cache_func(q, q[:, :2], q[:, :2], cache, *args, positions=torch.arange(rows, device="cuda"), add_weight=True, return_lse=True)
     assert bool((out == 0).all()) and bool(torch.isposinf(lse).all()) and unchanged(cache, before)
+
+
+def test_scratch_of_many_rows_is_bounded_by_what_rows_leave_behind():
+    """The gate's scores are a gigabyte, however many rows there are: what a prompt needs more are its visits and a bit for every row and page."""
+    lib = H.load_library()
+
+    def scratch(rows, length, batch=1):
+        pages = length // 128
+        a = attn_args(cache_struct(page_size=128, heads_k=8, head_dim=128), batch=batch, heads=32, total_q=rows, max_seqlen_q=rows // batch, max_seqlen_k=length, max_pages=pages, topk=8)
+        visits = rows * 32 * (8 * (128 * 2 + 8) + 8 * 4)
+        bits = 32 * (rows // 32 + batch) * pages * 4
+        return lib.fmoba_cache_attn_workspace_bytes(ctypes.byref(a)) - visits - bits
+
+    for rows, length, batch in ((262144, 262144, 1), (524288, 524288, 1), (8192, 1 << 20, 1), (131072, 1 << 22, 1), (65536, 262144, 4)):
+        assert 0 < scratch(rows, length, batch) <= (1 << 30) + (1 << 24), (rows, length)
+    assert 0 <= scratch(65536, 131072) < 1 << 12  # 1024 pages: in LDS
+
+
+@gpu
+@pytest.mark.parametrize("pages,rows,heads", [(1100, [5300, 700], 24), (3000, [4000], 24)])
+def test_blocks_of_rows_that_share_a_place_for_their_scores(pages, rows, heads):
+    """More blocks of rows than workgroups of the gate."""
+    P, dim = 64, 16
+    lens = [P * pages - 3, P * 1040][:len(rows)]
+    cache, table, q, cu = setup(heads, 1, dim, P, rows, lens, torch.bfloat16, torch.int8)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    args = (torch.tensor(cu, **i32), max(rows), torch.tensor(lens, **i32), max(lens), torch.tensor(table, **i32), 4)
+    out, lse = flash_moba.flash_moba_cache_attn_func(q, cache, *args, return_lse=True)
+    s = R.state(cache)
+    for b, n in enumerate(rows):
+        for first in (0, n // 2 // 32 * 32, n - 33):  # some blocks of every stretch
+            t = slice(cu[b] + first, cu[b] + first + 33)
+            want, want_lse, _, sizes = R.attention(s, q[t].cpu(), [0, 33], [lens[b] - n + first + 33], [table[b]], 4)
+            check(out[t], lse[:, t], want, want_lse, sizes, True)
+    whole = out.clone()
+    assert torch.equal(whole, flash_moba.flash_moba_cache_attn_func(q, cache, *args))
