@@ -397,6 +397,7 @@ py::object cache_step(const py::handle &hq, const py::handle &hk, const py::hand
     const AttnForm attn{max_q, max_k, topk, scale, add_weight};
     cache_view(c);
     check_attn(q, c, attn);
+    require(k.dim() == 3 && k.size(0) == q.size(0), "q, k and v must be of the same tokens");
     check_inference({&k});
     if (turned) check_rotary(q, k, unpack(hp), f);
     // (the attention is checked, and has its memory, before the cache changes: a step that is refused can be made again)

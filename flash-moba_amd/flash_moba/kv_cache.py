@@ -145,6 +145,8 @@ def flash_moba_with_cache_func(q, k, v, cache, cu_seqlens_q, max_seqlen_q, seqle
                                                       sections or (), base, rotary_dim or 0, interleaved, softmax_scale, add_weight)
         if res is not None:
             return res if return_lse else res[0]
+    if q.shape[0] != k.shape[0]:
+        raise RuntimeError("q, k and v must be of the same tokens")
     if positions is not None:
         q, k = flash_moba_rotary_func(q, k, positions, sections, base, rotary_dim, interleaved)
     flash_moba_cache_append_func(cache, k, v, cu_seqlens_q, max_seqlen_q, seqlens_k, block_table)

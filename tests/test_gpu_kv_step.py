@@ -178,3 +178,18 @@ def test_blocks_of_rows_that_share_a_place_for_their_scores(pages, rows, heads):
             check(out[t], lse[:, t], want, want_lse, sizes, True)
     whole = out.clone()
     assert torch.equal(whole, flash_moba.flash_moba_cache_attn_func(q, cache, *args))
+
+
+@gpu
+@pytest.mark.parametrize("traced", [False, True])
+@pytest.mark.parametrize("positions", [False, True])
+def test_a_step_has_the_keys_of_its_queries(positions, traced):
+    """More or fewer keys than queries would be written at other positions than the queries have."""
+    cache, args, kw = step_inputs(1, 5, 4, 6, positions)
+    before = [t.clone() for t in cache]
+    for n in (4, 6):
+        k = torch.ones((n, 1, 16), device="cuda", dtype=torch.bfloat16)
+        step = torch.compile(flash_moba.flash_moba_with_cache_func, backend="aot_eager") if traced else flash_moba.flash_moba_with_cache_func
+        with pytest.raises(Exception, match="same tokens"):
+            step(args[0], k, k, *args[3:], **kw)
+    assert unchanged(cache, before)
