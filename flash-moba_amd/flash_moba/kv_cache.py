@@ -99,6 +99,10 @@ def flash_moba_cache_append_func(cache, k, v, cu_seqlens, max_seqlen, seqlens_k,
     448 (e4m3) or 127 (int8) at most; infinities are held as that, NaN as NaN (int8: 0).  Where a later token needs a larger scale, the
     page's earlier tokens are rounded again.  Places behind the end of a sequence, tokens before its beginning and table entries
     that are no page (outside [0, pages)) are left alone.  A page's first token starts its sum and its weight anew.
+
+    Tokens are taken back (drafts that were refused) by smaller lengths: what is appended next lies over them.  k_sum of a page that had
+    tokens before them still has them, though, as nothing says how many it has summed: put back what cache.k_sum[page] was before they
+    came, and append again those of them that stay.  (The page's scale stays as large as they made it.)
     """
     if not torch.compiler.is_compiling() and flash_moba_gpu.host_module().cache_append(cache, k, v, cu_seqlens, max_seqlen, seqlens_k, block_table):
         return

@@ -351,7 +351,8 @@ typedef struct {
 /* New keys and values (total_new, heads_k, head_dim) of the tokens seqlens_k[b] - n_b .. seqlens_k[b] - 1, n_b = cu_seqlens[b + 1] - cu_seqlens[b] <=
  * max_seqlen_new, rounded into their pages.  The scale of a (page, head) is the least power of two, from 2^-64 to 2^64, that brings the
  * largest finite magnitude to 448 or 127; values beyond are cut off there, NaN is kept (int8: 0).  Where a page has tokens already its scale
- * never shrinks, and where it grows the tokens there are rounded again.  A page that receives its first token starts with an empty sum and weight. */
+ * never shrinks, and where it grows the tokens there are rounded again.  A page that receives its first token starts with an empty sum and weight.
+ * k_sum counts every token once that it was given: where tokens are written over that a page had, the caller puts k_sum back to what it was before them. */
 typedef struct {
   fmoba_kv_cache cache;
   const void *k, *v;

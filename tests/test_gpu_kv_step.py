@@ -193,3 +193,43 @@ def test_a_step_has_the_keys_of_its_queries(positions, traced):
         with pytest.raises(Exception, match="same tokens"):
             step(args[0], k, k, *args[3:], **kw)
     assert unchanged(cache, before)
+
+
+@gpu
+@pytest.mark.parametrize("start,draft,stay", [(70, 4, 2), (62, 4, 1), (62, 6, 3), (64, 3, 0), (1, 1, 0)])
+@pytest.mark.parametrize("held", [torch.float8_e4m3fn, torch.int8])
+def test_drafts_that_were_refused_are_taken_back(held, start, draft, stay):
+    """Within a page, across a page's end, from a page's beginning: as if the refused tokens had never come."""
+    P, dim = 64, 32
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.tensor([[3, 0, 2]], **i32)
+    g = torch.Generator(device="cuda").manual_seed(start)
+    k, v, refused = (torch.rand((100, 2, dim), generator=g, device="cuda").bfloat16() + 1 for _ in range(3))
+    caches = [flash_moba.MobaKVCache.allocate(4, P, 2, dim, cache_dtype=held) for _ in range(2)]
+
+    def append(cache, k, v, length):
+        flash_moba.flash_moba_cache_append_func(cache, k, v, torch.tensor([0, len(k)], **i32), len(k), torch.tensor([length], **i32), table)
+
+    for cache in caches:
+        append(cache, k[:start], v[:start], start)
+    drafted, plain = caches
+    page = table[0, (start - 1) // P]
+    was = drafted.k_sum[page].clone()
+    append(drafted, torch.cat([k[start:start + stay], refused[:draft - stay]]), torch.cat([v[start:start + stay], refused[:draft - stay]]), start + draft)
+    drafted.k_sum[page] = was
+    if stay:
+        append(drafted, k[start:start + stay], v[start:start + stay], start + stay)
+        append(plain, k[start:start + stay], v[start:start + stay], start + stay)
+    for cache in caches:
+        append(cache, k[start + stay:start + stay + 9], v[start + stay:start + stay + 9], start + stay + 9)
+    end = start + stay + 9
+    for c in range((end + P - 1) // P):
+        n, at = min(P, end - c * P), table[0, c]
+        for name in ("k", "v"):
+            # the same, or at a scale that the refused ones enlarged: each is rounded once more at most, half a step of int8 or 2^-4 of it
+            a, b = ((getattr(cache, name)[at, :, :n].double(), getattr(cache, name + "_scale")[at].double()[:, None, None]) for cache in caches)
+            assert bool((a[1] >= b[1]).all())
+            step = torch.where(a[1] == b[1], 0.0, (b[1] + a[1] / 2).expand_as(a[0]) if held == torch.int8 else 3 * 2.0 ** -4 * a[0].abs() * a[1])
+            assert bool(((a[0] * a[1] - b[0] * b[1]).abs() <= step).all()), name
+        for name in ("k_sum", "k_mean"):
+            assert torch.equal(getattr(drafted, name)[at], getattr(plain, name)[at]), name
