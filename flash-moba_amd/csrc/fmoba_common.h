@@ -34,7 +34,7 @@ void set_error(const char *fmt, ...);
     }                                                                                \
   } while (0)
 
-static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+static inline int ceil_div(int a, int b) { return a > 0 ? (a - 1) / b + 1 : (a + b - 1) / b; }  // (a up to the largest)
 static inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------------------------

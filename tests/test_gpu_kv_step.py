@@ -44,6 +44,12 @@ def test_the_check_says_what_the_call_would():
     assert ok(batch=1, heads_k=64, heads=64, total_q=300000, max_seqlen_q=300000, max_seqlen_k=64 * 30000, max_pages=30000, topk=1) == 0
 
 
+def test_the_largest_length_is_a_length():
+    lib = H.load_library()
+    need = [lib.fmoba_cache_attn_workspace_bytes(ctypes.byref(attn_args(cache_struct(), total_q=4096, max_seqlen_q=4096, max_seqlen_k=n))) for n in (64 * 8, 2 ** 31 - 1)]
+    assert need[0] == need[1] > 0
+
+
 def step_inputs(batch, rows, heads, cols, positions):
     """Sequences of cols pages of 64, of which the table has the last page only."""
     P, dim = 64, 16
@@ -233,3 +239,18 @@ def test_drafts_that_were_refused_are_taken_back(held, start, draft, stay):
             assert bool(((a[0] * a[1] - b[0] * b[1]).abs() <= step).all()), name
         for name in ("k_sum", "k_mean"):
             assert torch.equal(getattr(drafted, name)[at], getattr(plain, name)[at]), name
+
+
+@gpu
+@pytest.mark.parametrize("rows,pages", [(2, 20), (1100, 20), (2, 2100), (1100, 1100)])
+def test_lengths_may_be_said_to_be_anything(rows, pages):
+    """max_seqlen_k (and max_seqlen_q) of 2^31 - 1, as a program that captures its steps once for all lengths says."""
+    P, dim, most = 64, 32, 2 ** 31 - 1
+    cache, table, q, cu = setup(2, 1, dim, P, [rows], [P * pages - 9], torch.bfloat16, torch.int8)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    args = torch.tensor(cu, **i32), torch.tensor([P * pages - 9], **i32), torch.tensor(table, **i32)
+    k, v = (torch.randn((rows, 1, dim), device="cuda").bfloat16() for _ in range(2))
+    twin = flash_moba.MobaKVCache(*[t.clone() for t in cache])
+    want, want_lse = flash_moba.flash_moba_with_cache_func(q, k, v, cache, args[0], rows, args[1], P * pages, args[2], 5, add_weight=True, return_lse=True)
+    out, lse = flash_moba.flash_moba_with_cache_func(q, k, v, twin, args[0], most, args[1], most, args[2], 5, add_weight=True, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and unchanged(cache, twin) and bool((want != 0).any())
