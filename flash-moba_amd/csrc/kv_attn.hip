@@ -87,10 +87,11 @@ static_assert(kRowWaves == 8, "64 groups of candidates: eight threads each");
 constexpr int kOwnScores = 2048;
 // Rows share pages where there are kColumnRowsLeast (row, head) pairs or more and a page is selected by kVisitsOwn of them on average, or by kVisits if the scores are a
 // launch of their own; else the form for many rows takes longer, for its three launches and for pages that few rows visit.  Visits of a page, us of the form for many rows and of this
-// one, heads of 128, 8 pages a row: 16 sequences of 2048 tokens, 16 heads, 4 rows each 2: 91, 34; 8 rows 4: 93, 62; 16 rows 8: 94, 117; of 32768 tokens, 32 over 8
-// heads, 32 rows 4: 551, 513; of 8192 8 rows 4: 160, 122; 16 rows 8: 165, 233; a sequence of 100000 tokens 64 rows 2.6: 140, 103; 128 rows 5.2: 150, 191; 256 rows 10: 156, 364;
-// with its own launch for the scores, four sequences of 300000, 32 rows 0.4: 1007, 391; 128 rows 1.7: 1293, 1465.  One row of each of 64
-// sequences, 32 heads over one, of 2048 tokens 16: 41, 70; of 8192 4: 91, 76.  Few pairs, 1536: 16 over 2 heads, 262 visits: 56, 49; 1024, 32 over 8 heads, 64: 30, 34; 2048, 16 heads, 16: 46, 61.
+// one, heads of 128, 8 pages of 128 a row: 16 sequences of 2048 tokens, 16 heads, 4 rows each 2: 93, 34; 8 rows 4: 94, 63; 16 rows 8: 97, 119; of 32768 tokens, 32 over 8
+// heads, 32 rows 4: 624, 525; of 8192 8 rows 4: 172, 124; 16 rows 8: 180, 236; a sequence of 100000 tokens 64 rows 2.6: 145, 104; 128 rows 5.2: 160, 193; 256 rows 10: 169, 367;
+// with its own launch for the scores, four sequences of 300000, 32 rows 0.4: 1072, 391; 128 rows 1.7: 1436, 1466.  One row of each of 64
+// sequences, 32 heads over one, of 2048 tokens 16: 41, 64; of 8192 4: 97, 77.  Few pairs, 1536: 16 over 2 heads, 384 visits: 51, 48; 1024, 32 over 8 heads, 64: 29, 34; 2048, 16 heads, 64: 30, 63.
+// (Averages over the sequences of a call: one with a few long parts of prompts and many single rows takes the row form.)
 constexpr int kColumnRowsLeast = 2048, kVisitsOwn = 5, kVisits = 2;
 constexpr int kPickAlone = 256;  // candidates that one wave chooses from (by the groups' cut 128 of them took 2 us longer)
 constexpr int kPickList = 512;  // candidates that are left when the cut of the groups is known, beyond which all are looked through again

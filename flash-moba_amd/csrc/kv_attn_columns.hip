@@ -375,11 +375,11 @@ __global__ __launch_bounds__(256) void cache_gate_kernel(ColumnPlan p, int page_
 }
 
 // ------------------------------------------------------------------------------------
-// columns: a workgroup of four waves keeps a page in LDS and takes 128 of its rows a turn, what a turn needs of memory on its way during the one before.  Products and softmax of a turn
-// would take a third of what it does: of a workgroup's 33 thousand clocks (1.9 turns a page) 16 thousand are gone before its first product, on lengths and table,
-// words of bits and the page, the rows, one after the other, and two waves a SIMD (254 registers) hide little of it.  2825 rows of three sequences of 9216 to 33000
-// tokens, 32 over 8 heads of 128: 155 us, 385 MB at 2.5 TB/s; 8191 rows, 16 heads: 147 us, 0.47 PFLOP/s.  (Two pages a workgroup, the second one's bytes on their way during the first one's last
-// turn, in the registers of the rows: 185 and 206.)
+// columns: a workgroup of four waves keeps a page in LDS and takes 128 of its rows a turn, what a turn needs of memory on its way during the one before.  2825 rows of three sequences of 9216 to 33000
+// tokens, 32 over 8 heads of 128: 171 us, 402 MB at 2.4 TB/s; 8191 rows, 16 heads: 167 us, 0.41 PFLOP/s.  Bound by latency: products and softmax of a turn would take a third of what it does; with one product a
+// weight (155 and 147 us), 16 of a workgroup's 33 thousand clocks (1.9 turns a page) were gone before its first product, on lengths and table, words of bits and the page, the rows, one
+// after the other, and two waves a SIMD (256 registers) hide little of it.  (Two pages a workgroup, the second one's bytes on their way during the first one's last turn, in the registers of the
+// rows, then: 185 and 206.)
 // ------------------------------------------------------------------------------------
 constexpr int kColumnRows = 128;  // of a turn: 32 a wave
 constexpr int kColumnWords = 128;  // words of bits that are spread out at a time: 32 a wave
@@ -891,7 +891,7 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   p.gates = (int)std::min<int64_t>((int64_t)p.row_blocks * a.heads * a.batch, std::max<int64_t>(kGateScores / gate_score_bytes(cols) / 256, 1) * 256);
   // Pages of one step (64 keys, or 128 of heads up to 128, whose scores of a row fit the registers): nothing before it has to be scaled for, and its next rows can be on their way.  Larger pages are
   // several columns of one step each, as far as the combine has places for a row's visits; else one column of many steps, whose keys come into LDS 64 at a time, again for every turn,
-  // where two workgroups do not find room for all.  (8191 tokens, 16 over 4 heads of 128, pages of 256 keys, four a row: 260 us in two steps, 526 in one column; of 512, two a row: 245 and 670;
+  // where two workgroups do not find room for all.  (Whole calls, with one product a weight: 8191 tokens, 16 over 4 heads of 128, pages of 256 keys, four a row: 260 us in two steps, 526 in one column; of 512, two a row: 245 and 670;
   // heads of 256, pages of 128, eight a row: 785 and 1013.)
   const int pages = std::min(a.topk, cols);
   p.step_keys = a.cache.head_dim <= 128 && a.cache.page_size % 128 == 0 ? 128 : 64;
@@ -899,7 +899,7 @@ static ColumnSizes column_sizes(const fmoba_cache_attn_args &a, int cols, Column
   if (pages * p.steps > kCombineSlots) p.steps = 1, p.step_keys = a.cache.page_size;
   p.slots = pages * p.steps;
   // Workgroups of a page: four turns of rows each, if rows choose evenly, and an odd number: the last ones of a late page, which few rows see, have nothing to
-  // do, and would otherwise come to the same shader engines for every page (8191 tokens, 16 heads: 223 us even, 201 odd; 8192, 16 over 2 heads: 380 and 254;
+  // do, and would otherwise come to the same shader engines for every page (whole calls, with one product a weight: 8191 tokens, 16 heads: 223 us even, 201 odd; 8192, 16 over 2 heads: 380 and 254;
   // 4 x 4096, 32 over 8 heads: two turns 778, three 751, four 745, six 740, twelve 779; 16384, 28 over 4 heads: 870, 902, 949, 1037, 1126).
   const int64_t visits = (int64_t)p.tiles * kTileRows * std::min(a.topk, cols) / cols;
   p.parts = (int)std::min<int64_t>(std::max<int64_t>(std::max<int64_t>(visits / (4 * kColumnRows), ceil_div(p.tiles, kColumnPart - 32)), 1), ceil_div(p.tiles, 32)) | 1;
@@ -942,7 +942,7 @@ static int launch_gate(const ColumnPlan &p, hipStream_t s) {
   while ((1 << page_bits) < p.c.cols) ++page_bits;
   auto kern = lds ? cache_gate_kernel<T, HD, true> : cache_gate_kernel<T, HD, false>;
   if (int rc = with_lds(kern, bytes, "cache_gate")) return rc;
-  // whole calls, us with one wave, two, four: 64 pages 270, 274, 293; 256 pages 124, 121, 127; 512 188, 169, 164; 1024 395, 320, 286
+  // whole calls (with one product a weight in the columns), us with one wave, two, four: 64 pages 270, 274, 293; 256 pages 124, 121, 127; 512 188, 169, 164; 1024 395, 320, 286
   const int waves = p.c.cols <= 64 ? 1 : p.c.cols <= 320 ? 2 : 4;
   hipLaunchKernelGGL(kern, grid, dim3(64 * waves), bytes, s, p, page_bits);
   FMOBA_LAUNCH_CHECK("cache_gate_kernel");
@@ -970,7 +970,7 @@ static int launch_columns(const ColumnPlan &p, hipStream_t s) {
 template <typename T, int LPR>
 static void launch_combine(const ColumnPlan &p, hipStream_t s) {
   const int64_t pairs = (int64_t)p.c.a.total_q * p.c.a.heads;
-  // Rows of a workgroup: fewer where there are few, more spare the weights' atomics.  Whole calls, us with 16, 32, 64, 128 rows, heads of 128 without weights and with: 2048 pairs 35, 38, 44, 56
+  // Rows of a workgroup: fewer where there are few, more spare the weights' atomics.  Whole calls (with one product a weight in the columns), us with 16, 32, 64, 128 rows, heads of 128 without weights and with: 2048 pairs 35, 38, 44, 56
   // and 40, 42, 50, 64; 8192 49, 51, 56, 68 and 62, 59, 61, 75; 32768 78, 76, 80, 87 and 117, 99, 91, 96; 131056 219, 213, 212, 213 and 277, 243, 229, 225.
   const int rows = std::max(pairs <= 4096 ? 16 : pairs <= 16384 ? 32 : 64, 256 / LPR);
   const dim3 grid(ceil_div(p.c.a.total_q, rows), p.c.a.heads);

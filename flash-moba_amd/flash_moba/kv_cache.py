@@ -141,7 +141,7 @@ def flash_moba_with_cache_func(q, k, v, cache, cu_seqlens_q, max_seqlen_q, seqle
                                return_lse=False):
     """A serving step end to end: rotary positions on q and k (with `positions`, as flash_moba_rotary_func), the keys and values of the
     tokens into the cache (as flash_moba_cache_append_func), attention of the tokens over it (as flash_moba_cache_attn_func).  An eager
-    call that is refused, for want of memory too, has left the cache as it was."""
+    call on ordinary tensors that is refused, for want of memory too, has left the cache as it was."""
     if positions is not None:
         positions, sections, rotary_dim = rotary_form(q, positions, sections, rotary_dim)
     if not torch.compiler.is_compiling():
