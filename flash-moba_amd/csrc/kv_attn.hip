@@ -491,7 +491,7 @@ extern "C" int fmoba_cache_attn_check(const fmoba_cache_attn_args *a) {
   FMOBA_REQUIRE(a->workspace_bytes >= need && (a->workspace || need == 0) && (uintptr_t)a->workspace % 256 == 0, "cache_attn: workspace too small (%zu < %zu) or not 256-byte aligned", a->workspace_bytes, need);
   const int cols = call_cols(*a);
   if (many_rows(*a, cols)) {
-    FMOBA_REQUIRE(column_grid_fits(*a, cols), "cache_attn: too many sequences times pages for the launch grid");
+    FMOBA_REQUIRE(column_grid_fits(*a, cols), "cache_attn: too many rows, or sequences times pages for the launch grid");
   } else {
     FMOBA_REQUIRE(rows_grid_fits(*a), "cache_attn: too many rows times heads for the launch grid");
     FMOBA_REQUIRE(scores_grid_fits(*a, cols), "cache_attn: too many rows, or sequences times heads, for the launch grid");

@@ -920,7 +920,8 @@ size_t column_workspace_bytes(const fmoba_cache_attn_args &a, int cols) {
 bool column_grid_fits(const fmoba_cache_attn_args &a, int cols) {
   ColumnPlan p{};
   column_sizes(a, cols, p);
-  return (int64_t)a.batch * a.cache.heads_k * cols * p.steps * p.parts * 256 <= UINT32_MAX;
+  // (gate: a block of rows; columns: a page; combine: 64 rows or more)
+  return (int64_t)a.batch * a.cache.heads_k * cols * p.steps * p.parts * 256 <= UINT32_MAX && (int64_t)p.row_blocks * 256 <= UINT32_MAX && ceil_div64(a.total_q, 64) * 256 <= UINT32_MAX;
 }
 
 template <typename K>

@@ -33,6 +33,7 @@ def test_the_check_says_what_the_call_would():
     assert ok() == 0 and ok(total_q=0) == 0
     for kw, message in [(dict(topk=65), b"moba_topk"), (dict(heads=3), b"divide"), (dict(workspace=4100), b"workspace"),
                         (dict(batch=8400, heads_k=1, heads=64, total_q=8400 * 16, max_seqlen_q=16, max_seqlen_k=64 * 2000, max_pages=2000), b"rows times heads for the launch grid"),
+                        (dict(batch=1, heads_k=1, heads=1, total_q=(1 << 30) + (1 << 20), max_seqlen_q=(1 << 30) + (1 << 20)), b"too many rows"),
                         (dict(batch=3000, heads_k=32, heads=32, total_q=3000, max_seqlen_q=1, max_seqlen_k=64 * 33000, max_pages=33000), b"sequences times heads, for the launch grid")]:
         assert ok(**kw) != 0, kw
         assert message in lib.fmoba_last_error(), (kw, lib.fmoba_last_error())
