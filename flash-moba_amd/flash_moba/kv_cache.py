@@ -160,7 +160,8 @@ def flash_moba_with_cache_func(q, k, v, cache, cu_seqlens_q, max_seqlen_q, seqle
 def flash_moba_cache_evict_func(weight, seqlens_k, block_table, page_size, keep_pages, sink_pages=1, recent_pages=1):
     """Which pages every sequence keeps when it has more than `keep_pages`: the first `sink_pages`, the last `recent_pages` (at
     least 1, the page that is being filled), and of the others those that received most attention weight (cache.weight, summed over
-    heads; of equals the first).  Sequences with fewer pages keep all.
+    heads; of equals the first).  Sequences with fewer pages keep all.  A table entry that is no page has no weight, and is
+    let go as it stands.
 
     Returns (block_table, seqlens_k, freed, num_freed): the table of the pages kept, in order, and -1 behind them; the tokens
     that are left; the pages let go in the same form, and how many they are.  The cache itself stays as it is: the freed pages can be given out again
